@@ -131,6 +131,153 @@ TVARA_API int tvara_paged_attention(const tvara_attention_args* args, void* work
 TVARA_API size_t tvara_paged_attention_noalloc_max(void);
 TVARA_API int tvara_paged_attention_noalloc(const tvara_attention_args* args, void* stream);
 
+/* ---- drafted-token trees over the paged KV cache ------------------------
+ *
+ * The reference verifies one chain of drafted tokens at a time (a
+ * tvara_sequence_decode_batch, then tvara_sequence_truncate;
+ * python/tvara/speculative.py:255-295).  These three calls verify a *tree* of
+ * drafted tokens per sequence for a batch of sequences, with every length,
+ * table and choice on the device: nothing is copied to or from the host, the
+ * launches are asynchronous on `stream`, and all three can be captured into a
+ * CUDA graph.  A step is
+ *   tvara_tree_plan       blocks, slots, positions and masks of the drafts,
+ *   (per layer)           the drafts' K and V written to their slots, then
+ *   tvara_tree_attention  every draft over its sequence's cache and ancestors,
+ *   tvara_tree_commit     the walk along the model's choices; accepted rows
+ *                         move to where the sequence continues.
+ *
+ * Shared conventions.  Sequence s has lengths[s] cached positions and drafts
+ * the rows [cu_nodes[s], cu_nodes[s+1]) of the flat row arrays, its nodes
+ * (none is allowed); cu_nodes has n_seq + 1 entries, the first 0.  Node i's
+ * parent is a node of the same sequence with a smaller index, or -1 for a
+ * child of the last cached position.  The row arrays have room for `capacity`
+ * rows; rows from cu_nodes[n_seq] on are neither read nor written.  A slot is
+ * block * block_tokens + offset in the pool layout described above.  Table
+ * row s starts at tables + s * table_stride.  At most 8192 sequences and 1024
+ * nodes a sequence (max_nodes, the width the ancestor masks are laid out for:
+ * ceil(max_nodes / 64) words a row).
+ *
+ * What the host can check is refused as by the calls above.  What only the
+ * device sees sets bits of *status (device, one word, never cleared by these
+ * calls: zero it once and look when convenient), and nothing outside the
+ * caller's arrays is touched. */
+enum {
+    TVARA_TREE_BAD_BLOCK = 1,   /* a block id or slot outside the pool; its row is not read or written (in the
+                                   attention it counts as masked) */
+    TVARA_TREE_BAD_LENGTHS = 2, /* negative or decreasing cu_nodes, more rows than capacity, more nodes than
+                                   max_nodes, a negative length, a sequence longer than its table row, a count of
+                                   free blocks outside [0, free_capacity], or held blocks that are fewer than the
+                                   cached positions need: the plan writes nothing, the other calls skip the
+                                   sequence */
+    TVARA_TREE_NO_BLOCKS = 4,   /* the plan needs more blocks than are free: it writes nothing */
+    TVARA_TREE_BAD_PARENT = 8,  /* a parent that is not an earlier node: the plan treats the node as a root, the
+                                   commit never accepts it */
+    TVARA_TREE_TIMEOUT = 16     /* a bounded wait inside the attention ran out: its output is incomplete */
+};
+
+/* Block tables, slot maps, positions and ancestor masks of a step from the
+ * request lengths (for trees, and with parents NULL for prompt chunks or
+ * plain appends, where a sequence's rows are consecutive positions).
+ * Sequence s holds held[s] blocks in its table row.  If its lengths[s] + n
+ * positions need more, blocks are taken from the end of the free list,
+ * free_blocks[*free_count - 1] first, in sequence order, and appended to the
+ * row; row i gets the slot of position lengths[s] + i.  positions[i] is
+ * lengths[s] + depth of node i (roots have depth 0) and bit j of row i of
+ * ancestors says that node j is node i or one of its ancestors.  held_out and
+ * free_left may be held and free_count themselves; the free list is only
+ * read, its first *free_left entries stay free. */
+typedef struct tvara_tree_plan_args {
+    uint32_t struct_size;         /* sizeof(tvara_tree_plan_args) */
+    uint32_t block_tokens;
+    size_t n_seq, capacity, max_nodes, max_blocks, table_stride, free_capacity;
+    const int32_t* lengths;       /* device [n_seq] */
+    const int32_t* held;          /* device [n_seq] */
+    const int32_t* cu_nodes;      /* device [n_seq + 1] */
+    const int32_t* parents;       /* device [capacity], or NULL: rows are consecutive positions, any number of
+                                     them (max_nodes is not looked at) */
+    const int32_t* free_blocks;   /* device [free_capacity]; may be NULL if free_capacity is 0 */
+    const int32_t* free_count;    /* device, one entry */
+    int32_t* tables;              /* device [n_seq][table_stride], appended to */
+    int64_t* slots;               /* out, device [capacity] */
+    int32_t* positions;           /* out, device [capacity] */
+    uint64_t* ancestors;          /* out, device [capacity][ceil(max_nodes / 64)]; with parents only (else NULL) */
+    int32_t* held_out;            /* out, device [n_seq] */
+    int32_t* free_left;           /* out, device, one entry */
+    int32_t* status;              /* device, one word */
+} tvara_tree_plan_args;
+TVARA_API int tvara_tree_plan(const tvara_tree_plan_args* args, void* stream);
+
+/* Attention of drafted tokens over a paged cache: row i of sequence s attends
+ * to the cached positions [0, lengths[s]) through the table row of s and to
+ * the nodes j of its sequence whose bit is set in row i of ancestors (any
+ * mask; NULL: j <= i, a chain), their K and V at slots[cu_nodes[s] + j].
+ * Scores are q.k / sqrt(head_dim), query head h reads KV head
+ * h / (heads / kv_heads), arithmetic and outputs are F32 to within rounding
+ * for every pool type (as tvara_paged_attention).  A row that attends to
+ * nothing is zero; masked K and V may hold anything, NaN included.  One
+ * workspace serves one call at a time. */
+typedef struct tvara_tree_attention_args {
+    uint32_t struct_size;         /* sizeof(tvara_tree_attention_args) */
+    uint32_t kv_dtype;            /* TVARA_KV_F32, TVARA_KV_F16 or TVARA_KV_I8 (needs kv_scales) */
+    uint32_t heads, kv_heads, head_dim, block_tokens; /* head_dim 1..256 */
+    uint32_t layers, layer;
+    size_t n_seq, capacity, max_nodes, max_blocks, table_stride;
+    size_t q_stride, out_stride;  /* elements from row to row, at least heads * head_dim */
+    const float* q;               /* device [capacity][q_stride] */
+    float* out;                   /* device [capacity][out_stride] */
+    const void* pool;             /* device KV pool */
+    const float* kv_scales;       /* TVARA_KV_I8: device row scales (element offset / head_dim) */
+    const int32_t* tables;        /* device [n_seq][table_stride] */
+    const int32_t* lengths;       /* device [n_seq] */
+    const int32_t* cu_nodes;      /* device [n_seq + 1] */
+    const int64_t* slots;         /* device [capacity] */
+    const uint64_t* ancestors;    /* device [capacity][ceil(max_nodes / 64)], or NULL */
+    int32_t* status;              /* device, one word */
+} tvara_tree_attention_args;
+/* Device scratch (bytes) for these sizes; 0 with an error for invalid ones. */
+TVARA_API size_t tvara_tree_attention_workspace(const tvara_tree_attention_args* args);
+TVARA_API int tvara_tree_attention(const tvara_tree_attention_args* args, void* workspace, size_t workspace_bytes,
+                                   void* stream);
+
+/* Acceptance and commit.  choices[i] is the token the model chose after node
+ * i (its argmax, or a draw from its distribution: accepting the drafts that
+ * equal such choices keeps the model's distribution), first[s] the one after
+ * the last cached position.  The walk starts at the last cached position with
+ * first[s]; it goes to the child whose token equals the choice (the lowest
+ * index if several do) and on with that child's choice, until no child
+ * matches.  With first NULL, node 0 is accepted as it is (the token already
+ * emitted, its K and V not yet in the cache).  path[cu_nodes[s] + k] is the
+ * k-th accepted node, -1 behind the last; accepted[s] counts them; next[s] is
+ * the choice the walk ended with (0xFFFFFFFF when there is none);
+ * lengths_out[s] = lengths[s] + accepted[s], and may be lengths itself.
+ * With a pool, the K and V rows of the k-th accepted node (every layer and KV
+ * head, int8 scales too) are copied from its slot to dest[cu_nodes[s] + k];
+ * dest NULL means slots: the drafts were written behind the cached positions,
+ * and the accepted ones close up in place.  Other dest slots must not be
+ * slots of drafted rows of this call, and no two rows may share one. */
+typedef struct tvara_tree_commit_args {
+    uint32_t struct_size;         /* sizeof(tvara_tree_commit_args) */
+    uint32_t kv_dtype;            /* TVARA_KV_F32, TVARA_KV_F16 or TVARA_KV_I8 (needs kv_scales) */
+    uint32_t kv_heads, head_dim, block_tokens, layers;
+    size_t n_seq, capacity, max_nodes, max_blocks;
+    const int32_t* lengths;       /* device [n_seq] */
+    const int32_t* cu_nodes;      /* device [n_seq + 1] */
+    const int32_t* parents;       /* device [capacity] */
+    const uint32_t* tokens;       /* device [capacity] drafted token of each node */
+    const uint32_t* choices;      /* device [capacity]; 0xFFFFFFFF matches nothing */
+    const uint32_t* first;        /* device [n_seq], or NULL */
+    const int64_t* slots;         /* device [capacity]; with a pool */
+    const int64_t* dest;          /* device [capacity], or NULL */
+    void* pool;                   /* device KV pool, or NULL: nothing moves */
+    float* kv_scales;             /* TVARA_KV_I8: device row scales */
+    int32_t* path;                /* out, device [capacity] */
+    int32_t* accepted;            /* out, device [n_seq] */
+    uint32_t* next;               /* out, device [n_seq] */
+    int32_t* lengths_out;         /* out, device [n_seq] */
+    int32_t* status;              /* device, one word */
+} tvara_tree_commit_args;
+TVARA_API int tvara_tree_commit(const tvara_tree_commit_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

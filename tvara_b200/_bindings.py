@@ -126,6 +126,10 @@ SIGNATURES = {
     "tvara_paged_attention": (C.c_int, [P, P, SZ, P]),
     "tvara_paged_attention_noalloc_max": (SZ, []),
     "tvara_paged_attention_noalloc": (C.c_int, [P, P]),
+    "tvara_tree_plan": (C.c_int, [P, P]),
+    "tvara_tree_attention_workspace": (SZ, [P]),
+    "tvara_tree_attention": (C.c_int, [P, P, SZ, P]),
+    "tvara_tree_commit": (C.c_int, [P, P]),
 }
 
 
@@ -151,6 +155,36 @@ class AttentionArgs(C.Structure):
         ("visible", C.c_void_p),
         ("kv_scales", C.c_void_p),
     ]
+
+
+class TreePlanArgs(C.Structure):
+    """include/tvara_kernels.h tvara_tree_plan_args."""
+    _fields_ = [("struct_size", C.c_uint32), ("block_tokens", C.c_uint32)] + [
+        (name, C.c_size_t) for name in ("n_seq", "capacity", "max_nodes", "max_blocks", "table_stride",
+                                        "free_capacity")] + [
+        (name, C.c_void_p) for name in ("lengths", "held", "cu_nodes", "parents", "free_blocks", "free_count",
+                                        "tables", "slots", "positions", "ancestors", "held_out", "free_left",
+                                        "status")]
+
+
+class TreeAttentionArgs(C.Structure):
+    """include/tvara_kernels.h tvara_tree_attention_args."""
+    _fields_ = [(name, C.c_uint32) for name in ("struct_size", "kv_dtype", "heads", "kv_heads", "head_dim",
+                                                "block_tokens", "layers", "layer")] + [
+        (name, C.c_size_t) for name in ("n_seq", "capacity", "max_nodes", "max_blocks", "table_stride", "q_stride",
+                                        "out_stride")] + [
+        (name, C.c_void_p) for name in ("q", "out", "pool", "kv_scales", "tables", "lengths", "cu_nodes", "slots",
+                                        "ancestors", "status")]
+
+
+class TreeCommitArgs(C.Structure):
+    """include/tvara_kernels.h tvara_tree_commit_args."""
+    _fields_ = [(name, C.c_uint32) for name in ("struct_size", "kv_dtype", "kv_heads", "head_dim", "block_tokens",
+                                                "layers")] + [
+        (name, C.c_size_t) for name in ("n_seq", "capacity", "max_nodes", "max_blocks")] + [
+        (name, C.c_void_p) for name in ("lengths", "cu_nodes", "parents", "tokens", "choices", "first", "slots",
+                                        "dest", "pool", "kv_scales", "path", "accepted", "next", "lengths_out",
+                                        "status")]
 
 
 def declare(lib) -> None:

@@ -11,6 +11,7 @@
 
 #include "attention_plan.hpp"
 #include "kernels.cuh"
+#include "tree.cuh"
 
 namespace tvara {
 std::string& last_error();
@@ -331,6 +332,184 @@ int tvara_paged_attention(const tvara_attention_args* a, void* workspace, size_t
         if (word == 2) throw std::runtime_error("paged attention read a block id outside the KV pool");
         if (word) throw std::runtime_error("paged attention timed out waiting for a KV copy (error " +
                                            std::to_string(word) + ")");
+    });
+}
+
+}  // extern "C"
+
+// ------------------------------------------------- drafted-token trees
+namespace {
+
+// Sizes shared by the three calls.
+void check_tree_sizes(std::size_t n_seq, std::size_t capacity, std::size_t max_nodes, std::size_t max_blocks,
+                      std::size_t block_tokens) {
+    if (!n_seq || n_seq > std::size_t(tvara::kTreeMaxSeq)) throw std::invalid_argument("trees take 1 to 8192 sequences");
+    if (capacity > 0x7fffffff) throw std::invalid_argument("invalid tree row capacity");
+    if (!max_nodes || max_nodes > std::size_t(tvara::kTreeMaxNodes))
+        throw std::invalid_argument("trees hold 1 to 1024 nodes");
+    if (!max_blocks || max_blocks > 0x7fffffff || !block_tokens || block_tokens > (1u << 20))
+        throw std::invalid_argument("invalid KV pool size");
+}
+
+bool overlap(const void* a, std::size_t na, const void* b, std::size_t nb) {
+    const auto x = reinterpret_cast<std::uintptr_t>(a), y = reinterpret_cast<std::uintptr_t>(b);
+    return x < y + nb && y < x + na;
+}
+
+tvara::TreeAttn tree_attention_job(const tvara_tree_attention_args* a) {
+    if (!a || a->struct_size < sizeof(tvara_tree_attention_args))
+        throw std::invalid_argument("invalid tree attention arguments");
+    check_tree_sizes(a->n_seq, a->capacity, a->max_nodes, a->max_blocks, a->block_tokens);
+    if (a->kv_dtype > TVARA_KV_I8) throw std::invalid_argument("invalid KV dtype or missing int8 scales");
+    if (!a->heads || !a->kv_heads || a->heads % a->kv_heads || !a->layers || a->layer >= a->layers ||
+        a->heads > 65535 || a->layers > 65535 || !a->head_dim || a->head_dim > 256 || !a->table_stride ||
+        a->table_stride > 0x7fffffff)
+        throw std::invalid_argument("invalid attention geometry");
+    const std::size_t width = std::size_t(a->heads) * a->head_dim;
+    if (a->q_stride < width || a->out_stride < width || a->q_stride > 0x7fffffff || a->out_stride > 0x7fffffff)
+        throw std::invalid_argument("query and output rows are shorter than heads * head_dim");
+    tvara::TreeAttn j;
+    j.kv_kind = a->kv_dtype == TVARA_KV_F32 ? 0 : a->kv_dtype == TVARA_KV_F16 ? 1 : 2;
+    j.hq = int(a->heads);
+    j.hkv = int(a->kv_heads);
+    j.dim = int(a->head_dim);
+    j.bt = int(a->block_tokens);
+    j.n_seq = int(a->n_seq);
+    j.capacity = int(a->capacity);
+    j.max_nodes = int(a->max_nodes);
+    j.words = int((a->max_nodes + 63) / 64);
+    j.max_blocks = int(a->max_blocks);
+    j.stride = int(a->table_stride);
+    j.ldq = (long long)a->q_stride;
+    j.ldo = (long long)a->out_stride;
+    j.kind_stride = (long long)a->kv_heads * a->block_tokens * a->head_dim;
+    j.layer_offset = (long long)a->layer * 2 * j.kind_stride;
+    j.block_stride = (long long)a->layers * 2 * j.kind_stride;
+    j.q = a->q;
+    j.out = a->out;
+    j.kv = a->pool;
+    j.scales = j.kv_kind == 2 ? a->kv_scales : nullptr;
+    j.tables = a->tables;
+    j.lengths = a->lengths;
+    j.cu = a->cu_nodes;
+    j.slots = reinterpret_cast<const long long*>(a->slots);
+    j.ancestors = reinterpret_cast<const unsigned long long*>(a->ancestors);
+    j.status = a->status;
+    return j;
+}
+
+}  // namespace
+
+extern "C" {
+
+int tvara_tree_plan(const tvara_tree_plan_args* a, void* stream) {
+    return guarded([&] {
+        if (!a || a->struct_size < sizeof(tvara_tree_plan_args))
+            throw std::invalid_argument("invalid tree plan arguments");
+        // without parents there are no masks and rows of any number follow one another
+        const std::size_t max_nodes = a->parents ? a->max_nodes : 1;
+        check_tree_sizes(a->n_seq, a->capacity, max_nodes, a->max_blocks, a->block_tokens);
+        if (!a->lengths || !a->held || !a->cu_nodes || !a->free_count || !a->tables || !a->held_out || !a->free_left ||
+            !a->status || (a->capacity && (!a->slots || !a->positions)) || (a->free_capacity && !a->free_blocks))
+            throw std::invalid_argument("invalid tree plan arguments");
+        if (a->capacity && !a->parents != !a->ancestors)
+            throw std::invalid_argument("parents and ancestor masks go together");
+        if (!a->table_stride || a->table_stride > 0x7fffffff || a->free_capacity > 0x7fffffff)
+            throw std::invalid_argument("invalid block table width or free list");
+        const std::size_t counts = a->n_seq * 4;
+        if ((a->held_out != a->held && overlap(a->held_out, counts, a->held, counts)) ||
+            overlap(a->held_out, counts, a->lengths, counts) || overlap(a->free_left, 4, a->held, counts) ||
+            overlap(a->held_out, counts, a->free_count, 4))
+            throw std::invalid_argument("plan outputs overlap its inputs");
+        tvara::TreePlan j;
+        j.bt = int(a->block_tokens);
+        j.n_seq = int(a->n_seq);
+        j.capacity = int(a->capacity);
+        j.max_nodes = int(max_nodes);
+        j.words = int((max_nodes + 63) / 64);
+        j.max_blocks = int(a->max_blocks);
+        j.stride = int(a->table_stride);
+        j.free_capacity = int(a->free_capacity);
+        j.lengths = a->lengths;
+        j.held = a->held;
+        j.cu = a->cu_nodes;
+        j.parents = a->parents;
+        j.free_blocks = a->free_blocks;
+        j.free_count = a->free_count;
+        j.tables = a->tables;
+        j.slots = reinterpret_cast<long long*>(a->slots);
+        j.positions = a->positions;
+        j.ancestors = reinterpret_cast<unsigned long long*>(a->ancestors);
+        j.held_out = a->held_out;
+        j.free_left = a->free_left;
+        j.status = a->status;
+        tvara::launch_tree_plan(j, static_cast<cudaStream_t>(stream));
+    });
+}
+
+size_t tvara_tree_attention_workspace(const tvara_tree_attention_args* a) {
+    std::size_t n = 0;
+    if (guarded([&] { n = tvara::tree_attention_workspace(tree_attention_job(a)); })) return 0;
+    return n;
+}
+
+int tvara_tree_attention(const tvara_tree_attention_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+    return guarded([&] {
+        const tvara::TreeAttn j = tree_attention_job(a);
+        if (!a->tables || !a->lengths || !a->cu_nodes || !a->status || !a->pool ||
+            (a->capacity && (!a->q || !a->out || !a->slots)))
+            throw std::invalid_argument("invalid tree attention arguments");
+        if (a->kv_dtype == TVARA_KV_I8 && !a->kv_scales)
+            throw std::invalid_argument("invalid KV dtype or missing int8 scales");
+        if (!workspace || workspace_bytes < tvara::tree_attention_workspace(j))
+            throw std::invalid_argument("attention workspace too small");
+        if (!a->capacity) return;
+        tvara::launch_tree_attention(j, workspace, static_cast<cudaStream_t>(stream));
+    });
+}
+
+int tvara_tree_commit(const tvara_tree_commit_args* a, void* stream) {
+    return guarded([&] {
+        if (!a || a->struct_size < sizeof(tvara_tree_commit_args))
+            throw std::invalid_argument("invalid tree commit arguments");
+        check_tree_sizes(a->n_seq, a->capacity, a->max_nodes, a->pool ? a->max_blocks : 1, a->pool ? a->block_tokens : 1);
+        if (!a->lengths || !a->cu_nodes || !a->accepted || !a->next || !a->lengths_out || !a->status ||
+            (a->capacity && (!a->parents || !a->tokens || !a->choices || !a->path)))
+            throw std::invalid_argument("invalid tree commit arguments");
+        tvara::TreeCommit j;
+        if (a->pool) {
+            if (a->kv_dtype > TVARA_KV_I8 || (a->kv_dtype == TVARA_KV_I8 && !a->kv_scales))
+                throw std::invalid_argument("invalid KV dtype or missing int8 scales");
+            if (!a->kv_heads || !a->head_dim || !a->layers || a->kv_heads > 65535 || a->layers > 65535 ||
+                a->head_dim > 65535 || std::uint64_t(a->kv_heads) * a->layers * a->head_dim > (1u << 28) ||
+                (a->capacity && !a->slots))
+                throw std::invalid_argument("invalid tree commit geometry");
+            j.elem = a->kv_dtype == TVARA_KV_F32 ? 4 : a->kv_dtype == TVARA_KV_F16 ? 2 : 1;
+            j.hkv = int(a->kv_heads);
+            j.dim = int(a->head_dim);
+            j.bt = int(a->block_tokens);
+            j.layers = int(a->layers);
+            j.max_blocks = int(a->max_blocks);
+            j.pool = a->pool;
+            j.scales = a->kv_dtype == TVARA_KV_I8 ? a->kv_scales : nullptr;
+            j.slots = reinterpret_cast<const long long*>(a->slots);
+            j.dest = reinterpret_cast<const long long*>(a->dest);
+        }
+        j.n_seq = int(a->n_seq);
+        j.capacity = int(a->capacity);
+        j.max_nodes = int(a->max_nodes);
+        j.lengths = a->lengths;
+        j.cu = a->cu_nodes;
+        j.parents = a->parents;
+        j.tokens = a->tokens;
+        j.choices = a->choices;
+        j.first = a->first;
+        j.path = a->path;
+        j.accepted = a->accepted;
+        j.next = a->next;
+        j.lengths_out = a->lengths_out;
+        j.status = a->status;
+        tvara::launch_tree_commit(j, static_cast<cudaStream_t>(stream));
     });
 }
 
