@@ -603,7 +603,7 @@ def test_speculative_steps_equal_the_plain_continuation(capi, kv):
             mask = np.concatenate([np.ones((n, len(k_rows)), bool), T.ancestors(parents[r])], 1)
             k = np.concatenate([np.array(k_rows).reshape(-1, kv_heads, d), real[r, 0]]).transpose(1, 0, 2)
             v = np.concatenate([np.array(v_rows).reshape(-1, kv_heads, d), real[r, 1]]).transpose(1, 0, 2)
-            o, tol = T.attention(q[r].reshape(n, heads, d), k, v, mask, heads // kv_heads)
+            o, tol = T.attention(q[r].reshape(n, heads, d), k, v, mask, heads // kv_heads, kv == "f32")
             assert (np.abs(out[r].reshape(n, heads, d) - o) <= tol).all()
             logits = o.reshape(n, -1) @ head_h
             # the device's choice is the largest logit, up to rounding of a near tie

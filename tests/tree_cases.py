@@ -85,7 +85,7 @@ def walk(parents, tokens, choices, first):
     return path, want
 
 
-def attention(q, k, v, mask, group):
+def attention(q, k, v, mask, group, split=False):
     """Softmax attention in 64 bits: q [n, heads, d], k and v [kv_heads, m, d],
     mask [n, m].  Returns the rows and a bound on the rounding of an F32
     evaluation.  The bound: a score is 2 d/16 + 1 truncating F32 additions of
@@ -94,7 +94,16 @@ def attention(q, k, v, mask, group):
     2^-22 of the exponential; the weighted sum adds 24 additions' 2^-23; and a
     weight carries an absolute 2^-24 of the row's largest, of either sign,
     which over m terms adds up like a random walk (six deviations of
-    sqrt(m) 2^-25)."""
+    sqrt(m) 2^-25).
+
+    split: K and V are F32 and enter as two F16 parts, hi a multiple of 16 and
+    lo at most 8 for a row whose largest value lies in [2^14, 2^15).  lo rounds
+    by at most 2^-9, so an element is off by 2^-23 of its row's largest: a
+    score by 2^-23 kmax sum|q|, an output by 2^-23 of the weighted row maxima.
+    The lo x lo products are left out: q_lo k_lo is the product of two values
+    uniform within 2^-11 of the rows' largest, over d terms six deviations are
+    6 sqrt(d) (2^-11)^2 / 3; p_lo v_lo likewise with p_lo within 2^-12 of the
+    row's largest weight: 6 sqrt(m) 2^-12 2^-11 / 3."""
     n, heads, d = q.shape
     q, k, v = (x.astype(np.float64) for x in (q, k, v))
     out = np.zeros((n, heads, d))
@@ -112,8 +121,14 @@ def attention(q, k, v, mask, group):
             w /= w.sum()
             out[i, h] = w @ vs
             e = (2 * -(-d // 16) + 1) * 2.0 ** -23 * size.max()
+            if split:
+                kmax, qmax = np.abs(ks).max(), np.abs(q[i, h]).max()
+                e += (2.0 ** -23 * kmax * np.abs(q[i, h]).sum() + 2 * np.sqrt(d) * 2.0 ** -22 * qmax * kmax) / np.sqrt(d)
             tol[i, h] = (w @ np.abs(vs)) * (2 * e + 2.0 ** -22 + 24 * 2.0 ** -23) \
                 + 6 * np.sqrt(len(vs)) * 2.0 ** -25 * np.abs(vs).max(0) + 1e-30
+            if split:
+                row = np.abs(vs).max(1)
+                tol[i, h] += 2.0 ** -23 * (w @ row) + 2 * np.sqrt(len(vs)) * 2.0 ** -23 * row.max()
     return out, tol
 
 
@@ -246,7 +261,8 @@ class AttentionCase:
                 continue
             r = slice(self.cu[s], self.cu[s + 1])
             q = self.q[r, :width].reshape(n, self.heads, self.d)
-            o, t = attention(q, self.k[s], self.v[s], self.mask[s], self.heads // self.kv_heads)
+            o, t = attention(q, self.k[s], self.v[s], self.mask[s], self.heads // self.kv_heads,
+                             self.kv == "f32")
             out[r, :width], tol[r, :width] = o.reshape(n, width), t.reshape(n, width)
         return out, tol
 

@@ -9,6 +9,7 @@
 
 #include <cuda_fp16.h>
 
+#include "split.cuh"
 #include "tree.cuh"
 
 namespace tvara {
@@ -23,7 +24,7 @@ __device__ __forceinline__ bool tree_sequence_ok(const TreeAttn& a, int s, int& 
     const long long rows = (long long)c1 - c0;
     n = int(rows);
     return c0 >= 0 && rows >= 0 && rows <= a.max_nodes && c1 <= a.capacity && len >= 0 &&
-           len <= (long long)a.stride * a.bt;
+           len <= (long long)a.stride * a.bt && len <= 0x7fffffff - kTreeMaxNodes;
 }
 
 // Element offset of the K row (head 0 of the layer) of index p of a sequence
@@ -142,11 +143,1188 @@ __global__ void __launch_bounds__(kAnyWarps * 32) tree_any_kernel(TreeAttn a) {
     if (flags && lane == 0) atomicOr(a.status, flags);
 }
 
+// ------------------------------------------------------- tensor cores
+// head_dim up to 128 (rows of a multiple of 16 bytes), any block size.
+//
+// A work item is (sequence, KV head, group of query vectors): its n drafted
+// rows times the G query heads that share the KV head, up to 128 vectors on
+// the M dimension of a tcgen05.mma (256 as two M tiles for F16 pools).  The
+// L + n keys are walked in tiles of kBn positions; a tile may hold cached
+// positions and nodes, since every row of it is fetched by its own address
+// (block table or slot map), so any block size and slot order costs the same.
+//   S  = Q K^T   per tile into tensor memory,
+//   P  = 2^(S c - m + 11) by the softmax warps, one thread per query vector
+//        (no shuffles), written back over S as the A operand,
+//   Ot = P V     per tile into tensor memory, added to the thread's F32 row
+//        O = O 2^(m_old - m) + Ot in registers.
+// The tensor core's own F32 accumulation truncates, so it is kept to one
+// tile (the small lo products first) and the long sum over tiles is rounded
+// to nearest in registers; that costs one fused multiply-add per element.
+// F32 results from F16 operands: Q, P (and K, V of F32 pools) enter as exact
+// hi + lo F16 pairs of about 22 bits (split.cuh), int8 codes are exact in
+// F16; scales of int8 rows, and the powers of two that bring an F32 row below
+// 2^15, are applied to S columns and to P.
+//
+// Two softmax warpgroups ("streams") keep the tensor core busy: with one M
+// tile they take the even and the odd tiles of the same item, each with its
+// own O, m and l, merged through tensor memory at the end; with two M tiles
+// each owns one and every K/V tile is used twice.
+//
+// Work is dealt to one CTA per SM in equal runs of tiles over all items
+// (each CTA scans the lengths and cuts out its run), so ragged batches and a
+// single long sequence fill the device alike; an item cut by a run boundary
+// leaves partial (O, m, l) in the workspace for tree_combine_kernel.
+constexpr int kTreeThreads = 512;   // WG0, WG1 softmax; WG2 loads; WG3 warp 12 issues the MMAs
+constexpr int kTreeMmaWarp = 12;
+constexpr int kTreeLoadWarp = 8;
+constexpr unsigned kTreeSpin = 1u << 22;
+constexpr int kTreeRows = 256;      // query vectors of a partial slot
+constexpr int kMetaRing = 8;        // tiles of column masks and int8 scales kept
+
+template <int KV, int DP>
+struct TreeForm {  // KV: 0 F32, 1 F16, 2 int8
+    static constexpr bool kPairs = KV == 1;              // two M tiles per item
+    static constexpr int kBn = KV == 0 ? 64 : 128;       // positions per tile
+    static constexpr int kParts = KV == 0 ? 2 : 1;       // hi, lo planes of K and V
+    static constexpr int kHalves = DP / 64;              // 128-byte wide column halves
+    static constexpr int kQPart = kHalves * 128 * 128;   // bytes of one Q plane
+    static constexpr int kQTile = 2 * kQPart;
+    static constexpr int kSlotPart = kHalves * kBn * 128;
+    static constexpr int kSlot = kParts * kSlotPart;     // one K or V tile
+    static constexpr int kElem = KV == 0 ? 4 : KV == 1 ? 2 : 1;
+    static constexpr int kRaw = KV == 1 ? 0 : kBn * DP * kElem;  // one unconverted tile
+    static constexpr int kRawDepth = KV == 1 ? 0 : DP == 64 ? 4 : KV == 0 ? 2 : 3;
+    static constexpr int kBase = KV == 1 ? (DP == 64 ? 6 : 3) : (DP == 64 ? 4 : 3);  // ring slots
+    static constexpr int kExtra = kPairs ? 2 : 0;        // more of them in the second Q tile when it is not used
+    static constexpr int kScaleRing = KV == 1 ? 0 : KV == 2 ? kMetaRing : 4;
+    static constexpr int kOffSlots = kQTile * (kPairs ? 2 : 1);
+    static constexpr int kOffRaw = kOffSlots + kBase * kSlot;
+    static constexpr int kOffScale = kOffRaw + kRawDepth * kRaw;
+    static constexpr int kOffMeta = kOffScale + kScaleRing * 2 * kBn * 4;
+    static constexpr int kSmem = kOffMeta + 1024;
+    static_assert(kExtra * kSlot <= kQTile || !kPairs);
+    static_assert(kSmem <= 232448);
+};
+
+struct TreeMeta {  // at kOffMeta
+    std::uint64_t full[8], empty[8];
+    std::uint64_t s_full[2], p_full[2], o_full[2];
+    std::uint64_t v_ready[kMetaRing];  // a tile's V scales are in place (F32, int8)
+    std::uint64_t q_full, item_done, merge_ready, merge_read, drain;
+    alignas(16) unsigned valid[kMetaRing][4];   // columns of a tile that hold a row
+    alignas(16) float vmax[kMetaRing][4];       // largest V scale per load warp
+    int vbad[16];                   // an item's nodes hold a non-finite V
+    long long warp_sum[16];
+    long long total, excl0, excl1;
+    int seq0, seq1;
+    unsigned tmem;
+    int abort_flag;
+    int bad;
+};
+static_assert(sizeof(TreeMeta) <= 1024);
+
+struct TreeRec {  // an item that continues in the next CTAs, by the CTA it starts in
+    int c0, row0, rows, split, head, pieces;
+};
+
+__device__ __forceinline__ unsigned sm_addr(const void* p) { return unsigned(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void bar_init(std::uint64_t* b, unsigned n) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(sm_addr(b)), "r"(n));
+}
+__device__ __forceinline__ void bar_arrive(std::uint64_t* b) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(sm_addr(b)) : "memory");
+}
+__device__ __forceinline__ bool bar_test(std::uint64_t* b, unsigned parity) {
+    unsigned ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(sm_addr(b)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// Bounded; false after the limit or when another role gave up.
+__device__ __forceinline__ bool bar_wait(std::uint64_t* b, unsigned parity, volatile int* abort_flag, int* status) {
+    for (unsigned i = 0; i < kTreeSpin; ++i) {
+        if (bar_test(b, parity)) return true;
+        if (*abort_flag) return false;
+    }
+    *abort_flag = 1;
+    atomicOr(status, kTreeTimeout);
+    return false;
+}
+__device__ __forceinline__ void tree_commit_to(std::uint64_t* b) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(sm_addr(b))
+                 : "memory");
+}
+__device__ __forceinline__ void mma_ss(unsigned d, std::uint64_t a, std::uint64_t b, unsigned idesc, int acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+__device__ __forceinline__ void mma_ts(unsigned d, unsigned a, std::uint64_t b, unsigned idesc, int acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+// 128-byte swizzled operand: 8-row atoms of 1024 bytes (SBO); lbo is the
+// distance of 64-column halves for an operand with the MMA's N contiguous.
+__device__ __forceinline__ std::uint64_t sw128_desc(unsigned addr, unsigned lbo) {
+    return ((addr >> 4) & 0x3FFFull) | (std::uint64_t((lbo >> 4) & 0x3FFF) << 16) | (64ull << 32) | (1ull << 46) |
+           (2ull << 61);
+}
+__device__ __forceinline__ void tm_ld32(unsigned addr, unsigned (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tm_st16(unsigned addr, const unsigned (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+            addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tm_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tm_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void cp16(unsigned dst, const void* src, unsigned bytes) {  // bytes 16, or 0: zero fill
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp4(unsigned dst, const void* src, unsigned bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float two_to(int e) { return __uint_as_float(unsigned(127 + e) << 23); }  // |e| <= 126
+// The power of two that brings a largest |value| into [2^14, 2^15).
+__device__ __forceinline__ int lift(float top) {
+    const int e = int((__float_as_uint(top) >> 23) & 255) - 127;
+    return top > 0.f && e < 128 ? max(-113, min(112, 14 - e)) : 0;
+}
+// p in [0, 2^11] as hi (an integer) + lo (|lo| <= 1/2): F16 each, lo's
+// rounding is 2^-13, that is 2^-24 of the row's largest weight.
+__device__ __forceinline__ void split_weight(float x, float y, unsigned& hi, unsigned& lo) {
+    constexpr float kRound = 12582912.f;  // 1.5 * 2^23
+    const float hx = __fsub_rn(__fadd_rn(x, kRound), kRound), hy = __fsub_rn(__fadd_rn(y, kRound), kRound);
+    const __half2 h = __floats2half2_rn(hx, hy), l = __floats2half2_rn(x - hx, y - hy);
+    hi = *reinterpret_cast<const unsigned*>(&h);
+    lo = *reinterpret_cast<const unsigned*>(&l);
+}
+
+// What every role knows of a sequence, and its tiles in the global order
+// (KV heads outermost, then groups of query vectors, then tiles).
+struct TreeSeq {
+    int s, c0, n, len, groups, weight;
+    long long tiles;   // per item
+    long long total;   // hkv * groups * tiles
+    bool pair;
+};
+template <class F>
+__device__ __forceinline__ bool tree_seq(const TreeAttn& a, int s, TreeSeq& q) {
+    q.s = s;
+    if (!tree_sequence_ok(a, s, q.c0, q.n, q.len) || q.n == 0) {
+        q.total = 0;
+        return q.n == 0;
+    }
+    const int vectors = q.n * (a.hq / a.hkv);
+    const int most = F::kPairs ? 256 : 128;
+    q.groups = (vectors + most - 1) / most;
+    q.pair = F::kPairs && vectors > 128;
+    q.weight = q.pair ? 2 : 1;
+    q.tiles = ((long long)q.len + q.n + F::kBn - 1) / F::kBn;
+    q.total = q.tiles * q.groups * a.hkv;
+    return true;
+}
+
+// One piece of an item: tiles [t0, t1) of it run in this CTA.
+template <class F>
+struct TreeWalk {
+    TreeSeq q;
+    long long u, u_end;
+    int seq1;
+    long long u1;
+    long long t0, t1;
+    int head, row0, rows, split;  // split: vectors of the first M tile
+    long long item;
+    int count;                    // pieces begun, minus one
+    long long tile_base;          // tiles of earlier pieces
+
+    __device__ __forceinline__ void start(const TreeAttn& a, int seq0, long long u0, int last_seq, long long last_u) {
+        seq1 = last_seq;
+        u1 = last_u;
+        count = -1;
+        tile_base = 0;
+        t0 = t1 = 0;
+        tree_seq<F>(a, seq0, q);
+        u = u0;
+        u_end = seq0 == seq1 ? u1 : q.total;
+    }
+    __device__ __forceinline__ bool next(const TreeAttn& a) {
+        tile_base += t1 - t0;
+        while (u >= u_end) {
+            if (q.s >= seq1 || q.s + 1 >= a.n_seq) return false;
+            tree_seq<F>(a, q.s + 1, q);
+            u = 0;
+            u_end = q.s == seq1 ? min(u1, q.total) : q.total;
+        }
+        item = u / q.tiles;
+        t0 = u - item * q.tiles;
+        t1 = min(q.tiles, t0 + (u_end - u));
+        u += t1 - t0;
+        head = int(item / q.groups);
+        const int grp = int(item - (long long)head * q.groups), vectors = q.n * (a.hq / a.hkv);
+        // groups of nearly equal size, and M tiles of nearly equal size
+        const int per = (vectors + q.groups - 1) / q.groups;
+        row0 = grp * per;
+        rows = min(per, vectors - row0);
+        split = q.pair ? (rows + 1) / 2 : rows;
+        ++count;
+        return true;
+    }
+    // Entry e of the piece's 2 (t1 - t0) loads, in the order of their use:
+    // K runs `ahead` tiles before V.
+    __device__ __forceinline__ int entry(int e, bool& is_v) const {
+        const int c = int(t1 - t0), ahead = min(q.pair ? 1 : 2, c);
+        if (e < ahead) {
+            is_v = false;
+            return e;
+        }
+        const int f = e - ahead;
+        if (f < 2 * (c - ahead)) {
+            is_v = !(f & 1);
+            return is_v ? f >> 1 : (f >> 1) + ahead;
+        }
+        is_v = true;
+        return c - ahead + (f - 2 * (c - ahead));
+    }
+};
+
+// Bits [j0, j0 + 32) of the mask row of node `node` (negative j0: cached
+// positions, visible), columns behind the last node cleared.
+__device__ __forceinline__ unsigned node_bits(const TreeAttn& a, int c0, int n, int node, long long j0) {
+    if (j0 >= n) return 0;
+    if (j0 + 32 <= 0) return 0xffffffffu;
+    const int j = int(j0);
+    const int from = max(j, 0), shift = from & 31;  // bits [from, from + 32) of the nodes, moved up by from - j
+    unsigned w;
+    if (a.ancestors) {
+        const unsigned* row = reinterpret_cast<const unsigned*>(a.ancestors + (long long)(c0 + node) * a.words);
+        const int i = from >> 5;
+        w = row[i] >> shift;
+        if (shift && i + 1 < 2 * a.words) w |= row[i + 1] << (32 - shift);
+    } else {
+        const int left = node + 1 - from;  // a chain sees nodes up to its own
+        w = left <= 0 ? 0u : left >= 32 ? 0xffffffffu : (1u << left) - 1;
+    }
+    const int have = n - from;
+    if (have < 32) w &= (1u << have) - 1;
+    if (j < 0) w = (w << -j) | ((1u << -j) - 1);
+    return w;
+}
+
+template <int KV, int DP>
+__global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, float* partial, TreeRec* recs,
+                                                                   int min_weight) {
+    using F = TreeForm<KV, DP>;
+    extern __shared__ __align__(1024) unsigned char tree_smem[];
+    TreeMeta& M = *reinterpret_cast<TreeMeta*>(tree_smem + F::kOffMeta);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int group = a.hq / a.hkv;
+
+    if (tid == 0) {
+        for (int i = 0; i < 8; ++i) {
+            bar_init(&M.full[i], 4);
+            bar_init(&M.empty[i], 1);
+        }
+        for (int i = 0; i < kMetaRing; ++i) bar_init(&M.v_ready[i], 4);
+        for (int i = 0; i < 2; ++i) {
+            bar_init(&M.s_full[i], 1);
+            bar_init(&M.p_full[i], 4);
+            bar_init(&M.o_full[i], 1);
+        }
+        bar_init(&M.q_full, 8);
+        bar_init(&M.item_done, 1);
+        bar_init(&M.merge_ready, 4);
+        bar_init(&M.merge_read, 4);
+        bar_init(&M.drain, 1);
+        M.abort_flag = 0;
+        M.bad = 0;
+        for (int i = 0; i < 16; ++i) M.vbad[i] = 0;
+        M.total = 0;
+        M.seq0 = M.seq1 = a.n_seq;
+        M.excl0 = M.excl1 = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    // The run of tiles: weights are scanned in sequence order by every CTA.
+    const auto weight_of = [&](int s) -> long long {
+        TreeSeq q;
+        if (s >= a.n_seq) return 0;
+        if (!tree_seq<F>(a, s, q)) M.bad = 1;
+        return q.total ? q.total * q.weight : 0;
+    };
+    long long mine = 0;
+    for (int s = tid; s < a.n_seq; s += kTreeThreads) mine += weight_of(s);
+    if (mine) atomicAdd(reinterpret_cast<unsigned long long*>(&M.total), (unsigned long long)mine);
+    __syncthreads();
+    const long long total = M.total;
+    if (blockIdx.x == 0 && tid == 0 && M.bad) atomicOr(a.status, kTreeBadLengths);
+    const int ctas = int(max(1ll, min((long long)gridDim.x, total / min_weight)));
+    const int cta = blockIdx.x;
+    if (tid == 0) recs[cta].pieces = 0;
+    if (cta >= ctas || total == 0) return;
+    const long long w0 = total * cta / ctas, w1 = total * (cta + 1) / ctas;
+    long long carry = 0;
+    for (int base = 0; base < a.n_seq; base += kTreeThreads) {
+        const long long w = weight_of(base + tid);
+        long long scan = w;
+        for (int d = 1; d < 32; d <<= 1) {
+            const long long up = __shfl_up_sync(0xffffffffu, scan, d);
+            if (lane >= d) scan += up;
+        }
+        if (lane == 31) M.warp_sum[warp] = scan;
+        __syncthreads();
+        long long before = carry, all = 0;
+        for (int i = 0; i < kTreeThreads / 32; ++i) {
+            if (i < warp) before += M.warp_sum[i];
+            all += M.warp_sum[i];
+        }
+        const long long excl = before + scan - w;
+        if (w && excl <= w0 && w0 < excl + w) {
+            M.seq0 = base + tid;
+            M.excl0 = excl;
+        }
+        if (w && excl < w1 && w1 <= excl + w) {
+            M.seq1 = base + tid;
+            M.excl1 = excl;
+        }
+        carry += all;
+        __syncthreads();
+        if (carry >= w1) break;
+    }
+    if (warp == kTreeMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sm_addr(&M.tmem)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tm_before();
+    __syncthreads();
+    tm_after();
+    const unsigned tmem = M.tmem;
+    volatile int* abort_flag = &M.abort_flag;
+    TreeWalk<F> walk;
+    {
+        TreeSeq q;
+        tree_seq<F>(a, M.seq0, q);
+        const long long u0 = (w0 - M.excl0 + q.weight - 1) / q.weight;
+        tree_seq<F>(a, M.seq1, q);
+        const long long u1 = (w1 - M.excl1 + q.weight - 1) / q.weight;
+        walk.start(a, M.seq0, u0, M.seq1, u1);
+    }
+    const unsigned smem = sm_addr(tree_smem);
+    const auto slot_at = [&](int slot) -> unsigned {
+        return slot < F::kBase ? F::kOffSlots + slot * F::kSlot : F::kQTile + (slot - F::kBase) * F::kSlot;
+    };
+
+    if (warp < kTreeLoadWarp) {
+        // ------------------------------------------------ softmax warpgroups
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const int stream = warp >> 2, wq = warp & 3, r = tid & 127;
+        const unsigned lane_base = tmem + (unsigned(wq * 32) << 16);
+        const unsigned s_at = lane_base + stream * 128, o_at = lane_base + 256 + stream * 128;
+        const float score_unit = 1.4426950408889634f / sqrtf(float(a.dim));
+        unsigned n_s = 0, n_o = 0;  // completed waits on s_full / o_full
+        bool go = true;
+        float o[DP];
+        while (go && walk.next(a)) {
+            const TreeSeq& q = walk.q;
+            const int tile_rows = q.pair ? (stream ? walk.rows - walk.split : walk.split) : walk.rows;
+            const int row = q.pair && stream ? walk.split + r : r;  // vector of the item
+            const bool live = r < tile_rows, warp_live = wq * 32 < tile_rows;
+            const int vec = walk.row0 + row, node = live ? vec / group : 0;
+            const int head = walk.head * group + (vec - node * group);
+            // the query vector, scaled below 2^15 and split, into this stream's Q tile
+            float c = 0.f;
+            if (live) {
+                const float4* src = reinterpret_cast<const float4*>(a.q + (long long)(q.c0 + node) * a.ldq + (long long)head * a.dim);
+                float top = 0.f;
+                const int quads = a.dim >> 2;
+#pragma unroll 8
+                for (int i = 0; i < quads; ++i) {
+                    const float4 v = __ldg(src + i);
+                    top = fmaxf(fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+                }
+                const int up = lift(top);
+                c = score_unit * two_to(-up);
+                if (stream == 0 || q.pair) {
+                    const float f = two_to(up);
+                    unsigned char* tile = tree_smem + (stream ? F::kQTile : 0);
+#pragma unroll 4
+                    for (int i = 0; i < DP / 8; ++i) {
+                        const float4 x = 2 * i < quads ? __ldg(src + 2 * i) : make_float4(0, 0, 0, 0);
+                        const float4 y = 2 * i + 1 < quads ? __ldg(src + 2 * i + 1) : make_float4(0, 0, 0, 0);
+                        uint4 hi, lo;
+                        split_exact(x.x * f, x.y * f, hi.x, lo.x);
+                        split_exact(x.z * f, x.w * f, hi.y, lo.y);
+                        split_exact(y.x * f, y.y * f, hi.z, lo.z);
+                        split_exact(y.z * f, y.w * f, hi.w, lo.w);
+                        const int at = (i >> 3) * 16384 + r * 128 + (((i & 7) ^ (r & 7)) << 4);
+                        *reinterpret_cast<uint4*>(tile + at) = hi;
+                        *reinterpret_cast<uint4*>(tile + F::kQPart + at) = lo;
+                    }
+                }
+            }
+            proxy_fence();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&M.q_full);
+            float m = -INFINITY, l = 0.f, vref = 0.f;
+#pragma unroll
+            for (int i = 0; i < DP; ++i) o[i] = 0.f;
+            const int tiles = int(walk.t1 - walk.t0);
+            const int first = q.pair ? 0 : stream, step = q.pair ? 1 : 2;
+            for (int j = first; j < tiles && go; j += step) {
+                go = __all_sync(0xffffffffu, bar_wait(&M.s_full[stream], n_s & 1, abort_flag, a.status));
+                ++n_s;
+                if constexpr (KV != 1) {
+                    const long long t = walk.tile_base + j;
+                    go = go && __all_sync(0xffffffffu, bar_wait(&M.v_ready[t % kMetaRing], (t / kMetaRing) & 1, abort_flag, a.status));
+                }
+                if (!go) break;
+                tm_after();
+                if (warp_live) {
+                    const long long p0 = (walk.t0 + j) * F::kBn;
+                    const int ring = int((walk.tile_base + j) % kMetaRing);
+                    const bool nodes = p0 + F::kBn > q.len;
+                    unsigned seen[F::kBn / 32];
+#pragma unroll
+                    for (int k = 0; k < F::kBn / 32; ++k) {
+                        seen[k] = M.valid[ring][k];
+                        if (nodes) seen[k] &= node_bits(a, q.c0, q.n, node, p0 + 32 * k - q.len);
+                    }
+                    const float* k_scale = reinterpret_cast<const float*>(tree_smem + F::kOffScale) +
+                                           int((walk.tile_base + j) % max(1, F::kScaleRing)) * 2 * F::kBn;
+                    const float* v_scale = k_scale + F::kBn;
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int k = 0; k < F::kBn / 32; ++k) {
+                        unsigned x[32];
+                        tm_ld32(s_at + 32 * k, x);
+                        if constexpr (KV != 1) {
+#pragma unroll
+                            for (int i = 0; i < 32; i += 4) {
+                                const float4 f = *reinterpret_cast<const float4*>(k_scale + 32 * k + i);
+                                x[i] = __float_as_uint(__uint_as_float(x[i]) * f.x);
+                                x[i + 1] = __float_as_uint(__uint_as_float(x[i + 1]) * f.y);
+                                x[i + 2] = __float_as_uint(__uint_as_float(x[i + 2]) * f.z);
+                                x[i + 3] = __float_as_uint(__uint_as_float(x[i + 3]) * f.w);
+                            }
+                        }
+                        if (seen[k] == 0xffffffffu) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(x[i]));
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (seen[k] >> i & 1) top = fmaxf(top, __uint_as_float(x[i]));
+                        }
+                    }
+                    const float mn = fmaxf(m, top * c);
+                    float keep = mn == -INFINITY ? 1.f : ex2(m - mn);
+                    const float off = 11.f - (mn == -INFINITY ? 0.f : mn);
+                    m = mn;
+                    l *= keep;
+                    float v_unit = 1.f;
+                    if constexpr (KV != 1) {
+                        const float4 t = *reinterpret_cast<const float4*>(M.vmax[ring]);
+                        const float big = fmaxf(fmaxf(vref, fmaxf(t.x, t.y)), fmaxf(t.z, t.w));
+                        if (big > vref) {
+                            keep *= vref / big;
+                            vref = big;
+                        }
+                        v_unit = vref > 0.f ? 1.f / vref : 0.f;
+                    }
+                    float sum0 = 0.f, sum1 = 0.f;
+                    unsigned hold[2][16];  // lo halves waiting for their columns of S to be read
+#pragma unroll
+                    for (int k = 0; k < F::kBn / 32; ++k) {
+                        unsigned x[32], hi[16], lo[16];
+                        tm_ld32(s_at + 32 * k, x);
+                        const unsigned see = seen[k];
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            float p[4];
+                            float4 ks, vs;
+                            if constexpr (KV != 1) {
+                                ks = *reinterpret_cast<const float4*>(k_scale + 32 * k + i);
+                                vs = *reinterpret_cast<const float4*>(v_scale + 32 * k + i);
+                            }
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                float s = __uint_as_float(x[i + e]);
+                                if constexpr (KV != 1) s *= e == 0 ? ks.x : e == 1 ? ks.y : e == 2 ? ks.z : ks.w;
+                                p[e] = ex2(fmaf(s, c, off));
+                            }
+                            if (see != 0xffffffffu) {
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    if (!(see >> (i + e) & 1)) p[e] = 0.f;
+                            }
+                            sum0 += p[0] + p[2];
+                            sum1 += p[1] + p[3];
+                            if constexpr (KV != 1) {
+                                p[0] *= vs.x * v_unit;
+                                p[1] *= vs.y * v_unit;
+                                p[2] *= vs.z * v_unit;
+                                p[3] *= vs.w * v_unit;
+                                if (see != 0xffffffffu) {  // a masked row's scale may be anything
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e)
+                                        if (!(see >> (i + e) & 1)) p[e] = 0.f;
+                                }
+                            }
+                            split_weight(p[0], p[1], hi[i / 2], lo[i / 2]);
+                            split_weight(p[2], p[3], hi[i / 2 + 1], lo[i / 2 + 1]);
+                        }
+                        // hi half k in columns 16 k.., lo half k in kBn / 2 + 16 k..: written once those are read
+                        tm_st16(s_at + 16 * k, hi);
+                        constexpr int kHalf = F::kBn / 64;  // chunks before the upper half of S
+                        if (k < kHalf) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) hold[k][i] = lo[i];
+                        } else {
+                            // chunk k read: columns below 32 (k + 1) are free, lo halves up to 2 (k - kHalf) + 1 fit
+                            if (F::kBn == 64) {
+                                tm_st16(s_at + 32, hold[0]);
+                                tm_st16(s_at + 48, lo);
+                            } else if (k == 2) {
+                                tm_st16(s_at + 64, hold[0]);
+                                tm_st16(s_at + 80, hold[1]);
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) hold[0][i] = lo[i];
+                            } else {
+                                tm_st16(s_at + 96, hold[0]);
+                                tm_st16(s_at + 112, lo);
+                            }
+                        }
+                    }
+                    l += sum0 + sum1;
+                    tm_wait_st();
+                    tm_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(&M.p_full[stream]);
+                    go = __all_sync(0xffffffffu, bar_wait(&M.o_full[stream], n_o & 1, abort_flag, a.status));
+                    ++n_o;
+                    if (!go) break;
+                    tm_after();
+#pragma unroll
+                    for (int k = 0; k < DP / 32; ++k) {
+                        unsigned x[32];
+                        tm_ld32(o_at + 32 * k, x);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[32 * k + i] = fmaf(o[32 * k + i], keep, __uint_as_float(x[i]));
+                    }
+                } else {
+                    if (lane == 0) bar_arrive(&M.p_full[stream]);
+                    go = __all_sync(0xffffffffu, bar_wait(&M.o_full[stream], n_o & 1, abort_flag, a.status));
+                    ++n_o;
+                }
+            }
+            if (!go) break;
+            if constexpr (KV != 1) {
+#pragma unroll
+                for (int i = 0; i < DP; ++i) o[i] *= vref;
+            }
+            if (!q.pair) {
+                // the odd tiles' (O, m, l) through stream 1's tensor memory
+                const unsigned b_o = lane_base + 256 + 128, b_ml = lane_base + 128;
+                if (stream) {
+                    if (warp_live && tiles > 1) {
+#pragma unroll
+                        for (int k = 0; k < DP / 16; ++k) {
+                            unsigned x[16];
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(o[16 * k + i]);
+                            tm_st16(b_o + 16 * k, x);
+                        }
+                        unsigned x[16] = {__float_as_uint(m), __float_as_uint(l)};
+                        tm_st16(b_ml, x);
+                        tm_wait_st();
+                    }
+                    tm_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(&M.merge_ready);
+                    go = __all_sync(0xffffffffu, bar_wait(&M.merge_read, walk.count & 1, abort_flag, a.status));
+                    tm_after();
+                } else {
+                    go = __all_sync(0xffffffffu, bar_wait(&M.merge_ready, walk.count & 1, abort_flag, a.status));
+                    tm_after();
+                    if (go && warp_live && tiles > 1) {
+                        unsigned x[32];
+                        tm_ld32(b_ml, x);
+                        const float m2 = __uint_as_float(x[0]), l2 = __uint_as_float(x[1]);
+                        const float mn = fmaxf(m, m2);
+                        const float ka = mn == -INFINITY ? 0.f : ex2(m - mn), kb = mn == -INFINITY ? 0.f : ex2(m2 - mn);
+                        m = mn;
+                        l = l * ka + l2 * kb;
+#pragma unroll
+                        for (int k = 0; k < DP / 32; ++k) {
+                            tm_ld32(b_o + 32 * k, x);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                o[32 * k + i] = fmaf(o[32 * k + i], ka, __uint_as_float(x[i]) * kb);
+                        }
+                    }
+                    tm_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(&M.merge_read);
+                }
+            } else {  // both count every item
+                __syncwarp();
+                if (lane == 0) bar_arrive(stream ? &M.merge_ready : &M.merge_read);
+            }
+            if (!go) break;
+            if (live && (q.pair || stream == 0)) {
+                const bool whole = walk.t0 == 0 && walk.t1 == q.tiles;
+                float* dst;
+                float f = 1.f;
+                if (whole) {
+                    dst = a.out + (long long)(q.c0 + node) * a.ldo + (long long)head * a.dim;
+                    f = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
+                } else {
+                    // the CTA's slot 1 holds an item that begins here, slot 0 one that began earlier
+                    float* slot = partial + (long long)(2 * cta + (walk.t0 == 0)) * kTreeRows * (DP + 2);
+                    const int pr = stream * 128 + r;
+                    dst = slot + pr * DP;
+                    slot[kTreeRows * DP + pr] = m;
+                    slot[kTreeRows * DP + kTreeRows + pr] = l;
+                }
+#pragma unroll
+                for (int i = 0; i < DP; i += 4)
+                    if (!whole || i < a.dim)
+                        *reinterpret_cast<float4*>(dst + i) = make_float4(o[i] * f, o[i + 1] * f, o[i + 2] * f, o[i + 3] * f);
+                if (M.vbad[walk.count & 15]) {
+                    // non-finite V of nodes was kept out of the products (0 * inf): give it to the rows that see it
+                    int unused = 0;
+                    for (int j = 0; j < q.n; ++j) {
+                        if (!(node_bits(a, q.c0, q.n, node, j) & 1)) continue;
+                        const long long base = tree_row(a, q.s, q.c0, q.len, q.len + j, unused);
+                        if (base < 0) continue;
+                        const long long v = base + (long long)walk.head * a.bt * a.dim + a.kind_stride;
+                        const float sc = KV == 2 ? a.scales[v / a.dim] : 1.f;
+                        for (int d = 0; d < a.dim; ++d) {
+                            const float x = KV == 2 ? sc : kv_value(a, v + d);
+                            if (!isfinite(x)) dst[d] += x;
+                        }
+                    }
+                }
+            }
+            if (warp == 0 && lane == 0 && walk.t0 == 0 && walk.t1 < q.tiles) {
+                // the CTA in which the item's last tile starts
+                const long long excl = q.s == M.seq0 ? M.excl0 : q.s == M.seq1 ? M.excl1 : -1;
+                long long last;
+                if (excl >= 0) {
+                    last = excl + (walk.item * q.tiles + q.tiles - 1) * q.weight;
+                    const long long end = ((last + 1) * ctas + total - 1) / total - 1;
+                    TreeRec rec;
+                    rec.c0 = q.c0;
+                    rec.row0 = walk.row0;
+                    rec.rows = walk.rows;
+                    rec.split = walk.split;
+                    rec.head = walk.head;
+                    rec.pieces = int(end) - cta + 1;
+                    recs[cta] = rec;
+                }
+            }
+        }
+    } else if (warp < kTreeMmaWarp) {
+        // ------------------------------------------------------------ loads
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        const int lw = warp - kTreeLoadWarp;
+        constexpr int kRowsPerWarp = F::kBn / 4;
+        unsigned empty_phase = 0xffffffffu;
+        int slot = 0, flags = 0;
+        const int row_bytes = a.dim * F::kElem, chunks = row_bytes >> 4;
+        const unsigned char* pool = static_cast<const unsigned char*>(a.kv);
+        // Address of this lane's row of a tile (byte offset of its K row, -1: none)
+        const auto row_of = [&](const TreeWalk<F>& w, int j) -> long long {
+            const long long p = (w.t0 + j) * F::kBn + lw * kRowsPerWarp + (lane % kRowsPerWarp);
+            if (p >= (long long)w.q.len + w.q.n) return -1;
+            const long long at = tree_row(a, w.q.s, w.q.c0, w.q.len, int(p), flags);
+            return at < 0 ? -1 : at + (long long)w.head * a.bt * a.dim;
+        };
+        if constexpr (KV == 1) {
+            bool go = true, prev_pair = false;
+            int pend[2], n_pend = 0;
+            const auto signal = [&](int s) {
+                proxy_fence();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&M.full[s]);
+            };
+            const auto drain = [&]() {
+                cp_wait<0>();
+                for (int i = 0; i < n_pend; ++i) signal(pend[i]);
+                n_pend = 0;
+            };
+            while (go && walk.next(a)) {
+                const bool pair = walk.q.pair;
+                const int ns = pair ? F::kBase : F::kBase + F::kExtra;
+                if (slot >= ns) slot = 0;
+                bool wait_q = prev_pair && !pair;  // extra slots lie in the second Q tile: its MMAs first
+                if (lane == 0 && lw == 0) M.vbad[(walk.count + 8) & 15] = 0;  // no warp is that far ahead or behind
+                const int loads = 2 * int(walk.t1 - walk.t0);
+                for (int e = 0; e < loads && go; ++e) {
+                    bool is_v;
+                    const int j = walk.entry(e, is_v);
+                    const long long k_row = row_of(walk, j);
+                    const unsigned have = __ballot_sync(0xffffffffu, k_row >= 0);
+                    if (slot >= F::kBase && wait_q) {
+                        drain();
+                        go = __all_sync(0xffffffffu, bar_wait(&M.item_done, (walk.count - 1) & 1, abort_flag, a.status));
+                        wait_q = false;
+                        if (!go) break;
+                    }
+                    const unsigned parity = (empty_phase >> slot) & 1;
+                    if (!__all_sync(0xffffffffu, bar_test(&M.empty[slot], parity))) {
+                        drain();  // nothing can be issued: hand over what has landed meanwhile
+                        go = __all_sync(0xffffffffu, bar_wait(&M.empty[slot], parity, abort_flag, a.status));
+                        if (!go) break;
+                    }
+                    empty_phase ^= 1u << slot;
+                    if (!is_v && lane == 0) M.valid[(walk.tile_base + j) % kMetaRing][lw] = have;
+                    const unsigned dst = smem + slot_at(slot);
+                    const long long shift = is_v ? a.kind_stride : 0;
+                    constexpr int kLanes = DP / 8, kStep = 32 / kLanes;  // lanes per row, rows per instruction
+                    const int ch = lane % kLanes;
+#pragma unroll 8
+                    for (int i = 0; i < 32 / kStep; ++i) {
+                        const int rr = i * kStep + lane / kLanes;
+                        const long long at = __shfl_sync(0xffffffffu, k_row, rr);
+                        const bool ok = at >= 0 && ch < chunks;
+                        const int rt = lw * 32 + rr;
+                        cp16(dst + (ch >> 3) * (F::kBn * 128) + rt * 128 + (((ch & 7) ^ (rt & 7)) << 4),
+                             ok ? pool + (at + shift) * 2 + ch * 16 : pool, ok ? 16u : 0u);
+                    }
+                    cp_commit();
+                    if (is_v && (walk.t0 + j + 1) * F::kBn > walk.q.len) {
+                        // a tile with nodes: non-finite V must not meet a weight of zero in the products
+                        drain();
+                        cp_wait<0>();
+                        __syncwarp();
+                        const int rt = lw * 32 + lane;
+                        const bool is_node = (walk.t0 + j) * F::kBn + rt >= walk.q.len && k_row >= 0;
+                        bool bad = false;
+                        if (is_node) {
+                            for (int k = 0; k < kLanes; ++k) {
+                                uint4* at = reinterpret_cast<uint4*>(tree_smem + slot_at(slot) + (k >> 3) * (F::kBn * 128) +
+                                                                     rt * 128 + (((k & 7) ^ (rt & 7)) << 4));
+                                uint4 v = *at;
+                                unsigned* w = reinterpret_cast<unsigned*>(&v);
+                                bool hit = false;
+                                for (int x = 0; x < 4; ++x) {
+                                    if ((w[x] & 0x7c00u) == 0x7c00u) w[x] &= 0xffff0000u, hit = true;
+                                    if ((w[x] & 0x7c000000u) == 0x7c000000u) w[x] &= 0xffffu, hit = true;
+                                }
+                                if (hit) *at = v, bad = true;
+                            }
+                        }
+                        if (bad) M.vbad[walk.count & 15] = 1;
+                        signal(slot);
+                    } else {
+                        if (n_pend == 2) {
+                            cp_wait<2>();
+                            signal(pend[0]);
+                            pend[0] = pend[1];
+                            n_pend = 1;
+                        }
+                        pend[n_pend++] = slot;
+                    }
+                    slot = slot + 1 == ns ? 0 : slot + 1;
+                }
+                prev_pair = pair;
+            }
+            drain();
+        } else {
+            // Raw rows land in a small ring by cp.async, each 16 bytes in the
+            // place of the thread that converts them, so a thread waits only
+            // for its own copies.
+            bool go = true;
+            TreeWalk<F> ahead = walk;
+            int e_issue = 0, loads_issue = 0;
+            bool more = true;
+            int raw_in = 0, raw_out = 0;
+            constexpr int kLanes = DP * F::kElem / 16, kStep = 32 / kLanes;  // lanes per row, rows per instruction
+            constexpr int kIters = kRowsPerWarp / kStep;
+            const int ch = lane % kLanes;
+            const auto issue = [&]() {
+                if (e_issue == loads_issue) {
+                    more = ahead.next(a);
+                    if (!more) return;
+                    e_issue = 0;
+                    loads_issue = 2 * int(ahead.t1 - ahead.t0);
+                }
+                bool is_v;
+                const int j = ahead.entry(e_issue++, is_v);
+                const long long mine_row = row_of(ahead, j);
+                const unsigned have = __ballot_sync(0xffffffffu, mine_row >= 0);
+                if (!is_v && lane == 0) {
+                    unsigned* valid = M.valid[(ahead.tile_base + j) % kMetaRing];
+                    if constexpr (F::kBn == 128)
+                        valid[lw] = have;
+                    else
+                        reinterpret_cast<unsigned short*>(valid)[lw] = (unsigned short)(have & 0xffffu);
+                }
+                const unsigned dst = smem + F::kOffRaw + raw_in * F::kRaw + lw * (F::kRaw / 4);
+                const long long shift = is_v ? a.kind_stride : 0;
+#pragma unroll 4
+                for (int i = 0; i < kIters; ++i) {
+                    const int rr = i * kStep + lane / kLanes;
+                    const long long at = __shfl_sync(0xffffffffu, mine_row, rr);
+                    const bool ok = at >= 0 && ch < chunks;
+                    cp16(dst + (i * 32 + lane) * 16, ok ? pool + (at + shift) * F::kElem + ch * 16 : pool, ok ? 16u : 0u);
+                }
+                if constexpr (KV == 2) {  // this lane's row scale, straight into its column
+                    const int ring = int((ahead.tile_base + j) % F::kScaleRing);
+                    const unsigned to = smem + F::kOffScale + ((ring * 2 + is_v) * F::kBn + lw * 32 + lane) * 4;
+                    cp4(to, mine_row >= 0 ? a.scales + (mine_row + shift) / a.dim : a.scales, mine_row >= 0 ? 4u : 0u);
+                }
+                cp_commit();
+                raw_in = raw_in + 1 == F::kRawDepth ? 0 : raw_in + 1;
+            };
+            for (int i = 0; i < F::kRawDepth - 1; ++i) {
+                if (more) issue();
+                if (!more) cp_commit();  // keeps the count of groups
+            }
+            while (go && walk.next(a)) {
+                if (lane == 0 && lw == 0) M.vbad[(walk.count + 8) & 15] = 0;  // no warp is that far ahead or behind
+                const int loads = 2 * int(walk.t1 - walk.t0);
+                for (int e = 0; e < loads && go; ++e) {
+                    bool is_v;
+                    const int j = walk.entry(e, is_v);
+                    if (more) issue();
+                    if (!more) cp_commit();
+                    cp_wait<F::kRawDepth - 1>();
+                    const unsigned parity = (empty_phase >> slot) & 1;
+                    go = __all_sync(0xffffffffu, bar_wait(&M.empty[slot], parity, abort_flag, a.status));
+                    if (!go) break;
+                    empty_phase ^= 1u << slot;
+                    const int meta = int((walk.tile_base + j) % kMetaRing);
+                    const long long p0 = (walk.t0 + j) * F::kBn, lane_p = p0 + lw * kRowsPerWarp + (lane % kRowsPerWarp);
+                    const bool node_row = lane_p >= walk.q.len;
+                    float* scale_col = reinterpret_cast<float*>(tree_smem + F::kOffScale) +
+                                       (int((walk.tile_base + j) % F::kScaleRing) * 2 + is_v) * F::kBn;
+                    unsigned char* out = tree_smem + slot_at(slot);
+                    const uint4* raw = reinterpret_cast<const uint4*>(tree_smem + F::kOffRaw + raw_out * F::kRaw +
+                                                                      lw * (F::kRaw / 4));
+                    float big = 0.f;
+                    bool bad = false;
+                    if constexpr (KV == 2) {
+                        if (is_v) {
+                            float* mine_s = scale_col + lw * 32 + lane;
+                            float sc = *mine_s;
+                            if (node_row && !isfinite(sc)) {
+                                bad = true;
+                                *mine_s = sc = 0.f;
+                            }
+                            big = fabsf(sc);
+                        }
+#pragma unroll 4
+                        for (int i = 0; i < kIters; ++i) {
+                            const int rt = lw * 32 + i * kStep + lane / kLanes;
+                            const uint4 v = raw[i * 32 + lane];
+                            const unsigned w[4] = {v.x, v.y, v.z, v.w};
+                            unsigned h[8];
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) {
+                                // code + 128 beside 0x64: 1024 + 128 + code, exact in F16
+                                const unsigned b = w[x] ^ 0x80808080u;
+                                const __half2 off = __half2half2(__ushort_as_half(0x6480));
+                                const unsigned l0 = __byte_perm(b, 0x64646464u, 0x4140), l1 = __byte_perm(b, 0x64646464u, 0x4342);
+                                const __half2 a0 = __hsub2(*reinterpret_cast<const __half2*>(&l0), off);
+                                const __half2 a1 = __hsub2(*reinterpret_cast<const __half2*>(&l1), off);
+                                h[2 * x] = *reinterpret_cast<const unsigned*>(&a0);
+                                h[2 * x + 1] = *reinterpret_cast<const unsigned*>(&a1);
+                            }
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                const int hc = 2 * ch + x;  // 16-byte chunk of the F16 row
+                                *reinterpret_cast<uint4*>(out + (hc >> 3) * (F::kBn * 128) + rt * 128 +
+                                                          (((hc & 7) ^ (rt & 7)) << 4)) =
+                                    make_uint4(h[4 * x], h[4 * x + 1], h[4 * x + 2], h[4 * x + 3]);
+                            }
+                        }
+                    } else {
+#pragma unroll 2
+                        for (int i = 0; i < kIters; ++i) {
+                            const int rw = i * kStep + lane / kLanes, rt = lw * kRowsPerWarp + rw;
+                            uint4 raw_v = raw[i * 32 + lane];
+                            float v[4] = {__uint_as_float(raw_v.x), __uint_as_float(raw_v.y), __uint_as_float(raw_v.z),
+                                          __uint_as_float(raw_v.w)};
+                            if (is_v && p0 + rt >= walk.q.len) {
+#pragma unroll
+                                for (int x = 0; x < 4; ++x)
+                                    if (!isfinite(v[x])) v[x] = 0.f, bad = true;
+                            }
+                            float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+#pragma unroll
+                            for (int d = kLanes / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                            const int up = lift(top);
+                            const float f = two_to(up), back = two_to(-up);
+                            if (ch == 0) scale_col[rt] = back;
+                            big = fmaxf(big, top > 0.f ? back : 0.f);
+                            uint2 hi, lo;
+                            split_exact(v[0] * f, v[1] * f, hi.x, lo.x);
+                            split_exact(v[2] * f, v[3] * f, hi.y, lo.y);
+                            const int at = (ch >> 4) * (F::kBn * 128) + rt * 128 + ((((ch >> 1) & 7) ^ (rt & 7)) << 4) + (ch & 1) * 8;
+                            *reinterpret_cast<uint2*>(out + at) = hi;
+                            *reinterpret_cast<uint2*>(out + F::kSlotPart + at) = lo;
+                        }
+                    }
+                    if (bad) M.vbad[walk.count & 15] = 1;
+                    if (is_v) {
+#pragma unroll
+                        for (int d = 16; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
+                        if (lane == 0) M.vmax[meta][lw] = big;
+                    }
+                    raw_out = raw_out + 1 == F::kRawDepth ? 0 : raw_out + 1;
+                    proxy_fence();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (is_v) bar_arrive(&M.v_ready[meta]);
+                        bar_arrive(&M.full[slot]);
+                    }
+                    slot = slot + 1 == F::kBase ? 0 : slot + 1;
+                }
+            }
+            cp_wait<0>();
+        }
+        if (flags) atomicOr(a.status, flags);
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if (warp == kTreeMmaWarp && lane == 0) {
+            // -------------------------------------------------- MMA issue
+            constexpr unsigned kIdescS = (1u << 4) | (unsigned(F::kBn >> 3) << 17) | (8u << 24);
+            constexpr unsigned kIdescO = (1u << 4) | (1u << 16) | (unsigned(DP >> 3) << 17) | (8u << 24);
+            unsigned full_phase = 0, n_p[2] = {0, 0}, pieces = 0;
+            int slot = 0;
+            bool go = true;
+            const auto qk = [&](int q_tile, int stream, unsigned at) {
+                const unsigned d = tmem + stream * 128, q_lo = smem + q_tile * F::kQTile + F::kQPart,
+                               q_hi = smem + q_tile * F::kQTile, k = smem + at;
+                int acc = 0;
+#pragma unroll 1
+                for (int part = 0; part < F::kParts + 1; ++part) {
+                    // small products first: lo Q (and lo K) before hi hi
+                    const unsigned qa = part == 0 ? q_lo : q_hi, kb = F::kParts == 2 && part == 1 ? k + F::kSlotPart : k;
+#pragma unroll
+                    for (int kk = 0; kk < DP / 16; ++kk) {
+                        mma_ss(d, sw128_desc(qa + (kk >> 2) * 16384 + (kk & 3) * 32, 16),
+                               sw128_desc(kb + (kk >> 2) * (F::kBn * 128) + (kk & 3) * 32, 16), kIdescS, acc);
+                        acc = 1;
+                    }
+                }
+            };
+            const auto pv = [&](int stream, unsigned at) {
+                const unsigned d = tmem + 256 + stream * 128, p = tmem + stream * 128, v = smem + at;
+                int acc = 0;
+#pragma unroll 1
+                for (int part = 0; part < F::kParts + 1; ++part) {
+                    const unsigned pa = part == 0 ? p + F::kBn / 2 : p, vb = F::kParts == 2 && part == 1 ? v + F::kSlotPart : v;
+#pragma unroll
+                    for (int kk = 0; kk < F::kBn / 16; ++kk) {
+                        mma_ts(d, pa + kk * 8, sw128_desc(vb + kk * 2048, F::kBn * 128), kIdescO, acc);
+                        acc = 1;
+                    }
+                }
+            };
+            const auto take = [&](int ns) -> int {  // next ring slot, filled
+                const int s = slot;
+                go = bar_wait(&M.full[s], (full_phase >> s) & 1, abort_flag, a.status);
+                full_phase ^= 1u << s;
+                slot = s + 1 == ns ? 0 : s + 1;
+                tm_after();
+                return s;
+            };
+            while (go && walk.next(a)) {
+                const bool pair = walk.q.pair;
+                const int ns = pair ? F::kBase : F::kBase + F::kExtra, tiles = int(walk.t1 - walk.t0);
+                if (slot >= ns) slot = 0;
+                go = bar_wait(&M.q_full, pieces & 1, abort_flag, a.status);
+                ++pieces;
+                if (!go) break;
+                tm_after();
+                if (!pair) {
+                    for (int j = 0; j < min(2, tiles) && go; ++j) {
+                        const int s = take(ns);
+                        if (!go) break;
+                        qk(0, j, slot_at(s));
+                        tree_commit_to(&M.empty[s]);
+                        tree_commit_to(&M.s_full[j]);
+                    }
+                    for (int j = 0; j < tiles && go; ++j) {
+                        const int st = j & 1;
+                        const int s = take(ns);
+                        if (!go) break;
+                        go = bar_wait(&M.p_full[st], n_p[st] & 1, abort_flag, a.status);
+                        ++n_p[st];
+                        if (!go) break;
+                        tm_after();
+                        pv(st, slot_at(s));
+                        tree_commit_to(&M.empty[s]);
+                        tree_commit_to(&M.o_full[st]);
+                        if (j + 2 < tiles) {
+                            const int s2 = take(ns);
+                            if (!go) break;
+                            qk(0, st, slot_at(s2));
+                            tree_commit_to(&M.empty[s2]);
+                            tree_commit_to(&M.s_full[st]);
+                        }
+                    }
+                } else {
+                    int s = take(ns);
+                    if (!go) break;
+                    for (int st = 0; st < 2; ++st) {
+                        qk(st, st, slot_at(s));
+                        tree_commit_to(&M.s_full[st]);
+                    }
+                    tree_commit_to(&M.empty[s]);
+                    for (int j = 0; j < tiles && go; ++j) {
+                        s = take(ns);
+                        if (!go) break;
+                        int s2 = -1;
+                        for (int st = 0; st < 2 && go; ++st) {
+                            go = bar_wait(&M.p_full[st], n_p[st] & 1, abort_flag, a.status);
+                            ++n_p[st];
+                            if (!go) break;
+                            tm_after();
+                            pv(st, slot_at(s));
+                            tree_commit_to(&M.o_full[st]);
+                            if (st == 1) tree_commit_to(&M.empty[s]);
+                            if (j + 1 < tiles) {
+                                if (st == 0) s2 = take(ns);
+                                if (!go) break;
+                                qk(st, st, slot_at(s2));
+                                tree_commit_to(&M.s_full[st]);
+                                if (st == 1) tree_commit_to(&M.empty[s2]);
+                            }
+                        }
+                    }
+                }
+                if (!go) break;
+                tree_commit_to(&M.item_done);
+            }
+            // nothing of this CTA's may be in flight when its memory is given back
+            tree_commit_to(&M.drain);
+            for (unsigned i = 0; i < kTreeSpin && !bar_test(&M.drain, 0); ++i) {
+            }
+        }
+        __syncwarp();
+    }
+    tm_before();
+    __syncthreads();
+    if (warp == kTreeMmaWarp) {
+        tm_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    }
+}
+
+// Items cut by run boundaries: out = sum_i O_i 2^(m_i - M) / sum_i l_i 2^(m_i - M)
+// over the pieces in order (a fixed order, so results repeat bit for bit).
+// Block (b, y) takes rows 8 y .. 8 y + 7 of the item that starts in CTA b.
+template <int DP>
+__global__ void __launch_bounds__(256) tree_combine_kernel(TreeAttn a, const float* partial, const TreeRec* recs) {
+    const TreeRec rec = recs[blockIdx.x];
+    const int row = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (rec.pieces < 2 || row >= rec.rows) return;
+    const int pr = row < rec.split ? row : 128 + row - rec.split, group = a.hq / a.hkv;
+    constexpr int kPer = DP / 32;
+    const long long slot_floats = (long long)kTreeRows * (DP + 2);
+    const auto slot_of = [&](int i) { return partial + (2ll * (blockIdx.x + i) + (i == 0)) * slot_floats; };
+    float top = -INFINITY;
+    for (int i = 0; i < rec.pieces; ++i) top = fmaxf(top, slot_of(i)[kTreeRows * DP + pr]);
+    float l = 0.f, o[kPer] = {};
+    if (top != -INFINITY) {
+        for (int i = 0; i < rec.pieces; ++i) {
+            const float* slot = slot_of(i);
+            const float f = ex2(slot[kTreeRows * DP + pr] - top);
+            l += slot[kTreeRows * DP + kTreeRows + pr] * f;
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) o[e] += slot[pr * DP + e * 32 + lane] * f;
+        }
+    } else {  // nothing seen, or nothing but NaN scores
+        for (int i = 0; i < rec.pieces; ++i) l += slot_of(i)[kTreeRows * DP + kTreeRows + pr];
+    }
+    const int vec = rec.row0 + row, node = vec / group, head = rec.head * group + vec - node * group;
+    float* dst = a.out + (long long)(rec.c0 + node) * a.ldo + (long long)head * a.dim;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e)
+        if (e * 32 + lane < a.dim) dst[e * 32 + lane] = l == 0.f && top == -INFINITY ? 0.f : o[e] / l;
+}
+
+int tree_ctas() {
+    int device = 0, sms = 0;
+    TVARA_CUDA(cudaGetDevice(&device));
+    TVARA_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+    return sms;
+}
+
+constexpr int kTreeMaxCtas = 148;
+
+template <int KV, int DP>
+void run_tree_mma(const TreeAttn& a, void* workspace, cudaStream_t s) {
+    using F = TreeForm<KV, DP>;
+    const int ctas = std::min(tree_ctas(), kTreeMaxCtas);
+    auto* recs = static_cast<TreeRec*>(workspace);
+    auto* partial = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + 4096);
+    TVARA_CUDA(cudaFuncSetAttribute(tree_mma_kernel<KV, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem));
+    tree_mma_kernel<KV, DP><<<ctas, kTreeThreads, F::kSmem, s>>>(a, partial, recs, 2);
+    TVARA_LAUNCHED();
+    tree_combine_kernel<DP><<<dim3(unsigned(ctas), kTreeRows / 8), 256, 0, s>>>(a, partial, recs);
+    TVARA_LAUNCHED();
+}
+
+// The tensor-core form reads rows in 16-byte pieces.
+bool tree_mma_takes(const TreeAttn& a) {
+    const auto at = [](const void* p) { return reinterpret_cast<std::uintptr_t>(p); };
+    const int elem = a.kv_kind == 0 ? 4 : a.kv_kind == 1 ? 2 : 1;
+    return a.dim <= 128 && a.dim * elem % 16 == 0 && a.dim % 4 == 0 && at(a.kv) % 16 == 0 && at(a.q) % 16 == 0 &&
+           at(a.out) % 16 == 0 && a.ldq % 4 == 0 && a.ldo % 4 == 0;
+}
+
 }  // namespace
 
-std::size_t tree_attention_workspace(const TreeAttn&) { return 256; }
+std::size_t tree_attention_workspace(const TreeAttn& a) {
+    static_assert(sizeof(TreeRec) * kTreeMaxCtas <= 4096);
+    const int dp = a.dim <= 64 ? 64 : 128;
+    return a.dim <= 128 ? 4096 + std::size_t(2) * kTreeMaxCtas * kTreeRows * (dp + 2) * 4 : 256;
+}
 
-void launch_tree_attention(const TreeAttn& a, void*, cudaStream_t s) {
+void launch_tree_attention(const TreeAttn& a, void* workspace, cudaStream_t s) {
+    if (tree_mma_takes(a)) {
+        if (a.dim <= 64) {
+            if (a.kv_kind == 0) return run_tree_mma<0, 64>(a, workspace, s);
+            if (a.kv_kind == 1) return run_tree_mma<1, 64>(a, workspace, s);
+            return run_tree_mma<2, 64>(a, workspace, s);
+        }
+        if (a.kv_kind == 0) return run_tree_mma<0, 128>(a, workspace, s);
+        if (a.kv_kind == 1) return run_tree_mma<1, 128>(a, workspace, s);
+        return run_tree_mma<2, 128>(a, workspace, s);
+    }
     const dim3 grid(unsigned(a.capacity), unsigned(a.hq));
     if (a.dim <= 32)
         tree_any_kernel<1><<<grid, kAnyWarps * 32, 0, s>>>(a);

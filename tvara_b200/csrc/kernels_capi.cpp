@@ -463,6 +463,7 @@ int tvara_tree_attention(const tvara_tree_attention_args* a, void* workspace, si
             throw std::invalid_argument("invalid KV dtype or missing int8 scales");
         if (!workspace || workspace_bytes < tvara::tree_attention_workspace(j))
             throw std::invalid_argument("attention workspace too small");
+        if (reinterpret_cast<std::uintptr_t>(workspace) % 16) throw std::invalid_argument("attention workspace is not 16-byte aligned");
         if (!a->capacity) return;
         tvara::launch_tree_attention(j, workspace, static_cast<cudaStream_t>(stream));
     });
