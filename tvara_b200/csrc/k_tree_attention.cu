@@ -24,7 +24,7 @@ __device__ __forceinline__ bool tree_sequence_ok(const TreeAttn& a, int s, int& 
     const long long rows = (long long)c1 - c0;
     n = int(rows);
     return c0 >= 0 && rows >= 0 && rows <= a.max_nodes && c1 <= a.capacity && len >= 0 &&
-           len <= (long long)a.stride * a.bt && len <= 0x7fffffff - kTreeMaxNodes;
+           len <= (long long)a.stride * a.bt && len <= 0x7fffffff - 2 * kTreeMaxNodes;
 }
 
 // Element offset of the K row (head 0 of the layer) of index p of a sequence
@@ -174,12 +174,16 @@ __global__ void __launch_bounds__(kAnyWarps * 32) tree_any_kernel(TreeAttn a) {
 // (each CTA scans the lengths and cuts out its run), so ragged batches and a
 // single long sequence fill the device alike; an item cut by a run boundary
 // leaves partial (O, m, l) in the workspace for tree_combine_kernel.
-constexpr int kTreeThreads = 512;   // WG0, WG1 softmax; WG2 loads; WG3 warp 12 issues the MMAs
+constexpr int kTreeThreads = 512;   // WG0, WG1 softmax; WG2 loads; warp 12 issues the MMAs, warp 13 deals the pieces
 constexpr int kTreeMmaWarp = 12;
+constexpr int kTreePieceWarp = 13;
 constexpr int kTreeLoadWarp = 8;
-constexpr unsigned kTreeSpin = 1u << 22;
+constexpr unsigned kTreeSpin = 1u << 26;
 constexpr int kTreeRows = 256;      // query vectors of a partial slot
+constexpr int kPieceRing = 4;
 constexpr int kMetaRing = 8;        // tiles of column masks and int8 scales kept
+
+constexpr int kTreeMetaBytes = 1024;
 
 template <int KV, int DP>
 struct TreeForm {  // KV: 0 F32, 1 F16, 2 int8
@@ -201,27 +205,57 @@ struct TreeForm {  // KV: 0 F32, 1 F16, 2 int8
     static constexpr int kOffRaw = kOffSlots + kBase * kSlot;
     static constexpr int kOffScale = kOffRaw + kRawDepth * kRaw;
     static constexpr int kOffMeta = kOffScale + kScaleRing * 2 * kBn * 4;
-    static constexpr int kSmem = kOffMeta + 1024;
+    static constexpr int kSmem = kOffMeta + kTreeMetaBytes;
     static_assert(kExtra * kSlot <= kQTile || !kPairs);
     static_assert(kSmem <= 232448);
+};
+
+// One piece of an item: tiles [t0, t1) of it run in this CTA.
+struct TreePiece {
+    int s, c0, n, len;
+    int t0, t1, whole;            // whole: the item begins and ends here
+    int head, row0, rows, split;  // split: vectors of the first M tile; rows 0 ends the list
+    int pair;
+    unsigned tile_base, count;    // tiles and pieces before this one
+
+    // Entry e of the piece's 2 (t1 - t0) loads, in the order of their use:
+    // K runs two tiles (one with two M tiles) ahead of V.
+    __device__ __forceinline__ int entry(int e, bool& is_v) const {
+        const int c = t1 - t0, ahead = min(pair ? 1 : 2, c);
+        if (e < ahead) {
+            is_v = false;
+            return e;
+        }
+        const int f = e - ahead;
+        if (f < 2 * (c - ahead)) {
+            is_v = !(f & 1);
+            return is_v ? f >> 1 : (f >> 1) + ahead;
+        }
+        is_v = true;
+        return c - ahead + (f - 2 * (c - ahead));
+    }
 };
 
 struct TreeMeta {  // at kOffMeta
     std::uint64_t full[8], empty[8];
     std::uint64_t s_full[2], p_full[2], o_full[2];
     std::uint64_t v_ready[kMetaRing];  // a tile's V scales are in place (F32, int8)
-    std::uint64_t q_full, item_done, merge_ready, merge_read, drain;
+    std::uint64_t q_full, merge_ready, merge_read, drain;
+    std::uint64_t piece_full[kPieceRing], piece_empty[kPieceRing];
+    union {
+        TreePiece piece[kPieceRing];
+        long long warp_sum[16];  // while the run is cut out
+    };
     alignas(16) unsigned valid[kMetaRing][4];   // columns of a tile that hold a row
     alignas(16) float vmax[kMetaRing][4];       // largest V scale per load warp
     int vbad[16];                   // an item's nodes hold a non-finite V
-    long long warp_sum[16];
     long long total, excl0, excl1;
     int seq0, seq1;
     unsigned tmem;
     int abort_flag;
     int bad;
 };
-static_assert(sizeof(TreeMeta) <= 1024);
+static_assert(sizeof(TreeMeta) <= kTreeMetaBytes);
 
 struct TreeRec {  // an item that continues in the next CTAs, by the CTA it starts in
     int c0, row0, rows, split, head, pieces;
@@ -281,6 +315,14 @@ __device__ __forceinline__ void tm_ld32(unsigned addr, unsigned (&r)[32]) {
           "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
           "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tm_ld16(unsigned addr, unsigned (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(addr));
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
@@ -353,69 +395,6 @@ __device__ __forceinline__ bool tree_seq(const TreeAttn& a, int s, TreeSeq& q) {
     return true;
 }
 
-// One piece of an item: tiles [t0, t1) of it run in this CTA.
-template <class F>
-struct TreeWalk {
-    TreeSeq q;
-    long long u, u_end;
-    int seq1;
-    long long u1;
-    long long t0, t1;
-    int head, row0, rows, split;  // split: vectors of the first M tile
-    long long item;
-    int count;                    // pieces begun, minus one
-    long long tile_base;          // tiles of earlier pieces
-
-    __device__ __forceinline__ void start(const TreeAttn& a, int seq0, long long u0, int last_seq, long long last_u) {
-        seq1 = last_seq;
-        u1 = last_u;
-        count = -1;
-        tile_base = 0;
-        t0 = t1 = 0;
-        tree_seq<F>(a, seq0, q);
-        u = u0;
-        u_end = seq0 == seq1 ? u1 : q.total;
-    }
-    __device__ __forceinline__ bool next(const TreeAttn& a) {
-        tile_base += t1 - t0;
-        while (u >= u_end) {
-            if (q.s >= seq1 || q.s + 1 >= a.n_seq) return false;
-            tree_seq<F>(a, q.s + 1, q);
-            u = 0;
-            u_end = q.s == seq1 ? min(u1, q.total) : q.total;
-        }
-        item = u / q.tiles;
-        t0 = u - item * q.tiles;
-        t1 = min(q.tiles, t0 + (u_end - u));
-        u += t1 - t0;
-        head = int(item / q.groups);
-        const int grp = int(item - (long long)head * q.groups), vectors = q.n * (a.hq / a.hkv);
-        // groups of nearly equal size, and M tiles of nearly equal size
-        const int per = (vectors + q.groups - 1) / q.groups;
-        row0 = grp * per;
-        rows = min(per, vectors - row0);
-        split = q.pair ? (rows + 1) / 2 : rows;
-        ++count;
-        return true;
-    }
-    // Entry e of the piece's 2 (t1 - t0) loads, in the order of their use:
-    // K runs `ahead` tiles before V.
-    __device__ __forceinline__ int entry(int e, bool& is_v) const {
-        const int c = int(t1 - t0), ahead = min(q.pair ? 1 : 2, c);
-        if (e < ahead) {
-            is_v = false;
-            return e;
-        }
-        const int f = e - ahead;
-        if (f < 2 * (c - ahead)) {
-            is_v = !(f & 1);
-            return is_v ? f >> 1 : (f >> 1) + ahead;
-        }
-        is_v = true;
-        return c - ahead + (f - 2 * (c - ahead));
-    }
-};
-
 // Bits [j0, j0 + 32) of the mask row of node `node` (negative j0: cached
 // positions, visible), columns behind the last node cleared.
 __device__ __forceinline__ unsigned node_bits(const TreeAttn& a, int c0, int n, int node, long long j0) {
@@ -459,8 +438,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
             bar_init(&M.p_full[i], 4);
             bar_init(&M.o_full[i], 1);
         }
+        for (int i = 0; i < kPieceRing; ++i) {
+            bar_init(&M.piece_full[i], 1);
+            bar_init(&M.piece_empty[i], 13);  // 8 softmax warps, 4 load warps, the MMA thread
+        }
         bar_init(&M.q_full, 8);
-        bar_init(&M.item_done, 1);
         bar_init(&M.merge_ready, 4);
         bar_init(&M.merge_read, 4);
         bar_init(&M.drain, 1);
@@ -528,65 +510,128 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
     tm_after();
     const unsigned tmem = M.tmem;
     volatile int* abort_flag = &M.abort_flag;
-    TreeWalk<F> walk;
-    {
-        TreeSeq q;
-        tree_seq<F>(a, M.seq0, q);
-        const long long u0 = (w0 - M.excl0 + q.weight - 1) / q.weight;
-        tree_seq<F>(a, M.seq1, q);
-        const long long u1 = (w1 - M.excl1 + q.weight - 1) / q.weight;
-        walk.start(a, M.seq0, u0, M.seq1, u1);
+    if (warp >= kTreeMmaWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    if (warp == kTreePieceWarp) {
+        // --------------------------------------------------------- pieces
+        if (lane == 0) {
+            const int seq1 = M.seq1;
+            TreeSeq q;
+            tree_seq<F>(a, seq1, q);
+            const long long u1 = min(q.total, (w1 - M.excl1 + q.weight - 1) / q.weight);
+            tree_seq<F>(a, M.seq0, q);
+            long long u = (w0 - M.excl0 + q.weight - 1) / q.weight;
+            unsigned count = 0, tile_base = 0;
+            bool go = true;
+            for (int seq = M.seq0; go; ++count) {
+                long long end = seq == seq1 ? u1 : q.total;
+                while (u >= end && seq < seq1) {
+                    u = 0;
+                    tree_seq<F>(a, ++seq, q);
+                    end = seq == seq1 ? u1 : q.total;
+                }
+                const int ring = count % kPieceRing;
+                go = bar_wait(&M.piece_empty[ring], (count / kPieceRing & 1) ^ 1, abort_flag, a.status);
+                if (!go) break;
+                TreePiece& p = M.piece[ring];
+                if (u >= end) {
+                    p.rows = 0;
+                    bar_arrive(&M.piece_full[ring]);
+                    break;
+                }
+                const long long item = u / q.tiles;
+                const int t0 = int(u - item * q.tiles), t1 = int(min(q.tiles, t0 + (end - u)));
+                u += t1 - t0;
+                const int head = int(item / q.groups), grp = int(item - (long long)head * q.groups);
+                // groups of nearly equal size, and M tiles of nearly equal size
+                const int vectors = q.n * group, per = (vectors + q.groups - 1) / q.groups;
+                const int row0 = grp * per, rows = min(per, vectors - row0);
+                p.s = seq;
+                p.c0 = q.c0;
+                p.n = q.n;
+                p.len = q.len;
+                p.t0 = t0;
+                p.t1 = t1;
+                p.whole = t0 == 0 && t1 == q.tiles;
+                p.head = head;
+                p.row0 = row0;
+                p.rows = rows;
+                p.split = q.pair ? (rows + 1) / 2 : rows;
+                p.pair = q.pair;
+                p.tile_base = tile_base;
+                p.count = count;
+                bar_arrive(&M.piece_full[ring]);
+                tile_base += unsigned(t1 - t0);
+                if (t0 == 0 && t1 < q.tiles) {  // continues in other CTAs: up to the one its last tile starts in
+                    const long long last = M.excl1 + (item * q.tiles + q.tiles - 1) * q.weight;
+                    TreeRec rec;
+                    rec.c0 = q.c0;
+                    rec.row0 = row0;
+                    rec.rows = rows;
+                    rec.split = p.split;
+                    rec.head = head;
+                    rec.pieces = int(((last + 1) * ctas + total - 1) / total - 1) - cta + 1;
+                    recs[cta] = rec;
+                }
+            }
+        }
+        __syncwarp();
     }
     const unsigned smem = sm_addr(tree_smem);
     const auto slot_at = [&](int slot) -> unsigned {
         return slot < F::kBase ? F::kOffSlots + slot * F::kSlot : F::kQTile + (slot - F::kBase) * F::kSlot;
     };
 
+    // Piece i of the run is in M.piece[i % kPieceRing] until every role has released it; rows 0 ends the run.
+    const auto get_piece = [&](unsigned i) -> bool {
+        return bar_wait(&M.piece_full[i % kPieceRing], (i / kPieceRing) & 1, abort_flag, a.status) &&
+               M.piece[i % kPieceRing].rows != 0;
+    };
+    const auto release_piece = [&](unsigned i) { bar_arrive(&M.piece_empty[i % kPieceRing]); };
+
     if (warp < kTreeLoadWarp) {
         // ------------------------------------------------ softmax warpgroups
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         const int stream = warp >> 2, wq = warp & 3, r = tid & 127;
         const unsigned lane_base = tmem + (unsigned(wq * 32) << 16);
         const unsigned s_at = lane_base + stream * 128, o_at = lane_base + 256 + stream * 128;
         const float score_unit = 1.4426950408889634f / sqrtf(float(a.dim));
-        unsigned n_s = 0, n_o = 0;  // completed waits on s_full / o_full
+        unsigned n_s = 0;  // tiles of this stream so far
         bool go = true;
         float o[DP];
-        while (go && walk.next(a)) {
-            const TreeSeq& q = walk.q;
-            const int tile_rows = q.pair ? (stream ? walk.rows - walk.split : walk.split) : walk.rows;
-            const int row = q.pair && stream ? walk.split + r : r;  // vector of the item
+        for (unsigned piece = 0;; ++piece) {
+            go = __all_sync(0xffffffffu, get_piece(piece));
+            if (!go) break;
+            const TreePiece& q = M.piece[piece % kPieceRing];
+            const int tile_rows = q.pair ? (stream ? q.rows - q.split : q.split) : q.rows;
+            const int first_row = q.row0 + (q.pair && stream ? q.split : 0);  // this stream's rows within the sequence
+            const int node = (first_row + r) / group;
             const bool live = r < tile_rows, warp_live = wq * 32 < tile_rows;
-            const int vec = walk.row0 + row, node = live ? vec / group : 0;
-            const int head = walk.head * group + (vec - node * group);
-            // the query vector, scaled below 2^15 and split, into this stream's Q tile
+            // The warp's query vectors, one at a time across its lanes: scaled
+            // below 2^15, split, into this stream's Q tile; lane i keeps the
+            // score factor of vector i.
             float c = 0.f;
-            if (live) {
-                const float4* src = reinterpret_cast<const float4*>(a.q + (long long)(q.c0 + node) * a.ldq + (long long)head * a.dim);
-                float top = 0.f;
-                const int quads = a.dim >> 2;
-#pragma unroll 8
-                for (int i = 0; i < quads; ++i) {
-                    const float4 v = __ldg(src + i);
-                    top = fmaxf(fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
-                }
-                const int up = lift(top);
-                c = score_unit * two_to(-up);
-                if (stream == 0 || q.pair) {
-                    const float f = two_to(up);
-                    unsigned char* tile = tree_smem + (stream ? F::kQTile : 0);
+            if (warp_live) {
+                const int quads = a.dim >> 2, most = min(32, tile_rows - wq * 32);
+                unsigned char* tile = tree_smem + (q.pair && stream ? F::kQTile : 0);
 #pragma unroll 4
-                    for (int i = 0; i < DP / 8; ++i) {
-                        const float4 x = 2 * i < quads ? __ldg(src + 2 * i) : make_float4(0, 0, 0, 0);
-                        const float4 y = 2 * i + 1 < quads ? __ldg(src + 2 * i + 1) : make_float4(0, 0, 0, 0);
-                        uint4 hi, lo;
+                for (int i = 0; i < most; ++i) {
+                    const int v = first_row + wq * 32 + i, nd = v / group, hd = q.head * group + v - nd * group;
+                    const float4* src =
+                        reinterpret_cast<const float4*>(a.q + (long long)(q.c0 + nd) * a.ldq + (long long)hd * a.dim);
+                    const float4 x = lane < quads ? __ldg(src + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    float top = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+                    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+                    const int up = lift(top);
+                    if (lane == i) c = score_unit * two_to(-up);
+                    if ((stream == 0 || q.pair) && lane < DP / 4) {
+                        const float f = two_to(up);
+                        uint2 hi, lo;
                         split_exact(x.x * f, x.y * f, hi.x, lo.x);
                         split_exact(x.z * f, x.w * f, hi.y, lo.y);
-                        split_exact(y.x * f, y.y * f, hi.z, lo.z);
-                        split_exact(y.z * f, y.w * f, hi.w, lo.w);
-                        const int at = (i >> 3) * 16384 + r * 128 + (((i & 7) ^ (r & 7)) << 4);
-                        *reinterpret_cast<uint4*>(tile + at) = hi;
-                        *reinterpret_cast<uint4*>(tile + F::kQPart + at) = lo;
+                        const int row = wq * 32 + i, ch = lane >> 1;
+                        const int at = (ch >> 3) * 16384 + row * 128 + (((ch & 7) ^ (row & 7)) << 4) + (lane & 1) * 8;
+                        *reinterpret_cast<uint2*>(tile + at) = hi;
+                        *reinterpret_cast<uint2*>(tile + F::kQPart + at) = lo;
                     }
                 }
             }
@@ -596,29 +641,28 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
             float m = -INFINITY, l = 0.f, vref = 0.f;
 #pragma unroll
             for (int i = 0; i < DP; ++i) o[i] = 0.f;
-            const int tiles = int(walk.t1 - walk.t0);
-            const int first = q.pair ? 0 : stream, step = q.pair ? 1 : 2;
-            for (int j = first; j < tiles && go; j += step) {
-                go = __all_sync(0xffffffffu, bar_wait(&M.s_full[stream], n_s & 1, abort_flag, a.status));
-                ++n_s;
-                if constexpr (KV != 1) {
-                    const long long t = walk.tile_base + j;
-                    go = go && __all_sync(0xffffffffu, bar_wait(&M.v_ready[t % kMetaRing], (t / kMetaRing) & 1, abort_flag, a.status));
-                }
+            const int tiles = q.t1 - q.t0;
+            for (int j = q.pair ? 0 : stream; j < tiles && go; j += q.pair ? 1 : 2, ++n_s) {
+                const unsigned t = q.tile_base + j;
+                go = bar_wait(&M.s_full[stream], n_s & 1, abort_flag, a.status);
+                if constexpr (KV != 1)
+                    go = go && bar_wait(&M.v_ready[t % kMetaRing], (t / kMetaRing) & 1, abort_flag, a.status);
+                go = __all_sync(0xffffffffu, go);
                 if (!go) break;
                 tm_after();
+                float keep = 1.f;
                 if (warp_live) {
-                    const long long p0 = (walk.t0 + j) * F::kBn;
-                    const int ring = int((walk.tile_base + j) % kMetaRing);
+                    const int ring = t % kMetaRing;
+                    const long long p0 = (long long)(q.t0 + j) * F::kBn;
                     const bool nodes = p0 + F::kBn > q.len;
                     unsigned seen[F::kBn / 32];
 #pragma unroll
                     for (int k = 0; k < F::kBn / 32; ++k) {
                         seen[k] = M.valid[ring][k];
-                        if (nodes) seen[k] &= node_bits(a, q.c0, q.n, node, p0 + 32 * k - q.len);
+                        if (nodes) seen[k] &= node_bits(a, q.c0, q.n, live ? node : 0, p0 + 32 * k - q.len);
                     }
                     const float* k_scale = reinterpret_cast<const float*>(tree_smem + F::kOffScale) +
-                                           int((walk.tile_base + j) % max(1, F::kScaleRing)) * 2 * F::kBn;
+                                           t % (F::kScaleRing ? F::kScaleRing : 1) * 2 * F::kBn;
                     const float* v_scale = k_scale + F::kBn;
                     float top = -INFINITY;
 #pragma unroll
@@ -635,103 +679,89 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
                                 x[i + 3] = __float_as_uint(__uint_as_float(x[i + 3]) * f.w);
                             }
                         }
-                        if (seen[k] == 0xffffffffu) {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(x[i]));
-                        } else {
+                        if (seen[k] != 0xffffffffu) {
 #pragma unroll
                             for (int i = 0; i < 32; ++i)
-                                if (seen[k] >> i & 1) top = fmaxf(top, __uint_as_float(x[i]));
+                                if (!(seen[k] >> i & 1)) x[i] = 0xff800000u;
                         }
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(x[i]));
                     }
                     const float mn = fmaxf(m, top * c);
-                    float keep = mn == -INFINITY ? 1.f : ex2(m - mn);
-                    const float off = 11.f - (mn == -INFINITY ? 0.f : mn);
+                    const float off = mn == -INFINITY ? 11.f : 11.f - mn;
+                    keep = mn == -INFINITY ? 1.f : ex2(m - mn);
                     m = mn;
                     l *= keep;
                     float v_unit = 1.f;
                     if constexpr (KV != 1) {
-                        const float4 t = *reinterpret_cast<const float4*>(M.vmax[ring]);
-                        const float big = fmaxf(fmaxf(vref, fmaxf(t.x, t.y)), fmaxf(t.z, t.w));
+                        const float4 big4 = *reinterpret_cast<const float4*>(M.vmax[ring]);
+                        const float big = fmaxf(fmaxf(vref, fmaxf(big4.x, big4.y)), fmaxf(big4.z, big4.w));
                         if (big > vref) {
                             keep *= vref / big;
                             vref = big;
                         }
                         v_unit = vref > 0.f ? 1.f / vref : 0.f;
                     }
+                    // P over S, sixteen positions (one K step of the MMA) at a
+                    // time: hi in their first eight columns, lo in the others.
                     float sum0 = 0.f, sum1 = 0.f;
-                    unsigned hold[2][16];  // lo halves waiting for their columns of S to be read
 #pragma unroll
-                    for (int k = 0; k < F::kBn / 32; ++k) {
-                        unsigned x[32], hi[16], lo[16];
-                        tm_ld32(s_at + 32 * k, x);
-                        const unsigned see = seen[k];
+                    for (int w = 0; w < F::kBn / 32; ++w) {
+                        const unsigned see = seen[w];
+#pragma unroll 1
+                        for (int k = 2 * w; k < 2 * w + 2; ++k) {
+                            unsigned x[16], y[16];
+                            tm_ld16(s_at + 16 * k, x);
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            float p[4];
-                            float4 ks, vs;
-                            if constexpr (KV != 1) {
-                                ks = *reinterpret_cast<const float4*>(k_scale + 32 * k + i);
-                                vs = *reinterpret_cast<const float4*>(v_scale + 32 * k + i);
-                            }
+                            for (int i = 0; i < 16; i += 4) {
+                                float p[4];
+                                float4 ks, vs;
+                                if constexpr (KV != 1) {
+                                    ks = *reinterpret_cast<const float4*>(k_scale + 16 * k + i);
+                                    vs = *reinterpret_cast<const float4*>(v_scale + 16 * k + i);
+                                }
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                float s = __uint_as_float(x[i + e]);
-                                if constexpr (KV != 1) s *= e == 0 ? ks.x : e == 1 ? ks.y : e == 2 ? ks.z : ks.w;
-                                p[e] = ex2(fmaf(s, c, off));
-                            }
-                            if (see != 0xffffffffu) {
-#pragma unroll
-                                for (int e = 0; e < 4; ++e)
-                                    if (!(see >> (i + e) & 1)) p[e] = 0.f;
-                            }
-                            sum0 += p[0] + p[2];
-                            sum1 += p[1] + p[3];
-                            if constexpr (KV != 1) {
-                                p[0] *= vs.x * v_unit;
-                                p[1] *= vs.y * v_unit;
-                                p[2] *= vs.z * v_unit;
-                                p[3] *= vs.w * v_unit;
-                                if (see != 0xffffffffu) {  // a masked row's scale may be anything
+                                for (int e = 0; e < 4; ++e) {
+                                    float sc = __uint_as_float(x[i + e]);
+                                    if constexpr (KV != 1) sc *= e == 0 ? ks.x : e == 1 ? ks.y : e == 2 ? ks.z : ks.w;
+                                    p[e] = ex2(fmaf(sc, c, off));
+                                }
+                                if (see != 0xffffffffu) {
+                                    const unsigned bits = see >> ((k & 1) * 16 + i);
 #pragma unroll
                                     for (int e = 0; e < 4; ++e)
-                                        if (!(see >> (i + e) & 1)) p[e] = 0.f;
+                                        if (!(bits >> e & 1)) p[e] = 0.f;
                                 }
-                            }
-                            split_weight(p[0], p[1], hi[i / 2], lo[i / 2]);
-                            split_weight(p[2], p[3], hi[i / 2 + 1], lo[i / 2 + 1]);
-                        }
-                        // hi half k in columns 16 k.., lo half k in kBn / 2 + 16 k..: written once those are read
-                        tm_st16(s_at + 16 * k, hi);
-                        constexpr int kHalf = F::kBn / 64;  // chunks before the upper half of S
-                        if (k < kHalf) {
+                                sum0 += p[0] + p[2];
+                                sum1 += p[1] + p[3];
+                                if constexpr (KV != 1) {
+                                    p[0] *= vs.x * v_unit;
+                                    p[1] *= vs.y * v_unit;
+                                    p[2] *= vs.z * v_unit;
+                                    p[3] *= vs.w * v_unit;
+                                    if (see != 0xffffffffu) {  // a masked row's scale may be anything
+                                        const unsigned bits = see >> ((k & 1) * 16 + i);
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) hold[k][i] = lo[i];
-                        } else {
-                            // chunk k read: columns below 32 (k + 1) are free, lo halves up to 2 (k - kHalf) + 1 fit
-                            if (F::kBn == 64) {
-                                tm_st16(s_at + 32, hold[0]);
-                                tm_st16(s_at + 48, lo);
-                            } else if (k == 2) {
-                                tm_st16(s_at + 64, hold[0]);
-                                tm_st16(s_at + 80, hold[1]);
-#pragma unroll
-                                for (int i = 0; i < 16; ++i) hold[0][i] = lo[i];
-                            } else {
-                                tm_st16(s_at + 96, hold[0]);
-                                tm_st16(s_at + 112, lo);
+                                        for (int e = 0; e < 4; ++e)
+                                            if (!(bits >> e & 1)) p[e] = 0.f;
+                                    }
+                                }
+                                split_weight(p[0], p[1], y[i / 2], y[8 + i / 2]);
+                                split_weight(p[2], p[3], y[i / 2 + 1], y[8 + i / 2 + 1]);
                             }
+                            tm_st16(s_at + 16 * k, y);
                         }
                     }
                     l += sum0 + sum1;
                     tm_wait_st();
-                    tm_before();
-                    __syncwarp();
-                    if (lane == 0) bar_arrive(&M.p_full[stream]);
-                    go = __all_sync(0xffffffffu, bar_wait(&M.o_full[stream], n_o & 1, abort_flag, a.status));
-                    ++n_o;
-                    if (!go) break;
-                    tm_after();
+                }
+                tm_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&M.p_full[stream]);
+                go = __all_sync(0xffffffffu, bar_wait(&M.o_full[stream], n_s & 1, abort_flag, a.status));
+                if (!go) break;
+                tm_after();
+                if (warp_live) {
 #pragma unroll
                     for (int k = 0; k < DP / 32; ++k) {
                         unsigned x[32];
@@ -739,10 +769,6 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
 #pragma unroll
                         for (int i = 0; i < 32; ++i) o[32 * k + i] = fmaf(o[32 * k + i], keep, __uint_as_float(x[i]));
                     }
-                } else {
-                    if (lane == 0) bar_arrive(&M.p_full[stream]);
-                    go = __all_sync(0xffffffffu, bar_wait(&M.o_full[stream], n_o & 1, abort_flag, a.status));
-                    ++n_o;
                 }
             }
             if (!go) break;
@@ -769,21 +795,22 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
                     tm_before();
                     __syncwarp();
                     if (lane == 0) bar_arrive(&M.merge_ready);
-                    go = __all_sync(0xffffffffu, bar_wait(&M.merge_read, walk.count & 1, abort_flag, a.status));
+                    go = __all_sync(0xffffffffu, bar_wait(&M.merge_read, q.count & 1, abort_flag, a.status));
                     tm_after();
                 } else {
-                    go = __all_sync(0xffffffffu, bar_wait(&M.merge_ready, walk.count & 1, abort_flag, a.status));
+                    go = __all_sync(0xffffffffu, bar_wait(&M.merge_ready, q.count & 1, abort_flag, a.status));
                     tm_after();
                     if (go && warp_live && tiles > 1) {
-                        unsigned x[32];
-                        tm_ld32(b_ml, x);
-                        const float m2 = __uint_as_float(x[0]), l2 = __uint_as_float(x[1]);
+                        unsigned ml[16];
+                        tm_ld16(b_ml, ml);
+                        const float m2 = __uint_as_float(ml[0]), l2 = __uint_as_float(ml[1]);
                         const float mn = fmaxf(m, m2);
                         const float ka = mn == -INFINITY ? 0.f : ex2(m - mn), kb = mn == -INFINITY ? 0.f : ex2(m2 - mn);
                         m = mn;
                         l = l * ka + l2 * kb;
 #pragma unroll
                         for (int k = 0; k < DP / 32; ++k) {
+                            unsigned x[32];
                             tm_ld32(b_o + 32 * k, x);
 #pragma unroll
                             for (int i = 0; i < 32; ++i)
@@ -794,78 +821,82 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
                     __syncwarp();
                     if (lane == 0) bar_arrive(&M.merge_read);
                 }
-            } else {  // both count every item
+            } else {  // both barriers count every piece
                 __syncwarp();
                 if (lane == 0) bar_arrive(stream ? &M.merge_ready : &M.merge_read);
             }
             if (!go) break;
-            if (live && (q.pair || stream == 0)) {
-                const bool whole = walk.t0 == 0 && walk.t1 == q.tiles;
-                float* dst;
+            if (warp_live && (q.pair || stream == 0)) {
+                // Rows through the Q tile, whose MMAs are done (the places of this
+                // warp's own vectors), so that each is written by a whole warp.
+                unsigned char* tile = tree_smem + (q.pair && stream ? F::kQTile : 0) + wq * 4096;
+                const auto stage = [&](int row, int ch) {
+                    return reinterpret_cast<float4*>(tile + (ch >> 3) * 16384 + row * 128 + (((ch & 7) ^ (row & 7)) << 4));
+                };
                 float f = 1.f;
-                if (whole) {
-                    dst = a.out + (long long)(q.c0 + node) * a.ldo + (long long)head * a.dim;
-                    f = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
-                } else {
-                    // the CTA's slot 1 holds an item that begins here, slot 0 one that began earlier
-                    float* slot = partial + (long long)(2 * cta + (walk.t0 == 0)) * kTreeRows * (DP + 2);
-                    const int pr = stream * 128 + r;
-                    dst = slot + pr * DP;
-                    slot[kTreeRows * DP + pr] = m;
-                    slot[kTreeRows * DP + kTreeRows + pr] = l;
-                }
+                if (q.whole) f = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-                for (int i = 0; i < DP; i += 4)
-                    if (!whole || i < a.dim)
-                        *reinterpret_cast<float4*>(dst + i) = make_float4(o[i] * f, o[i + 1] * f, o[i + 2] * f, o[i + 3] * f);
-                if (M.vbad[walk.count & 15]) {
+                for (int i = 0; i < DP / 4; ++i)
+                    *stage(lane, i) = make_float4(o[4 * i] * f, o[4 * i + 1] * f, o[4 * i + 2] * f, o[4 * i + 3] * f);
+                // the CTA's slot 1 holds an item that begins here, slot 0 one that began earlier
+                float* part = partial + (long long)(2 * cta + (q.t0 == 0)) * kTreeRows * (DP + 2);
+                const int pr = stream * 128 + r;
+                if (!q.whole && live) {
+                    part[kTreeRows * DP + pr] = m;
+                    part[kTreeRows * DP + kTreeRows + pr] = l;
+                }
+                __syncwarp();
+                const int most = min(32, tile_rows - wq * 32);
+                const bool fix = M.vbad[q.count & 15] != 0;
+#pragma unroll 4
+                for (int i = 0; i < most; ++i) {
+                    const int v = first_row + wq * 32 + i, nd = v / group, hd = q.head * group + v - nd * group;
+                    float* dst = q.whole ? a.out + (long long)(q.c0 + nd) * a.ldo + (long long)hd * a.dim
+                                         : part + (stream * 128 + wq * 32 + i) * DP;
+                    if (lane < (q.whole ? a.dim >> 2 : DP / 4))
+                        reinterpret_cast<float4*>(dst)[lane] = *stage(i, lane);
+                }
+                if (fix) {
                     // non-finite V of nodes was kept out of the products (0 * inf): give it to the rows that see it
+                    __syncwarp();
                     int unused = 0;
-                    for (int j = 0; j < q.n; ++j) {
-                        if (!(node_bits(a, q.c0, q.n, node, j) & 1)) continue;
-                        const long long base = tree_row(a, q.s, q.c0, q.len, q.len + j, unused);
-                        if (base < 0) continue;
-                        const long long v = base + (long long)walk.head * a.bt * a.dim + a.kind_stride;
-                        const float sc = KV == 2 ? a.scales[v / a.dim] : 1.f;
-                        for (int d = 0; d < a.dim; ++d) {
-                            const float x = KV == 2 ? sc : kv_value(a, v + d);
-                            if (!isfinite(x)) dst[d] += x;
+                    for (int i = 0; i < most; ++i) {
+                        const int v = first_row + wq * 32 + i, nd = v / group, hd = q.head * group + v - nd * group;
+                        float* dst = q.whole ? a.out + (long long)(q.c0 + nd) * a.ldo + (long long)hd * a.dim
+                                             : part + (stream * 128 + wq * 32 + i) * DP;
+                        for (int jn = 0; jn < q.n; ++jn) {
+                            if (!(node_bits(a, q.c0, q.n, nd, jn) & 1)) continue;
+                            const long long base = tree_row(a, q.s, q.c0, q.len, q.len + jn, unused);
+                            if (base < 0) continue;
+                            const long long at = base + (long long)q.head * a.bt * a.dim + a.kind_stride;
+                            for (int d = lane; d < a.dim; d += 32) {
+                                const float x = KV == 2 ? a.scales[at / a.dim] : kv_value(a, at + d);
+                                if (!isfinite(x)) dst[d] += x;
+                            }
                         }
                     }
                 }
             }
-            if (warp == 0 && lane == 0 && walk.t0 == 0 && walk.t1 < q.tiles) {
-                // the CTA in which the item's last tile starts
-                const long long excl = q.s == M.seq0 ? M.excl0 : q.s == M.seq1 ? M.excl1 : -1;
-                long long last;
-                if (excl >= 0) {
-                    last = excl + (walk.item * q.tiles + q.tiles - 1) * q.weight;
-                    const long long end = ((last + 1) * ctas + total - 1) / total - 1;
-                    TreeRec rec;
-                    rec.c0 = q.c0;
-                    rec.row0 = walk.row0;
-                    rec.rows = walk.rows;
-                    rec.split = walk.split;
-                    rec.head = walk.head;
-                    rec.pieces = int(end) - cta + 1;
-                    recs[cta] = rec;
-                }
-            }
+            proxy_fence();  // the Q tile's next readers and writers
+            __syncwarp();
+            if (lane == 0) release_piece(piece);
         }
     } else if (warp < kTreeMmaWarp) {
         // ------------------------------------------------------------ loads
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         const int lw = warp - kTreeLoadWarp;
         constexpr int kRowsPerWarp = F::kBn / 4;
         unsigned empty_phase = 0xffffffffu;
         int slot = 0, flags = 0;
         const int row_bytes = a.dim * F::kElem, chunks = row_bytes >> 4;
         const unsigned char* pool = static_cast<const unsigned char*>(a.kv);
-        // Address of this lane's row of a tile (byte offset of its K row, -1: none)
-        const auto row_of = [&](const TreeWalk<F>& w, int j) -> long long {
-            const long long p = (w.t0 + j) * F::kBn + lw * kRowsPerWarp + (lane % kRowsPerWarp);
-            if (p >= (long long)w.q.len + w.q.n) return -1;
-            const long long at = tree_row(a, w.q.s, w.q.c0, w.q.len, int(p), flags);
+        // This lane's row of a tile: the element offset of its K row (-1: none).
+        // V of a tile uses the row that K left behind: by the order of the
+        // entries it is the last or the last but one.
+        const auto row_of = [&](const TreePiece& w, int j) -> long long {
+            const int p = (w.t0 + j) * F::kBn + lw * kRowsPerWarp + (lane % kRowsPerWarp);
+            if (p >= w.len + w.n) return -1;
+            const long long at = tree_row(a, w.s, w.c0, w.len, p, flags);
             return at < 0 ? -1 : at + (long long)w.head * a.bt * a.dim;
         };
         if constexpr (KV == 1) {
@@ -881,21 +912,30 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
                 for (int i = 0; i < n_pend; ++i) signal(pend[i]);
                 n_pend = 0;
             };
-            while (go && walk.next(a)) {
-                const bool pair = walk.q.pair;
+            for (unsigned piece = 0; go; ++piece) {
+                if (!__all_sync(0xffffffffu, get_piece(piece))) break;
+                const TreePiece& walk = M.piece[piece % kPieceRing];
+                const bool pair = walk.pair;
                 const int ns = pair ? F::kBase : F::kBase + F::kExtra;
                 if (slot >= ns) slot = 0;
-                bool wait_q = prev_pair && !pair;  // extra slots lie in the second Q tile: its MMAs first
+                bool wait_q = prev_pair && !pair;  // extra slots lie in the second Q tile: its last use first
                 if (lane == 0 && lw == 0) M.vbad[(walk.count + 8) & 15] = 0;  // no warp is that far ahead or behind
-                const int loads = 2 * int(walk.t1 - walk.t0);
+                const int loads = 2 * (walk.t1 - walk.t0);
+                long long row_cur = -1, row_prev = -1;
+                int k_last = -1;
                 for (int e = 0; e < loads && go; ++e) {
                     bool is_v;
                     const int j = walk.entry(e, is_v);
-                    const long long k_row = row_of(walk, j);
+                    if (!is_v) {
+                        row_prev = row_cur;
+                        row_cur = row_of(walk, j);
+                        k_last = j;
+                    }
+                    const long long k_row = j == k_last ? row_cur : row_prev;
                     const unsigned have = __ballot_sync(0xffffffffu, k_row >= 0);
                     if (slot >= F::kBase && wait_q) {
                         drain();
-                        go = __all_sync(0xffffffffu, bar_wait(&M.item_done, (walk.count - 1) & 1, abort_flag, a.status));
+                        go = __all_sync(0xffffffffu, bar_wait(&M.q_full, piece & 1, abort_flag, a.status));
                         wait_q = false;
                         if (!go) break;
                     }
@@ -921,13 +961,13 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
                              ok ? pool + (at + shift) * 2 + ch * 16 : pool, ok ? 16u : 0u);
                     }
                     cp_commit();
-                    if (is_v && (walk.t0 + j + 1) * F::kBn > walk.q.len) {
+                    if (is_v && (walk.t0 + j + 1) * F::kBn > walk.len) {
                         // a tile with nodes: non-finite V must not meet a weight of zero in the products
                         drain();
                         cp_wait<0>();
                         __syncwarp();
                         const int rt = lw * 32 + lane;
-                        const bool is_node = (walk.t0 + j) * F::kBn + rt >= walk.q.len && k_row >= 0;
+                        const bool is_node = (walk.t0 + j) * F::kBn + rt >= walk.len && k_row >= 0;
                         bool bad = false;
                         if (is_node) {
                             for (int k = 0; k < kLanes; ++k) {
@@ -957,6 +997,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
                     slot = slot + 1 == ns ? 0 : slot + 1;
                 }
                 prev_pair = pair;
+                if (lane == 0) release_piece(piece);
             }
             drain();
         } else {
@@ -964,8 +1005,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
             // place of the thread that converts them, so a thread waits only
             // for its own copies.
             bool go = true;
-            TreeWalk<F> ahead = walk;
-            int e_issue = 0, loads_issue = 0;
+            unsigned piece_issue = 0xffffffffu;  // the piece that is being fetched
+            int e_issue = 0, loads_issue = 0, k_last = -1;
+            long long row_cur = -1, row_prev = -1;
             bool more = true;
             int raw_in = 0, raw_out = 0;
             constexpr int kLanes = DP * F::kElem / 16, kStep = 32 / kLanes;  // lanes per row, rows per instruction
@@ -973,14 +1015,21 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
             const int ch = lane % kLanes;
             const auto issue = [&]() {
                 if (e_issue == loads_issue) {
-                    more = ahead.next(a);
+                    more = __all_sync(0xffffffffu, get_piece(++piece_issue));
                     if (!more) return;
                     e_issue = 0;
-                    loads_issue = 2 * int(ahead.t1 - ahead.t0);
+                    loads_issue = 2 * (M.piece[piece_issue % kPieceRing].t1 - M.piece[piece_issue % kPieceRing].t0);
+                    k_last = -1;
                 }
+                const TreePiece& ahead = M.piece[piece_issue % kPieceRing];
                 bool is_v;
                 const int j = ahead.entry(e_issue++, is_v);
-                const long long mine_row = row_of(ahead, j);
+                if (!is_v) {
+                    row_prev = row_cur;
+                    row_cur = row_of(ahead, j);
+                    k_last = j;
+                }
+                const long long mine_row = j == k_last ? row_cur : row_prev;
                 const unsigned have = __ballot_sync(0xffffffffu, mine_row >= 0);
                 if (!is_v && lane == 0) {
                     unsigned* valid = M.valid[(ahead.tile_base + j) % kMetaRing];
@@ -1010,9 +1059,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
                 if (more) issue();
                 if (!more) cp_commit();  // keeps the count of groups
             }
-            while (go && walk.next(a)) {
+            for (unsigned piece = 0; go; ++piece) {
+                if (!__all_sync(0xffffffffu, get_piece(piece))) break;
+                const TreePiece& walk = M.piece[piece % kPieceRing];
                 if (lane == 0 && lw == 0) M.vbad[(walk.count + 8) & 15] = 0;  // no warp is that far ahead or behind
-                const int loads = 2 * int(walk.t1 - walk.t0);
+                const int loads = 2 * (walk.t1 - walk.t0);
                 for (int e = 0; e < loads && go; ++e) {
                     bool is_v;
                     const int j = walk.entry(e, is_v);
@@ -1024,8 +1075,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
                     if (!go) break;
                     empty_phase ^= 1u << slot;
                     const int meta = int((walk.tile_base + j) % kMetaRing);
-                    const long long p0 = (walk.t0 + j) * F::kBn, lane_p = p0 + lw * kRowsPerWarp + (lane % kRowsPerWarp);
-                    const bool node_row = lane_p >= walk.q.len;
+                    const int p0 = (walk.t0 + j) * F::kBn;
+                    const bool node_row = p0 + lw * kRowsPerWarp + (lane % kRowsPerWarp) >= walk.len;
                     float* scale_col = reinterpret_cast<float*>(tree_smem + F::kOffScale) +
                                        (int((walk.tile_base + j) % F::kScaleRing) * 2 + is_v) * F::kBn;
                     unsigned char* out = tree_smem + slot_at(slot);
@@ -1075,7 +1126,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
                             uint4 raw_v = raw[i * 32 + lane];
                             float v[4] = {__uint_as_float(raw_v.x), __uint_as_float(raw_v.y), __uint_as_float(raw_v.z),
                                           __uint_as_float(raw_v.w)};
-                            if (is_v && p0 + rt >= walk.q.len) {
+                            if (is_v && p0 + rt >= walk.len) {
 #pragma unroll
                                 for (int x = 0; x < 4; ++x)
                                     if (!isfinite(v[x])) v[x] = 0.f, bad = true;
@@ -1110,17 +1161,17 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
                     }
                     slot = slot + 1 == F::kBase ? 0 : slot + 1;
                 }
+                if (lane == 0) release_piece(piece);
             }
             cp_wait<0>();
         }
         if (flags) atomicOr(a.status, flags);
-    } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-        if (warp == kTreeMmaWarp && lane == 0) {
+    } else if (warp == kTreeMmaWarp) {
+        if (lane == 0) {
             // -------------------------------------------------- MMA issue
             constexpr unsigned kIdescS = (1u << 4) | (unsigned(F::kBn >> 3) << 17) | (8u << 24);
             constexpr unsigned kIdescO = (1u << 4) | (1u << 16) | (unsigned(DP >> 3) << 17) | (8u << 24);
-            unsigned full_phase = 0, n_p[2] = {0, 0}, pieces = 0;
+            unsigned full_phase = 0, n_p[2] = {0, 0};
             int slot = 0;
             bool go = true;
             const auto qk = [&](int q_tile, int stream, unsigned at) {
@@ -1144,10 +1195,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
                 int acc = 0;
 #pragma unroll 1
                 for (int part = 0; part < F::kParts + 1; ++part) {
-                    const unsigned pa = part == 0 ? p + F::kBn / 2 : p, vb = F::kParts == 2 && part == 1 ? v + F::kSlotPart : v;
+                    const unsigned pa = part == 0 ? p + 8 : p, vb = F::kParts == 2 && part == 1 ? v + F::kSlotPart : v;
 #pragma unroll
                     for (int kk = 0; kk < F::kBn / 16; ++kk) {
-                        mma_ts(d, pa + kk * 8, sw128_desc(vb + kk * 2048, F::kBn * 128), kIdescO, acc);
+                        mma_ts(d, pa + kk * 16, sw128_desc(vb + kk * 2048, F::kBn * 128), kIdescO, acc);
                         acc = 1;
                     }
                 }
@@ -1160,12 +1211,13 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
                 tm_after();
                 return s;
             };
-            while (go && walk.next(a)) {
-                const bool pair = walk.q.pair;
-                const int ns = pair ? F::kBase : F::kBase + F::kExtra, tiles = int(walk.t1 - walk.t0);
+            for (unsigned piece = 0; go; ++piece) {
+                if (!get_piece(piece)) break;
+                const TreePiece& walk = M.piece[piece % kPieceRing];
+                const bool pair = walk.pair;
+                const int ns = pair ? F::kBase : F::kBase + F::kExtra, tiles = walk.t1 - walk.t0;
                 if (slot >= ns) slot = 0;
-                go = bar_wait(&M.q_full, pieces & 1, abort_flag, a.status);
-                ++pieces;
+                go = bar_wait(&M.q_full, piece & 1, abort_flag, a.status);
                 if (!go) break;
                 tm_after();
                 if (!pair) {
@@ -1226,7 +1278,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
                     }
                 }
                 if (!go) break;
-                tree_commit_to(&M.item_done);
+                release_piece(piece);
             }
             // nothing of this CTA's may be in flight when its memory is given back
             tree_commit_to(&M.drain);
