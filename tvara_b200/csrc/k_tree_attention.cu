@@ -30,15 +30,22 @@ __device__ __forceinline__ bool tree_sequence_ok(const TreeAttn& a, int s, int& 
 // Element offset of the K row (head 0 of the layer) of index p of a sequence
 // (cached positions, then nodes), or -1 with the status bit for a block or
 // slot outside the pool.
+// x / bt for x < 2^44 by the reciprocal 2^64 / bt rounded up (0 stands for
+// bt 1): it is too large by less than bt / 2^64 <= 2^-44, so the product is
+// off by less than one step of the quotient's fraction.
+__device__ __forceinline__ long long div_bt(const TreeAttn& a, long long x) {
+    return a.bt_inverse ? (long long)__umul64hi((unsigned long long)x, a.bt_inverse) : x;
+}
 __device__ __forceinline__ long long tree_row(const TreeAttn& a, int s, int c0, int len, int p, int& flags) {
     long long block, off;
     if (p < len) {
-        const int e = p / a.bt;
+        const int e = int(div_bt(a, p));
         block = a.tables[(long long)s * a.stride + e];
         off = p - e * a.bt;
     } else {
         const long long slot = a.slots[c0 + p - len];
-        block = slot < 0 ? -1 : slot / a.bt;
+        const bool in = slot >= 0 && slot < (long long)a.max_blocks * a.bt;
+        block = in ? div_bt(a, slot) : -1;
         off = slot - block * a.bt;
     }
     if (block < 0 || block >= a.max_blocks) {
@@ -82,7 +89,7 @@ __global__ void __launch_bounds__(kAnyWarps * 32) tree_any_kernel(TreeAttn a) {
         if (threadIdx.x == 0 && h == 0) atomicOr(a.status, kTreeBadLengths);
         return;
     }
-    const int node = t - c0, g = h / (a.hq / a.hkv);
+    const int node = t - c0, g = h / a.group;
     const unsigned long long* mask = a.ancestors ? a.ancestors + (long long)t * a.words : nullptr;
     const float* q = a.q + (long long)t * a.ldq + (long long)h * a.dim;
     float qv[E], acc[E];
@@ -239,7 +246,7 @@ struct TreePiece {
 struct TreeMeta {  // at kOffMeta
     std::uint64_t full[8], empty[8];
     std::uint64_t s_full[2], p_full[2], o_full[2];
-    std::uint64_t v_ready[kMetaRing];  // a tile's V scales are in place (F32, int8)
+    std::uint64_t v_ready[kMetaRing];  // a tile's V scales and vbad are in place
     std::uint64_t q_full, merge_ready, merge_read, drain;
     std::uint64_t piece_full[kPieceRing], piece_empty[kPieceRing];
     union {
@@ -248,7 +255,7 @@ struct TreeMeta {  // at kOffMeta
     };
     alignas(16) unsigned valid[kMetaRing][4];   // columns of a tile that hold a row
     alignas(16) float vmax[kMetaRing][4];       // largest V scale per load warp
-    int vbad[16];                   // an item's nodes hold a non-finite V
+    unsigned vbad[kMetaRing][4];    // nodes whose V (kept out of the products: 0 * inf) is not finite
     long long total, excl0, excl1;
     int seq0, seq1;
     unsigned tmem;
@@ -279,6 +286,7 @@ __device__ __forceinline__ bool bar_test(std::uint64_t* b, unsigned parity) {
 }
 // Bounded; false after the limit or when another role gave up.
 __device__ __forceinline__ bool bar_wait(std::uint64_t* b, unsigned parity, volatile int* abort_flag, int* status) {
+#pragma unroll 1
     for (unsigned i = 0; i < kTreeSpin; ++i) {
         if (bar_test(b, parity)) return true;
         if (*abort_flag) return false;
@@ -286,6 +294,11 @@ __device__ __forceinline__ bool bar_wait(std::uint64_t* b, unsigned parity, vola
     *abort_flag = 1;
     atomicOr(status, kTreeTimeout);
     return false;
+}
+__device__ __forceinline__ bool elect_one() {
+    unsigned p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+    return p != 0;
 }
 __device__ __forceinline__ void tree_commit_to(std::uint64_t* b) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(sm_addr(b))
@@ -385,12 +398,12 @@ __device__ __forceinline__ bool tree_seq(const TreeAttn& a, int s, TreeSeq& q) {
         q.total = 0;
         return q.n == 0;
     }
-    const int vectors = q.n * (a.hq / a.hkv);
+    const int vectors = q.n * a.group;
     const int most = F::kPairs ? 256 : 128;
-    q.groups = (vectors + most - 1) / most;
+    q.groups = unsigned(vectors + most - 1) / most;
     q.pair = F::kPairs && vectors > 128;
     q.weight = q.pair ? 2 : 1;
-    q.tiles = ((long long)q.len + q.n + F::kBn - 1) / F::kBn;
+    q.tiles = (unsigned(q.len) + unsigned(q.n) + F::kBn - 1) / F::kBn;
     q.total = q.tiles * q.groups * a.hkv;
     return true;
 }
@@ -425,19 +438,23 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
     extern __shared__ __align__(1024) unsigned char tree_smem[];
     TreeMeta& M = *reinterpret_cast<TreeMeta*>(tree_smem + F::kOffMeta);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int group = a.hq / a.hkv;
+    const int group = a.group;
 
     if (tid == 0) {
+#pragma unroll 1
         for (int i = 0; i < 8; ++i) {
             bar_init(&M.full[i], 4);
             bar_init(&M.empty[i], 1);
         }
+#pragma unroll 1
         for (int i = 0; i < kMetaRing; ++i) bar_init(&M.v_ready[i], 4);
+#pragma unroll 1
         for (int i = 0; i < 2; ++i) {
             bar_init(&M.s_full[i], 1);
             bar_init(&M.p_full[i], 4);
             bar_init(&M.o_full[i], 1);
         }
+#pragma unroll 1
         for (int i = 0; i < kPieceRing; ++i) {
             bar_init(&M.piece_full[i], 1);
             bar_init(&M.piece_empty[i], 13);  // 8 softmax warps, 4 load warps, the MMA thread
@@ -448,7 +465,6 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
         bar_init(&M.drain, 1);
         M.abort_flag = 0;
         M.bad = 0;
-        for (int i = 0; i < 16; ++i) M.vbad[i] = 0;
         M.total = 0;
         M.seq0 = M.seq1 = a.n_seq;
         M.excl0 = M.excl1 = 0;
@@ -463,6 +479,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
         return q.total ? q.total * q.weight : 0;
     };
     long long mine = 0;
+#pragma unroll 1
     for (int s = tid; s < a.n_seq; s += kTreeThreads) mine += weight_of(s);
     if (mine) atomicAdd(reinterpret_cast<unsigned long long*>(&M.total), (unsigned long long)mine);
     __syncthreads();
@@ -474,9 +491,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
     if (cta >= ctas || total == 0) return;
     const long long w0 = total * cta / ctas, w1 = total * (cta + 1) / ctas;
     long long carry = 0;
+#pragma unroll 1
     for (int base = 0; base < a.n_seq; base += kTreeThreads) {
         const long long w = weight_of(base + tid);
         long long scan = w;
+#pragma unroll 1
         for (int d = 1; d < 32; d <<= 1) {
             const long long up = __shfl_up_sync(0xffffffffu, scan, d);
             if (lane >= d) scan += up;
@@ -484,6 +503,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
         if (lane == 31) M.warp_sum[warp] = scan;
         __syncthreads();
         long long before = carry, all = 0;
+#pragma unroll 1
         for (int i = 0; i < kTreeThreads / 32; ++i) {
             if (i < warp) before += M.warp_sum[i];
             all += M.warp_sum[i];
@@ -522,8 +542,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
             long long u = (w0 - M.excl0 + q.weight - 1) / q.weight;
             unsigned count = 0, tile_base = 0;
             bool go = true;
+#pragma unroll 1
             for (int seq = M.seq0; go; ++count) {
                 long long end = seq == seq1 ? u1 : q.total;
+#pragma unroll 1
                 while (u >= end && seq < seq1) {
                     u = 0;
                     tree_seq<F>(a, ++seq, q);
@@ -604,40 +626,76 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
             const TreePiece& q = M.piece[piece % kPieceRing];
             const int tile_rows = q.pair ? (stream ? q.rows - q.split : q.split) : q.rows;
             const int first_row = q.row0 + (q.pair && stream ? q.split : 0);  // this stream's rows within the sequence
-            const int node = (first_row + r) / group;
+            const int node = unsigned(first_row + r) / unsigned(group);
+            const int first_node = unsigned(first_row + wq * 32) / unsigned(group);  // of the warp's vectors
+            const int first_g = first_row + wq * 32 - first_node * group;
             const bool live = r < tile_rows, warp_live = wq * 32 < tile_rows;
             // The warp's query vectors, one at a time across its lanes: scaled
             // below 2^15, split, into this stream's Q tile; lane i keeps the
             // score factor of vector i.
             float c = 0.f;
             if (warp_live) {
+                // raw rows first, all in flight, each in the 512 (256) bytes its two halves will take
                 const int quads = a.dim >> 2, most = min(32, tile_rows - wq * 32);
-                unsigned char* tile = tree_smem + (q.pair && stream ? F::kQTile : 0);
-#pragma unroll 4
-                for (int i = 0; i < most; ++i) {
-                    const int v = first_row + wq * 32 + i, nd = v / group, hd = q.head * group + v - nd * group;
-                    const float4* src =
-                        reinterpret_cast<const float4*>(a.q + (long long)(q.c0 + nd) * a.ldq + (long long)hd * a.dim);
-                    const float4 x = lane < quads ? __ldg(src + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    float top = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
-                    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-                    const int up = lift(top);
-                    if (lane == i) c = score_unit * two_to(-up);
-                    if ((stream == 0 || q.pair) && lane < DP / 4) {
+                const bool writes = stream == 0 || q.pair;
+                unsigned char* tile = tree_smem + (q.pair && stream ? F::kQTile : 0) + wq * 4096;
+                int g = first_g;
+                const float* src = a.q + (long long)(q.c0 + first_node) * a.ldq + (long long)(q.head * group + g) * a.dim + lane * 4;
+                const long long turn = a.ldq - (long long)(group - 1) * a.dim;  // to the next node's first head
+                if (writes) {
+                    const unsigned to = sm_addr(tile) + (lane >> 3) * 16384 + ((lane & 7) << 4);
+#pragma unroll 1
+                    for (int i = 0; i < most; ++i) {
+                        if (lane < DP / 4) cp16(to + i * 128, lane < quads ? src : a.q, lane < quads ? 16u : 0u);
+                        const bool last = g + 1 == group;
+                        src += last ? turn : a.dim;
+                        g = last ? 0 : g + 1;
+                    }
+                    cp_commit();
+                    cp_wait<0>();
+                    __syncwarp();
+#pragma unroll 1
+                    for (int i = 0; i < most; ++i) {
+                        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (lane < DP / 4) x = *reinterpret_cast<const float4*>(tile + (lane >> 3) * 16384 + i * 128 + ((lane & 7) << 4));
+                        float top = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+                        top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+                        const int up = lift(top);
+                        if (lane == i) c = score_unit * two_to(-up);
                         const float f = two_to(up);
                         uint2 hi, lo;
                         split_exact(x.x * f, x.y * f, hi.x, lo.x);
                         split_exact(x.z * f, x.w * f, hi.y, lo.y);
-                        const int row = wq * 32 + i, ch = lane >> 1;
-                        const int at = (ch >> 3) * 16384 + row * 128 + (((ch & 7) ^ (row & 7)) << 4) + (lane & 1) * 8;
-                        *reinterpret_cast<uint2*>(tile + at) = hi;
-                        *reinterpret_cast<uint2*>(tile + F::kQPart + at) = lo;
+                        __syncwarp();  // the row is read
+                        const int ch = lane >> 1, at = (ch >> 3) * 16384 + i * 128 + (((ch & 7) ^ (i & 7)) << 4) + (lane & 1) * 8;
+                        if (lane < DP / 4) {
+                            *reinterpret_cast<uint2*>(tile + at) = hi;
+                            *reinterpret_cast<uint2*>(tile + F::kQPart + at) = lo;
+                        }
+                    }
+                    if (!q.pair) {  // for the other stream, in its idle tensor memory
+                        asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(lane_base + 384),
+                                     "r"(__float_as_uint(c))
+                                     : "memory");
+                        tm_wait_st();
+                        tm_before();
                     }
                 }
             }
             proxy_fence();
             __syncwarp();
             if (lane == 0) bar_arrive(&M.q_full);
+            if (!q.pair && stream) {
+                go = __all_sync(0xffffffffu, bar_wait(&M.q_full, piece & 1, abort_flag, a.status));
+                if (!go) break;
+                if (warp_live) {
+                    unsigned x;
+                    tm_after();
+                    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(x) : "r"(lane_base + 384));
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    c = __uint_as_float(x);
+                }
+            }
             float m = -INFINITY, l = 0.f, vref = 0.f;
 #pragma unroll
             for (int i = 0; i < DP; ++i) o[i] = 0.f;
@@ -645,7 +703,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
             for (int j = q.pair ? 0 : stream; j < tiles && go; j += q.pair ? 1 : 2, ++n_s) {
                 const unsigned t = q.tile_base + j;
                 go = bar_wait(&M.s_full[stream], n_s & 1, abort_flag, a.status);
-                if constexpr (KV != 1)
+                if (KV != 1 || (q.t0 + j + 1) * F::kBn > q.len)  // scales of V, nodes with a non-finite V
                     go = go && bar_wait(&M.v_ready[t % kMetaRing], (t / kMetaRing) & 1, abort_flag, a.status);
                 go = __all_sync(0xffffffffu, go);
                 if (!go) break;
@@ -655,17 +713,21 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
                     const int ring = t % kMetaRing;
                     const long long p0 = (long long)(q.t0 + j) * F::kBn;
                     const bool nodes = p0 + F::kBn > q.len;
-                    unsigned seen[F::kBn / 32];
+                    bool all = !nodes;
 #pragma unroll
-                    for (int k = 0; k < F::kBn / 32; ++k) {
-                        seen[k] = M.valid[ring][k];
-                        if (nodes) seen[k] &= node_bits(a, q.c0, q.n, live ? node : 0, p0 + 32 * k - q.len);
-                    }
+                    for (int k = 0; k < F::kBn / 32; ++k) all &= M.valid[ring][k] == 0xffffffffu;
+                    unsigned seen[F::kBn / 32] = {};  // columns 32 k .. that this vector sees, when not all
+                    const auto see_of = [&](int k) -> unsigned {
+                        unsigned w = seen[0];
+#pragma unroll
+                        for (int i = 1; i < F::kBn / 32; ++i) w = k == i ? seen[i] : w;
+                        return w;
+                    };
                     const float* k_scale = reinterpret_cast<const float*>(tree_smem + F::kOffScale) +
                                            t % (F::kScaleRing ? F::kScaleRing : 1) * 2 * F::kBn;
                     const float* v_scale = k_scale + F::kBn;
-                    float top = -INFINITY;
-#pragma unroll
+                    float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
                     for (int k = 0; k < F::kBn / 32; ++k) {
                         unsigned x[32];
                         tm_ld32(s_at + 32 * k, x);
@@ -679,14 +741,22 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
                                 x[i + 3] = __float_as_uint(__uint_as_float(x[i + 3]) * f.w);
                             }
                         }
-                        if (seen[k] != 0xffffffffu) {
+                        if (!all) {
+                            unsigned see = M.valid[ring][k];
+                            if (nodes) {
+                                see &= node_bits(a, q.c0, q.n, live ? node : 0, p0 + 32 * k - q.len);
+                                if (see & M.vbad[ring][k]) l = NAN;  // the row's result is not finite
+                            }
+#pragma unroll
+                            for (int i = 0; i < F::kBn / 32; ++i) seen[i] = k == i ? see : seen[i];
 #pragma unroll
                             for (int i = 0; i < 32; ++i)
-                                if (!(seen[k] >> i & 1)) x[i] = 0xff800000u;
+                                if (!(see >> i & 1)) x[i] = 0xff800000u;
                         }
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(x[i]));
+                        for (int i = 0; i < 32; ++i) tops[i & 3] = fmaxf(tops[i & 3], __uint_as_float(x[i]));
                     }
+                    const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
                     const float mn = fmaxf(m, top * c);
                     const float off = mn == -INFINITY ? 11.f : 11.f - mn;
                     keep = mn == -INFINITY ? 1.f : ex2(m - mn);
@@ -705,52 +775,52 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
                     // P over S, sixteen positions (one K step of the MMA) at a
                     // time: hi in their first eight columns, lo in the others.
                     float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-                    for (int w = 0; w < F::kBn / 32; ++w) {
-                        const unsigned see = seen[w];
 #pragma unroll 1
-                        for (int k = 2 * w; k < 2 * w + 2; ++k) {
-                            unsigned x[16], y[16];
-                            tm_ld16(s_at + 16 * k, x);
+                    for (int k = 0; k < F::kBn / 16; ++k) {
+                        unsigned x[16], y[16];
+                        tm_ld16(s_at + 16 * k, x);
+                        if constexpr (KV != 1) {
 #pragma unroll
                             for (int i = 0; i < 16; i += 4) {
-                                float p[4];
-                                float4 ks, vs;
-                                if constexpr (KV != 1) {
-                                    ks = *reinterpret_cast<const float4*>(k_scale + 16 * k + i);
-                                    vs = *reinterpret_cast<const float4*>(v_scale + 16 * k + i);
-                                }
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    float sc = __uint_as_float(x[i + e]);
-                                    if constexpr (KV != 1) sc *= e == 0 ? ks.x : e == 1 ? ks.y : e == 2 ? ks.z : ks.w;
-                                    p[e] = ex2(fmaf(sc, c, off));
-                                }
-                                if (see != 0xffffffffu) {
-                                    const unsigned bits = see >> ((k & 1) * 16 + i);
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e)
-                                        if (!(bits >> e & 1)) p[e] = 0.f;
-                                }
-                                sum0 += p[0] + p[2];
-                                sum1 += p[1] + p[3];
-                                if constexpr (KV != 1) {
-                                    p[0] *= vs.x * v_unit;
-                                    p[1] *= vs.y * v_unit;
-                                    p[2] *= vs.z * v_unit;
-                                    p[3] *= vs.w * v_unit;
-                                    if (see != 0xffffffffu) {  // a masked row's scale may be anything
-                                        const unsigned bits = see >> ((k & 1) * 16 + i);
-#pragma unroll
-                                        for (int e = 0; e < 4; ++e)
-                                            if (!(bits >> e & 1)) p[e] = 0.f;
-                                    }
-                                }
-                                split_weight(p[0], p[1], y[i / 2], y[8 + i / 2]);
-                                split_weight(p[2], p[3], y[i / 2 + 1], y[8 + i / 2 + 1]);
+                                const float4 f = *reinterpret_cast<const float4*>(k_scale + 16 * k + i);
+                                x[i] = __float_as_uint(__uint_as_float(x[i]) * f.x);
+                                x[i + 1] = __float_as_uint(__uint_as_float(x[i + 1]) * f.y);
+                                x[i + 2] = __float_as_uint(__uint_as_float(x[i + 2]) * f.z);
+                                x[i + 3] = __float_as_uint(__uint_as_float(x[i + 3]) * f.w);
                             }
-                            tm_st16(s_at + 16 * k, y);
                         }
+                        float p[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) p[i] = ex2(fmaf(__uint_as_float(x[i]), c, off));
+                        const unsigned see = all ? 0xffffffffu : see_of(k >> 1) >> ((k & 1) * 16);
+                        if (!all) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+                                if (!(see >> i & 1)) p[i] = 0.f;
+                        }
+#pragma unroll
+                        for (int i = 0; i < 16; i += 2) {
+                            sum0 += p[i];
+                            sum1 += p[i + 1];
+                        }
+                        if constexpr (KV != 1) {
+#pragma unroll
+                            for (int i = 0; i < 16; i += 4) {
+                                const float4 f = *reinterpret_cast<const float4*>(v_scale + 16 * k + i);
+                                p[i] *= f.x * v_unit;
+                                p[i + 1] *= f.y * v_unit;
+                                p[i + 2] *= f.z * v_unit;
+                                p[i + 3] *= f.w * v_unit;
+                            }
+                            if (!all) {  // a masked row's scale may be anything
+#pragma unroll
+                                for (int i = 0; i < 16; ++i)
+                                    if (!(see >> i & 1)) p[i] = 0.f;
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) split_weight(p[2 * i], p[2 * i + 1], y[i], y[8 + i]);
+                        tm_st16(s_at + 16 * k, y);
                     }
                     l += sum0 + sum1;
                     tm_wait_st();
@@ -836,7 +906,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
                 float f = 1.f;
                 if (q.whole) f = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-                for (int i = 0; i < DP / 4; ++i)
+                for (int i = 0; i < DP / 4; ++i)  // lane is the row
                     *stage(lane, i) = make_float4(o[4 * i] * f, o[4 * i + 1] * f, o[4 * i + 2] * f, o[4 * i + 3] * f);
                 // the CTA's slot 1 holds an item that begins here, slot 0 one that began earlier
                 float* part = partial + (long long)(2 * cta + (q.t0 == 0)) * kTreeRows * (DP + 2);
@@ -847,33 +917,19 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
                 }
                 __syncwarp();
                 const int most = min(32, tile_rows - wq * 32);
-                const bool fix = M.vbad[q.count & 15] != 0;
-#pragma unroll 4
-                for (int i = 0; i < most; ++i) {
-                    const int v = first_row + wq * 32 + i, nd = v / group, hd = q.head * group + v - nd * group;
-                    float* dst = q.whole ? a.out + (long long)(q.c0 + nd) * a.ldo + (long long)hd * a.dim
-                                         : part + (stream * 128 + wq * 32 + i) * DP;
-                    if (lane < (q.whole ? a.dim >> 2 : DP / 4))
-                        reinterpret_cast<float4*>(dst)[lane] = *stage(i, lane);
-                }
-                if (fix) {
-                    // non-finite V of nodes was kept out of the products (0 * inf): give it to the rows that see it
-                    __syncwarp();
-                    int unused = 0;
+                {
+                    const int width = q.whole ? a.dim >> 2 : DP / 4;
+                    int g = q.whole ? first_g : 0;
+                    float* dst = q.whole ? a.out + (long long)(q.c0 + first_node) * a.ldo + (long long)(q.head * group + g) * a.dim
+                                         : part + (stream * 128 + wq * 32) * DP;
+                    const int heads = q.whole ? group : 1;
+                    const long long step = q.whole ? a.dim : DP, turn = q.whole ? a.ldo - (long long)(group - 1) * a.dim : DP;
+#pragma unroll 2
                     for (int i = 0; i < most; ++i) {
-                        const int v = first_row + wq * 32 + i, nd = v / group, hd = q.head * group + v - nd * group;
-                        float* dst = q.whole ? a.out + (long long)(q.c0 + nd) * a.ldo + (long long)hd * a.dim
-                                             : part + (stream * 128 + wq * 32 + i) * DP;
-                        for (int jn = 0; jn < q.n; ++jn) {
-                            if (!(node_bits(a, q.c0, q.n, nd, jn) & 1)) continue;
-                            const long long base = tree_row(a, q.s, q.c0, q.len, q.len + jn, unused);
-                            if (base < 0) continue;
-                            const long long at = base + (long long)q.head * a.bt * a.dim + a.kind_stride;
-                            for (int d = lane; d < a.dim; d += 32) {
-                                const float x = KV == 2 ? a.scales[at / a.dim] : kv_value(a, at + d);
-                                if (!isfinite(x)) dst[d] += x;
-                            }
-                        }
+                        if (lane < width) reinterpret_cast<float4*>(dst)[lane] = *stage(i, lane);
+                        const bool last = g + 1 == heads;
+                        dst += last ? turn : step;
+                        g = last ? 0 : g + 1;
                     }
                 }
             }
@@ -919,7 +975,6 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
                 const int ns = pair ? F::kBase : F::kBase + F::kExtra;
                 if (slot >= ns) slot = 0;
                 bool wait_q = prev_pair && !pair;  // extra slots lie in the second Q tile: its last use first
-                if (lane == 0 && lw == 0) M.vbad[(walk.count + 8) & 15] = 0;  // no warp is that far ahead or behind
                 const int loads = 2 * (walk.t1 - walk.t0);
                 long long row_cur = -1, row_prev = -1;
                 int k_last = -1;
@@ -951,7 +1006,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
                     const long long shift = is_v ? a.kind_stride : 0;
                     constexpr int kLanes = DP / 8, kStep = 32 / kLanes;  // lanes per row, rows per instruction
                     const int ch = lane % kLanes;
-#pragma unroll 8
+#pragma unroll 4
                     for (int i = 0; i < 32 / kStep; ++i) {
                         const int rr = i * kStep + lane / kLanes;
                         const long long at = __shfl_sync(0xffffffffu, k_row, rr);
@@ -964,28 +1019,27 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
                     if (is_v && (walk.t0 + j + 1) * F::kBn > walk.len) {
                         // a tile with nodes: non-finite V must not meet a weight of zero in the products
                         drain();
-                        cp_wait<0>();
                         __syncwarp();
+                        unsigned bad_rows = 0;
                         const int rt = lw * 32 + lane;
-                        const bool is_node = (walk.t0 + j) * F::kBn + rt >= walk.len && k_row >= 0;
                         bool bad = false;
-                        if (is_node) {
-                            for (int k = 0; k < kLanes; ++k) {
-                                uint4* at = reinterpret_cast<uint4*>(tree_smem + slot_at(slot) + (k >> 3) * (F::kBn * 128) +
-                                                                     rt * 128 + (((k & 7) ^ (rt & 7)) << 4));
-                                uint4 v = *at;
-                                unsigned* w = reinterpret_cast<unsigned*>(&v);
-                                bool hit = false;
-                                for (int x = 0; x < 4; ++x) {
-                                    if ((w[x] & 0x7c00u) == 0x7c00u) w[x] &= 0xffff0000u, hit = true;
-                                    if ((w[x] & 0x7c000000u) == 0x7c000000u) w[x] &= 0xffffu, hit = true;
-                                }
-                                if (hit) *at = v, bad = true;
+                        if ((walk.t0 + j) * F::kBn + rt >= walk.len && k_row >= 0) {
+#pragma unroll 1
+                            for (int k = 0; k < kLanes * 4; ++k) {
+                                unsigned* at = reinterpret_cast<unsigned*>(tree_smem + slot_at(slot) + (k >> 5) * (F::kBn * 128) +
+                                                                           rt * 128 + ((((k >> 2) & 7) ^ (rt & 7)) << 4)) + (k & 3);
+                                const unsigned w = *at;
+                                if ((w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u) *at = 0, bad = true;
                             }
                         }
-                        if (bad) M.vbad[walk.count & 15] = 1;
+                        bad_rows = __ballot_sync(0xffffffffu, bad);
+                        if (lane == 0) {
+                            M.vbad[(walk.tile_base + j) % kMetaRing][lw] = bad_rows;
+                            bar_arrive(&M.v_ready[(walk.tile_base + j) % kMetaRing]);
+                        }
                         signal(slot);
                     } else {
+                        if (is_v && lane == 0) bar_arrive(&M.v_ready[(walk.tile_base + j) % kMetaRing]);  // nothing to report
                         if (n_pend == 2) {
                             cp_wait<2>();
                             signal(pend[0]);
@@ -1062,7 +1116,6 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
             for (unsigned piece = 0; go; ++piece) {
                 if (!__all_sync(0xffffffffu, get_piece(piece))) break;
                 const TreePiece& walk = M.piece[piece % kPieceRing];
-                if (lane == 0 && lw == 0) M.vbad[(walk.count + 8) & 15] = 0;  // no warp is that far ahead or behind
                 const int loads = 2 * (walk.t1 - walk.t0);
                 for (int e = 0; e < loads && go; ++e) {
                     bool is_v;
@@ -1084,6 +1137,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
                                                                       lw * (F::kRaw / 4));
                     float big = 0.f;
                     bool bad = false;
+                    unsigned bad_rows = 0;
                     if constexpr (KV == 2) {
                         if (is_v) {
                             float* mine_s = scale_col + lw * 32 + lane;
@@ -1131,6 +1185,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
                                 for (int x = 0; x < 4; ++x)
                                     if (!isfinite(v[x])) v[x] = 0.f, bad = true;
                             }
+                            const unsigned hit = __ballot_sync(0xffffffffu, bad);
+                            bad = false;
+                            if (hit) bad_rows |= kLanes == 32 ? 1u << i : ((hit & 0xffffu) ? 1u << (2 * i) : 0u) | ((hit >> 16) ? 2u << (2 * i) : 0u);
                             float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
 #pragma unroll
                             for (int d = kLanes / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
@@ -1146,8 +1203,12 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
                             *reinterpret_cast<uint2*>(out + F::kSlotPart + at) = lo;
                         }
                     }
-                    if (bad) M.vbad[walk.count & 15] = 1;
                     if (is_v) {
+                        if constexpr (KV == 2) {
+                            const unsigned rows = __ballot_sync(0xffffffffu, bad);
+                            if (lane == 0) M.vbad[meta][lw] = rows;
+                        } else if (lane == 0)
+                            reinterpret_cast<unsigned short*>(M.vbad[meta])[lw] = (unsigned short)bad_rows;
 #pragma unroll
                         for (int d = 16; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
                         if (lane == 0) M.vmax[meta][lw] = big;
@@ -1167,121 +1228,97 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
         }
         if (flags) atomicOr(a.status, flags);
     } else if (warp == kTreeMmaWarp) {
-        if (lane == 0) {
+        {
             // -------------------------------------------------- MMA issue
             constexpr unsigned kIdescS = (1u << 4) | (unsigned(F::kBn >> 3) << 17) | (8u << 24);
             constexpr unsigned kIdescO = (1u << 4) | (1u << 16) | (unsigned(DP >> 3) << 17) | (8u << 24);
-            unsigned full_phase = 0, n_p[2] = {0, 0};
+            unsigned full_phase = 0, n_p = 0;  // phase bits per slot and stream
             int slot = 0;
             bool go = true;
-            const auto qk = [&](int q_tile, int stream, unsigned at) {
-                const unsigned d = tmem + stream * 128, q_lo = smem + q_tile * F::kQTile + F::kQPart,
-                               q_hi = smem + q_tile * F::kQTile, k = smem + at;
-                int acc = 0;
-#pragma unroll 1
-                for (int part = 0; part < F::kParts + 1; ++part) {
-                    // small products first: lo Q (and lo K) before hi hi
-                    const unsigned qa = part == 0 ? q_lo : q_hi, kb = F::kParts == 2 && part == 1 ? k + F::kSlotPart : k;
-#pragma unroll
-                    for (int kk = 0; kk < DP / 16; ++kk) {
-                        mma_ss(d, sw128_desc(qa + (kk >> 2) * 16384 + (kk & 3) * 32, 16),
-                               sw128_desc(kb + (kk >> 2) * (F::kBn * 128) + (kk & 3) * 32, 16), kIdescS, acc);
-                        acc = 1;
-                    }
-                }
-            };
-            const auto pv = [&](int stream, unsigned at) {
-                const unsigned d = tmem + 256 + stream * 128, p = tmem + stream * 128, v = smem + at;
-                int acc = 0;
-#pragma unroll 1
-                for (int part = 0; part < F::kParts + 1; ++part) {
-                    const unsigned pa = part == 0 ? p + 8 : p, vb = F::kParts == 2 && part == 1 ? v + F::kSlotPart : v;
-#pragma unroll
-                    for (int kk = 0; kk < F::kBn / 16; ++kk) {
-                        mma_ts(d, pa + kk * 16, sw128_desc(vb + kk * 2048, F::kBn * 128), kIdescO, acc);
-                        acc = 1;
-                    }
-                }
-            };
+            const auto at128 = [&](unsigned addr) { return sw128_desc(addr, 16); };
+            const std::uint64_t q_desc = at128(smem), v_desc = sw128_desc(smem, F::kBn * 128);
             const auto take = [&](int ns) -> int {  // next ring slot, filled
                 const int s = slot;
-                go = bar_wait(&M.full[s], (full_phase >> s) & 1, abort_flag, a.status);
+                go = __all_sync(0xffffffffu, bar_wait(&M.full[s], (full_phase >> s) & 1, abort_flag, a.status));
                 full_phase ^= 1u << s;
                 slot = s + 1 == ns ? 0 : s + 1;
                 tm_after();
                 return s;
             };
             for (unsigned piece = 0; go; ++piece) {
-                if (!get_piece(piece)) break;
+                if (!__all_sync(0xffffffffu, get_piece(piece))) break;
                 const TreePiece& walk = M.piece[piece % kPieceRing];
-                const bool pair = walk.pair;
-                const int ns = pair ? F::kBase : F::kBase + F::kExtra, tiles = walk.t1 - walk.t0;
+                const bool pair = __shfl_sync(0xffffffffu, walk.pair, 0);
+                const int ns = pair ? F::kBase : F::kBase + F::kExtra, tiles = __shfl_sync(0xffffffffu, walk.t1 - walk.t0, 0);
                 if (slot >= ns) slot = 0;
-                go = bar_wait(&M.q_full, piece & 1, abort_flag, a.status);
+                go = __all_sync(0xffffffffu, bar_wait(&M.q_full, piece & 1, abort_flag, a.status));
                 if (!go) break;
                 tm_after();
-                if (!pair) {
-                    for (int j = 0; j < min(2, tiles) && go; ++j) {
-                        const int s = take(ns);
-                        if (!go) break;
-                        qk(0, j, slot_at(s));
-                        tree_commit_to(&M.empty[s]);
-                        tree_commit_to(&M.s_full[j]);
-                    }
-                    for (int j = 0; j < tiles && go; ++j) {
-                        const int st = j & 1;
-                        const int s = take(ns);
-                        if (!go) break;
-                        go = bar_wait(&M.p_full[st], n_p[st] & 1, abort_flag, a.status);
-                        ++n_p[st];
+                // Products i of S = Q K^T and of P V, stream i & 1: one K and V
+                // tile each, or one for the two streams of a pair.  S of
+                // product i + 2 follows P V of product i, whose P it overwrites.
+                const int steps = pair ? 2 * tiles : tiles;
+                int s_k = 0, s_v = 0;
+#pragma unroll 1
+                for (int i = -2; i < steps && go; ++i) {
+                    const int st = i & 1;
+                    if (i >= 0) {
+                        if (!pair || !st) s_v = take(ns);
+                        go = go && __all_sync(0xffffffffu, bar_wait(&M.p_full[st], (n_p >> st) & 1, abort_flag, a.status));
+                        n_p ^= 1u << st;
                         if (!go) break;
                         tm_after();
-                        pv(st, slot_at(s));
-                        tree_commit_to(&M.empty[s]);
-                        tree_commit_to(&M.o_full[st]);
-                        if (j + 2 < tiles) {
-                            const int s2 = take(ns);
-                            if (!go) break;
-                            qk(0, st, slot_at(s2));
-                            tree_commit_to(&M.empty[s2]);
-                            tree_commit_to(&M.s_full[st]);
-                        }
-                    }
-                } else {
-                    int s = take(ns);
-                    if (!go) break;
-                    for (int st = 0; st < 2; ++st) {
-                        qk(st, st, slot_at(s));
-                        tree_commit_to(&M.s_full[st]);
-                    }
-                    tree_commit_to(&M.empty[s]);
-                    for (int j = 0; j < tiles && go; ++j) {
-                        s = take(ns);
-                        if (!go) break;
-                        int s2 = -1;
-                        for (int st = 0; st < 2 && go; ++st) {
-                            go = bar_wait(&M.p_full[st], n_p[st] & 1, abort_flag, a.status);
-                            ++n_p[st];
-                            if (!go) break;
-                            tm_after();
-                            pv(st, slot_at(s));
-                            tree_commit_to(&M.o_full[st]);
-                            if (st == 1) tree_commit_to(&M.empty[s]);
-                            if (j + 1 < tiles) {
-                                if (st == 0) s2 = take(ns);
-                                if (!go) break;
-                                qk(st, st, slot_at(s2));
-                                tree_commit_to(&M.s_full[st]);
-                                if (st == 1) tree_commit_to(&M.empty[s2]);
+                        const unsigned d = tmem + 256 + st * 128;
+                        const std::uint64_t v = v_desc + (slot_at(s_v) >> 4);
+                        int acc = 0;
+                        if (elect_one()) {
+#pragma unroll 1
+                        for (int part = 0; part <= F::kParts; ++part) {  // small products first: P lo (and V lo)
+                            const unsigned pa = tmem + st * 128 + (part == 0 ? 8 : 0);
+                            const std::uint64_t vb = v + (F::kParts == 2 && part == 1 ? F::kSlotPart >> 4 : 0);
+#pragma unroll 4
+                            for (int kk = 0; kk < F::kBn / 16; ++kk) {
+                                mma_ts(d, pa + kk * 16, vb + kk * (2048 >> 4), kIdescO, acc);
+                                acc = 1;
                             }
                         }
+                        if (!pair || st) tree_commit_to(&M.empty[s_v]);
+                        tree_commit_to(&M.o_full[st]);
+                        }
+                        __syncwarp();
+                    }
+                    if (i + 2 < steps) {
+                        if (!pair || !st) s_k = take(ns);
+                        if (!go) break;
+                        const unsigned d = tmem + st * 128;
+                        const std::uint64_t q = q_desc + (pair && st ? F::kQTile >> 4 : 0), k = q_desc + (slot_at(s_k) >> 4);
+                        int acc = 0;
+                        if (elect_one()) {
+#pragma unroll 1
+                        for (int part = 0; part <= F::kParts; ++part) {  // lo Q, (lo K,) hi hi
+                            const std::uint64_t qa = q + (part == 0 ? F::kQPart >> 4 : 0);
+                            const std::uint64_t kb = k + (F::kParts == 2 && part == 1 ? F::kSlotPart >> 4 : 0);
+#pragma unroll 1
+                            for (int half = 0; half < F::kHalves; ++half)
+#pragma unroll
+                                for (int kk = 0; kk < 4; ++kk) {
+                                    mma_ss(d, qa + half * (16384 >> 4) + kk * 2, kb + half * ((F::kBn * 128) >> 4) + kk * 2,
+                                           kIdescS, acc);
+                                    acc = 1;
+                                }
+                        }
+                        if (!pair || st) tree_commit_to(&M.empty[s_k]);
+                        tree_commit_to(&M.s_full[st]);
+                        }
+                        __syncwarp();
                     }
                 }
                 if (!go) break;
-                release_piece(piece);
+                if (lane == 0) release_piece(piece);
             }
             // nothing of this CTA's may be in flight when its memory is given back
-            tree_commit_to(&M.drain);
+            if (lane == 0) tree_commit_to(&M.drain);
+#pragma unroll 1
             for (unsigned i = 0; i < kTreeSpin && !bar_test(&M.drain, 0); ++i) {
             }
         }
@@ -1303,14 +1340,16 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(TreeAttn a, const flo
     const TreeRec rec = recs[blockIdx.x];
     const int row = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (rec.pieces < 2 || row >= rec.rows) return;
-    const int pr = row < rec.split ? row : 128 + row - rec.split, group = a.hq / a.hkv;
+    const int pr = row < rec.split ? row : 128 + row - rec.split, group = a.group;
     constexpr int kPer = DP / 32;
     const long long slot_floats = (long long)kTreeRows * (DP + 2);
     const auto slot_of = [&](int i) { return partial + (2ll * (blockIdx.x + i) + (i == 0)) * slot_floats; };
     float top = -INFINITY;
+#pragma unroll 1
     for (int i = 0; i < rec.pieces; ++i) top = fmaxf(top, slot_of(i)[kTreeRows * DP + pr]);
     float l = 0.f, o[kPer] = {};
     if (top != -INFINITY) {
+#pragma unroll 2
         for (int i = 0; i < rec.pieces; ++i) {
             const float* slot = slot_of(i);
             const float f = ex2(slot[kTreeRows * DP + pr] - top);
@@ -1319,9 +1358,10 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(TreeAttn a, const flo
             for (int e = 0; e < kPer; ++e) o[e] += slot[pr * DP + e * 32 + lane] * f;
         }
     } else {  // nothing seen, or nothing but NaN scores
+#pragma unroll 1
         for (int i = 0; i < rec.pieces; ++i) l += slot_of(i)[kTreeRows * DP + kTreeRows + pr];
     }
-    const int vec = rec.row0 + row, node = vec / group, head = rec.head * group + vec - node * group;
+    const int vec = rec.row0 + row, node = unsigned(vec) / unsigned(group), head = rec.head * group + vec - node * group;
     float* dst = a.out + (long long)(rec.c0 + node) * a.ldo + (long long)head * a.dim;
 #pragma unroll
     for (int e = 0; e < kPer; ++e)

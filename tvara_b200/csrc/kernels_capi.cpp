@@ -347,7 +347,8 @@ void check_tree_sizes(std::size_t n_seq, std::size_t capacity, std::size_t max_n
     if (capacity > 0x7fffffff) throw std::invalid_argument("invalid tree row capacity");
     if (!max_nodes || max_nodes > std::size_t(tvara::kTreeMaxNodes))
         throw std::invalid_argument("trees hold 1 to 1024 nodes");
-    if (!max_blocks || max_blocks > 0x7fffffff || !block_tokens || block_tokens > (1u << 20))
+    if (!max_blocks || max_blocks > 0x7fffffff || !block_tokens || block_tokens > (1u << 20) ||
+        std::uint64_t(max_blocks) * block_tokens > (1ull << 44))
         throw std::invalid_argument("invalid KV pool size");
 }
 
@@ -372,8 +373,10 @@ tvara::TreeAttn tree_attention_job(const tvara_tree_attention_args* a) {
     j.kv_kind = a->kv_dtype == TVARA_KV_F32 ? 0 : a->kv_dtype == TVARA_KV_F16 ? 1 : 2;
     j.hq = int(a->heads);
     j.hkv = int(a->kv_heads);
+    j.group = j.hq / j.hkv;
     j.dim = int(a->head_dim);
     j.bt = int(a->block_tokens);
+    j.bt_inverse = ~0ull / a->block_tokens + 1;
     j.n_seq = int(a->n_seq);
     j.capacity = int(a->capacity);
     j.max_nodes = int(a->max_nodes);

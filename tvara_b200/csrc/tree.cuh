@@ -36,8 +36,9 @@ void launch_tree_plan(const TreePlan& a, cudaStream_t s);
 
 struct TreeAttn {
     int kv_kind = 0;  // 0 F32, 1 F16, 2 int8 with row scales
-    int hq = 0, hkv = 0, dim = 0, bt = 0;
+    int hq = 0, hkv = 0, group = 1, dim = 0, bt = 0;  // group = hq / hkv
     int n_seq = 0, capacity = 0, max_nodes = 0, words = 0, max_blocks = 0, stride = 0;
+    unsigned long long bt_inverse = 0;  // 2^64 / bt rounded up, 0 for bt 1
     long long ldq = 0, ldo = 0;
     long long block_stride = 0, layer_offset = 0, kind_stride = 0;  // elements
     const float* q = nullptr;
