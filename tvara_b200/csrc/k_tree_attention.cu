@@ -10,6 +10,7 @@
 #include <cuda_fp16.h>
 
 #include "split.cuh"
+#include "tma.cuh"
 #include "tree.cuh"
 
 namespace tvara {
@@ -27,9 +28,9 @@ __device__ __forceinline__ bool tree_sequence_ok(const TreeAttn& a, int s, int& 
            len <= (long long)a.stride * a.bt && len <= 0x7fffffff - 2 * kTreeMaxNodes;
 }
 
-// Element offset of the K row (head 0 of the layer) of index p of a sequence
-// (cached positions, then nodes), or -1 with the status bit for a block or
-// slot outside the pool.
+// Row (of dim elements) in the pool that holds K of head 0 of the layer for
+// index p of a sequence (cached positions, then nodes), or -1 with the status
+// bit for a block or slot outside the pool.
 // x / bt for x < 2^44 by the reciprocal 2^64 / bt rounded up (0 stands for
 // bt 1): it is too large by less than bt / 2^64 <= 2^-44, so the product is
 // off by less than one step of the quotient's fraction.
@@ -52,7 +53,7 @@ __device__ __forceinline__ long long tree_row(const TreeAttn& a, int s, int c0, 
         flags |= kTreeBadBlock;
         return -1;
     }
-    return block * a.block_stride + a.layer_offset + off * a.dim;
+    return block * a.block_rows + a.layer_rows + off;
 }
 
 // ---------------------------------------------------------- any shape
@@ -108,7 +109,7 @@ __global__ void __launch_bounds__(kAnyWarps * 32) tree_any_kernel(TreeAttn a) {
         }
         const long long base = tree_row(a, lo, c0, len, int(p), flags);
         if (base < 0) continue;
-        const long long k = base + (long long)g * a.bt * a.dim, v = k + a.kind_stride;
+        const long long k_row = base + (long long)g * a.bt, k = k_row * a.dim, v = k + a.kind_rows * a.dim;
         float dot = 0.f;
 #pragma unroll
         for (int e = 0; e < E; ++e)
@@ -117,8 +118,8 @@ __global__ void __launch_bounds__(kAnyWarps * 32) tree_any_kernel(TreeAttn a) {
         for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
         float s = dot * scale, sv = 1.f;
         if (a.scales) {
-            s *= a.scales[k / a.dim];
-            sv = a.scales[v / a.dim];
+            s *= a.scales[k_row];
+            sv = a.scales[k_row + a.kind_rows];
         }
         const float mn = fmaxf(m, s);
         const float ref = mn == -INFINITY ? 0.f : mn;
@@ -432,8 +433,9 @@ __device__ __forceinline__ unsigned node_bits(const TreeAttn& a, int c0, int n, 
 }
 
 template <int KV, int DP>
-__global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, float* partial, TreeRec* recs,
-                                                                   int min_weight) {
+__global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_constant__ CUtensorMap kv_map,
+                                                                   const __grid_constant__ TreeAttn a, float* partial,
+                                                                   TreeRec* recs, int min_weight) {
     using F = TreeForm<KV, DP>;
     extern __shared__ __align__(1024) unsigned char tree_smem[];
     TreeMeta& M = *reinterpret_cast<TreeMeta*>(tree_smem + F::kOffMeta);
@@ -946,14 +948,14 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
         int slot = 0, flags = 0;
         const int row_bytes = a.dim * F::kElem, chunks = row_bytes >> 4;
         const unsigned char* pool = static_cast<const unsigned char*>(a.kv);
-        // This lane's row of a tile: the element offset of its K row (-1: none).
+        // This lane's row of a tile: its K row in the pool (-1: none).
         // V of a tile uses the row that K left behind: by the order of the
         // entries it is the last or the last but one.
         const auto row_of = [&](const TreePiece& w, int j) -> long long {
             const int p = (w.t0 + j) * F::kBn + lw * kRowsPerWarp + (lane % kRowsPerWarp);
             if (p >= w.len + w.n) return -1;
             const long long at = tree_row(a, w.s, w.c0, w.len, p, flags);
-            return at < 0 ? -1 : at + (long long)w.head * a.bt * a.dim;
+            return at < 0 ? -1 : at + (long long)w.head * a.bt;
         };
         if constexpr (KV == 1) {
             bool go = true, prev_pair = false;
@@ -1003,17 +1005,40 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
                     empty_phase ^= 1u << slot;
                     if (!is_v && lane == 0) M.valid[(walk.tile_base + j) % kMetaRing][lw] = have;
                     const unsigned dst = smem + slot_at(slot);
-                    const long long shift = is_v ? a.kind_stride : 0;
+                    const long long shift = is_v ? a.kind_rows : 0;
                     constexpr int kLanes = DP / 8, kStep = 32 / kLanes;  // lanes per row, rows per instruction
                     const int ch = lane % kLanes;
-#pragma unroll 4
+                    // a slab of 32 cached positions, all in the pool: by TMA,
+                    // box_rows rows x 64 columns at a time
+                    if (a.box_rows && have == 0xffffffffu && (walk.t0 + j) * F::kBn + lw * 32 + 32 <= walk.len) {
+                        if (lane == 0) {
+                            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(sm_addr(&M.full[slot])),
+                                         "r"(32 * DP * 2)
+                                         : "memory");
+                            if (is_v) {
+                                M.vbad[(walk.tile_base + j) % kMetaRing][lw] = 0;
+                                bar_arrive(&M.v_ready[(walk.tile_base + j) % kMetaRing]);
+                            }
+                        }
+                        __syncwarp();
+                        if ((lane & (a.box_rows - 1)) == 0) {
+#pragma unroll
+                            for (int half = 0; half < F::kHalves; ++half)
+                                tma_load_2d(dst + half * (F::kBn * 128) + (lw * 32 + lane) * 128, &kv_map, half * 64,
+                                            int(k_row + shift), sm_addr(&M.full[slot]));
+                        }
+                        __syncwarp();
+                        slot = slot + 1 == ns ? 0 : slot + 1;
+                        continue;
+                    }
+#pragma unroll 2
                     for (int i = 0; i < 32 / kStep; ++i) {
                         const int rr = i * kStep + lane / kLanes;
                         const long long at = __shfl_sync(0xffffffffu, k_row, rr);
                         const bool ok = at >= 0 && ch < chunks;
                         const int rt = lw * 32 + rr;
                         cp16(dst + (ch >> 3) * (F::kBn * 128) + rt * 128 + (((ch & 7) ^ (rt & 7)) << 4),
-                             ok ? pool + (at + shift) * 2 + ch * 16 : pool, ok ? 16u : 0u);
+                             ok ? pool + (at + shift) * row_bytes + ch * 16 : pool, ok ? 16u : 0u);
                     }
                     cp_commit();
                     if (is_v && (walk.t0 + j + 1) * F::kBn > walk.len) {
@@ -1093,18 +1118,18 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(TreeAttn a, f
                         reinterpret_cast<unsigned short*>(valid)[lw] = (unsigned short)(have & 0xffffu);
                 }
                 const unsigned dst = smem + F::kOffRaw + raw_in * F::kRaw + lw * (F::kRaw / 4);
-                const long long shift = is_v ? a.kind_stride : 0;
+                const long long shift = is_v ? a.kind_rows : 0;
 #pragma unroll 4
                 for (int i = 0; i < kIters; ++i) {
                     const int rr = i * kStep + lane / kLanes;
                     const long long at = __shfl_sync(0xffffffffu, mine_row, rr);
                     const bool ok = at >= 0 && ch < chunks;
-                    cp16(dst + (i * 32 + lane) * 16, ok ? pool + (at + shift) * F::kElem + ch * 16 : pool, ok ? 16u : 0u);
+                    cp16(dst + (i * 32 + lane) * 16, ok ? pool + (at + shift) * row_bytes + ch * 16 : pool, ok ? 16u : 0u);
                 }
                 if constexpr (KV == 2) {  // this lane's row scale, straight into its column
                     const int ring = int((ahead.tile_base + j) % F::kScaleRing);
                     const unsigned to = smem + F::kOffScale + ((ring * 2 + is_v) * F::kBn + lw * 32 + lane) * 4;
-                    cp4(to, mine_row >= 0 ? a.scales + (mine_row + shift) / a.dim : a.scales, mine_row >= 0 ? 4u : 0u);
+                    cp4(to, mine_row >= 0 ? a.scales + (mine_row + shift) : a.scales, mine_row >= 0 ? 4u : 0u);
                 }
                 cp_commit();
                 raw_in = raw_in + 1 == F::kRawDepth ? 0 : raw_in + 1;
@@ -1384,7 +1409,23 @@ void run_tree_mma(const TreeAttn& a, void* workspace, cudaStream_t s) {
     auto* recs = static_cast<TreeRec*>(workspace);
     auto* partial = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + 4096);
     TVARA_CUDA(cudaFuncSetAttribute(tree_mma_kernel<KV, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem));
-    tree_mma_kernel<KV, DP><<<ctas, kTreeThreads, F::kSmem, s>>>(a, partial, recs, 2);
+    // F16 pools of whole 128-byte row halves and blocks of a multiple of 8
+    // positions: cached positions come by TMA, whose boxes never cross a block
+    CUtensorMap map{};
+    TreeAttn job = a;
+    job.box_rows = 0;
+    const unsigned long long rows = (unsigned long long)a.max_blocks * a.block_rows;
+    if (KV == 1 && a.dim % 64 == 0 && a.bt % 8 == 0 && rows < 0x7fffffffull) {
+        job.box_rows = a.bt % 32 == 0 ? 32 : a.bt % 16 == 0 ? 16 : 8;
+        const cuuint64_t dims[2] = {cuuint64_t(a.dim), cuuint64_t(rows)};
+        const cuuint64_t strides[1] = {cuuint64_t(a.dim) * 2};
+        const cuuint32_t box[2] = {64, cuuint32_t(job.box_rows)}, ones[2] = {1, 1};
+        if (tensor_map_encoder()(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(a.kv), dims, strides, box, ones,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            throw std::runtime_error("cuTensorMapEncodeTiled failed for the KV pool");
+    }
+    tree_mma_kernel<KV, DP><<<ctas, kTreeThreads, F::kSmem, s>>>(map, job, partial, recs, 2);
     TVARA_LAUNCHED();
     tree_combine_kernel<DP><<<dim3(unsigned(ctas), kTreeRows / 8), 256, 0, s>>>(a, partial, recs);
     TVARA_LAUNCHED();

@@ -385,9 +385,9 @@ tvara::TreeAttn tree_attention_job(const tvara_tree_attention_args* a) {
     j.stride = int(a->table_stride);
     j.ldq = (long long)a->q_stride;
     j.ldo = (long long)a->out_stride;
-    j.kind_stride = (long long)a->kv_heads * a->block_tokens * a->head_dim;
-    j.layer_offset = (long long)a->layer * 2 * j.kind_stride;
-    j.block_stride = (long long)a->layers * 2 * j.kind_stride;
+    j.kind_rows = (long long)a->kv_heads * a->block_tokens;
+    j.layer_rows = (long long)a->layer * 2 * j.kind_rows;
+    j.block_rows = (long long)a->layers * 2 * j.kind_rows;
     j.q = a->q;
     j.out = a->out;
     j.kv = a->pool;

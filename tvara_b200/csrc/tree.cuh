@@ -40,7 +40,8 @@ struct TreeAttn {
     int n_seq = 0, capacity = 0, max_nodes = 0, words = 0, max_blocks = 0, stride = 0;
     unsigned long long bt_inverse = 0;  // 2^64 / bt rounded up, 0 for bt 1
     long long ldq = 0, ldo = 0;
-    long long block_stride = 0, layer_offset = 0, kind_stride = 0;  // elements
+    long long block_rows = 0, layer_rows = 0, kind_rows = 0;  // rows of dim elements: a block, to the layer, K to V
+    int box_rows = 0;  // rows of a TMA box, 0: no TMA
     const float* q = nullptr;
     float* out = nullptr;
     const void* kv = nullptr;
