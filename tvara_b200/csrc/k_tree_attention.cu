@@ -368,20 +368,53 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float max3(float x, float y, float z) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+    return r;
+}
 __device__ __forceinline__ float two_to(int e) { return __uint_as_float(unsigned(127 + e) << 23); }  // |e| <= 126
 // The power of two that brings a largest |value| into [2^14, 2^15).
 __device__ __forceinline__ int lift(float top) {
     const int e = int((__float_as_uint(top) >> 23) & 255) - 127;
     return top > 0.f && e < 128 ? max(-113, min(112, 14 - e)) : 0;
 }
-// p in [0, 2^11] as hi (an integer) + lo (|lo| <= 1/2): F16 each, lo's
-// rounding is 2^-13, that is 2^-24 of the row's largest weight.
-__device__ __forceinline__ void split_weight(float x, float y, unsigned& hi, unsigned& lo) {
-    constexpr float kRound = 12582912.f;  // 1.5 * 2^23
-    const float hx = __fsub_rn(__fadd_rn(x, kRound), kRound), hy = __fsub_rn(__fadd_rn(y, kRound), kRound);
-    const __half2 h = __floats2half2_rn(hx, hy), l = __floats2half2_rn(x - hx, y - hy);
-    hi = *reinterpret_cast<const unsigned*>(&h);
-    lo = *reinterpret_cast<const unsigned*>(&l);
+// Packed pairs of F32.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair_of(float x, float y) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void halves_of(f32x2 r, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(r)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ unsigned half2_of(f32x2 v) {
+    float x, y;
+    halves_of(v, x, y);
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const unsigned*>(&h);
+}
+// A pair of weights in [0, 2^11] as hi (integers) + lo (|lo| <= 1/2): F16
+// each, lo's rounding is 2^-13, that is 2^-24 of the row's largest weight.
+__device__ __forceinline__ void split_weight(f32x2 p, unsigned& hi, unsigned& lo) {
+    const f32x2 up = pair_of(12582912.f, 12582912.f), down = pair_of(-12582912.f, -12582912.f);  // 1.5 * 2^23
+    const f32x2 h = add2(add2(p, up), down);
+    hi = half2_of(h);
+    lo = half2_of(fma2(h, pair_of(-1.f, -1.f), p));
 }
 
 // What every role knows of a sequence, and its tiles in the global order
@@ -656,7 +689,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                     cp_commit();
                     cp_wait<0>();
                     __syncwarp();
-#pragma unroll 1
+#pragma unroll 4
                     for (int i = 0; i < most; ++i) {
                         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
                         if (lane < DP / 4) x = *reinterpret_cast<const float4*>(tile + (lane >> 3) * 16384 + i * 128 + ((lane & 7) << 4));
@@ -756,7 +789,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                                 if (!(see >> i & 1)) x[i] = 0xff800000u;
                         }
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) tops[i & 3] = fmaxf(tops[i & 3], __uint_as_float(x[i]));
+                        for (int i = 0; i < 32; i += 2)
+                            tops[(i >> 1) & 3] = max3(tops[(i >> 1) & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
                     }
                     const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
                     const float mn = fmaxf(m, top * c);
@@ -776,54 +810,49 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                     }
                     // P over S, sixteen positions (one K step of the MMA) at a
                     // time: hi in their first eight columns, lo in the others.
-                    float sum0 = 0.f, sum1 = 0.f;
+                    f32x2 sums[2] = {0, 0};
+                    const f32x2 c2 = pair_of(c, c), off2 = pair_of(off, off), unit2 = pair_of(v_unit, v_unit);
 #pragma unroll 1
-                    for (int k = 0; k < F::kBn / 16; ++k) {
-                        unsigned x[16], y[16];
-                        tm_ld16(s_at + 16 * k, x);
+                    for (int k = 0; k < F::kBn / 32; ++k) {
+                        unsigned x[32];
+                        tm_ld32(s_at + 32 * k, x);
                         if constexpr (KV != 1) {
 #pragma unroll
-                            for (int i = 0; i < 16; i += 4) {
-                                const float4 f = *reinterpret_cast<const float4*>(k_scale + 16 * k + i);
-                                x[i] = __float_as_uint(__uint_as_float(x[i]) * f.x);
-                                x[i + 1] = __float_as_uint(__uint_as_float(x[i + 1]) * f.y);
-                                x[i + 2] = __float_as_uint(__uint_as_float(x[i + 2]) * f.z);
-                                x[i + 3] = __float_as_uint(__uint_as_float(x[i + 3]) * f.w);
+                            for (int i = 0; i < 32; i += 2) {
+                                float v0, v1;
+                                halves_of(mul2(pair_of(__uint_as_float(x[i]), __uint_as_float(x[i + 1])),
+                                               *reinterpret_cast<const f32x2*>(k_scale + 32 * k + i)),
+                                          v0, v1);
+                                x[i] = __float_as_uint(v0);
+                                x[i + 1] = __float_as_uint(v1);
                             }
                         }
-                        float p[16];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) p[i] = ex2(fmaf(__uint_as_float(x[i]), c, off));
-                        const unsigned see = all ? 0xffffffffu : see_of(k >> 1) >> ((k & 1) * 16);
                         if (!all) {
+                            const unsigned see = see_of(k);
 #pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                if (!(see >> i & 1)) p[i] = 0.f;
+                            for (int i = 0; i < 32; ++i)
+                                if (!(see >> i & 1)) x[i] = 0xff800000u;  // weight 0
                         }
 #pragma unroll
-                        for (int i = 0; i < 16; i += 2) {
-                            sum0 += p[i];
-                            sum1 += p[i + 1];
-                        }
-                        if constexpr (KV != 1) {
+                        for (int g = 0; g < 2; ++g) {
+                            unsigned y[16];
 #pragma unroll
-                            for (int i = 0; i < 16; i += 4) {
-                                const float4 f = *reinterpret_cast<const float4*>(v_scale + 16 * k + i);
-                                p[i] *= f.x * v_unit;
-                                p[i + 1] *= f.y * v_unit;
-                                p[i + 2] *= f.z * v_unit;
-                                p[i + 3] *= f.w * v_unit;
+                            for (int i = 0; i < 8; ++i) {
+                                const int at = 16 * g + 2 * i;
+                                const f32x2 v = pair_of(__uint_as_float(x[at]), __uint_as_float(x[at + 1]));
+                                float p0, p1;
+                                halves_of(fma2(v, c2, off2), p0, p1);
+                                f32x2 p = pair_of(ex2(p0), ex2(p1));
+                                sums[i & 1] = add2(sums[i & 1], p);
+                                if constexpr (KV != 1)
+                                    p = mul2(p, mul2(unit2, *reinterpret_cast<const f32x2*>(v_scale + 32 * k + at)));
+                                split_weight(p, y[i], y[8 + i]);
                             }
-                            if (!all) {  // a masked row's scale may be anything
-#pragma unroll
-                                for (int i = 0; i < 16; ++i)
-                                    if (!(see >> i & 1)) p[i] = 0.f;
-                            }
+                            tm_st16(s_at + 32 * k + 16 * g, y);
                         }
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) split_weight(p[2 * i], p[2 * i + 1], y[i], y[8 + i]);
-                        tm_st16(s_at + 16 * k, y);
                     }
+                    float sum0, sum1;
+                    halves_of(add2(sums[0], sums[1]), sum0, sum1);
                     l += sum0 + sum1;
                     tm_wait_st();
                 }
@@ -834,12 +863,16 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                 if (!go) break;
                 tm_after();
                 if (warp_live) {
+                    const f32x2 keep2 = pair_of(keep, keep);
 #pragma unroll
                     for (int k = 0; k < DP / 32; ++k) {
                         unsigned x[32];
                         tm_ld32(o_at + 32 * k, x);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[32 * k + i] = fmaf(o[32 * k + i], keep, __uint_as_float(x[i]));
+                        for (int i = 0; i < 32; i += 2)
+                            halves_of(fma2(pair_of(o[32 * k + i], o[32 * k + i + 1]), keep2,
+                                           pair_of(__uint_as_float(x[i]), __uint_as_float(x[i + 1]))),
+                                      o[32 * k + i], o[32 * k + i + 1]);
                     }
                 }
             }
