@@ -1064,7 +1064,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                         slot = slot + 1 == ns ? 0 : slot + 1;
                         continue;
                     }
-#pragma unroll 2
+#pragma unroll 4
                     for (int i = 0; i < 32 / kStep; ++i) {
                         const int rr = i * kStep + lane / kLanes;
                         const long long at = __shfl_sync(0xffffffffu, k_row, rr);
@@ -1082,12 +1082,22 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                         const int rt = lw * 32 + lane;
                         bool bad = false;
                         if ((walk.t0 + j) * F::kBn + rt >= walk.len && k_row >= 0) {
+                            const auto chunk = [&](int k) {
+                                return reinterpret_cast<uint4*>(tree_smem + slot_at(slot) + (k >> 3) * (F::kBn * 128) + rt * 128 +
+                                                                (((k & 7) ^ (rt & 7)) << 4));
+                            };
+                            // an exponent of all ones carries into the sign bit
+                            const auto full = [](unsigned w) { return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u; };
+                            unsigned any = 0;
+#pragma unroll 8
+                            for (int k = 0; k < kLanes; ++k) {
+                                const uint4 w = *chunk(k);
+                                any |= full(w.x) | full(w.y) | full(w.z) | full(w.w);
+                            }
+                            if (any) {
+                                bad = true;
 #pragma unroll 1
-                            for (int k = 0; k < kLanes * 4; ++k) {
-                                unsigned* at = reinterpret_cast<unsigned*>(tree_smem + slot_at(slot) + (k >> 5) * (F::kBn * 128) +
-                                                                           rt * 128 + ((((k >> 2) & 7) ^ (rt & 7)) << 4)) + (k & 3);
-                                const unsigned w = *at;
-                                if ((w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u) *at = 0, bad = true;
+                                for (int k = 0; k < kLanes; ++k) *chunk(k) = make_uint4(0, 0, 0, 0);
                             }
                         }
                         bad_rows = __ballot_sync(0xffffffffu, bad);
