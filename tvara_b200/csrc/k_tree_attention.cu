@@ -182,9 +182,11 @@ __global__ void __launch_bounds__(kAnyWarps * 32) tree_any_kernel(TreeAttn a) {
 // (each CTA scans the lengths and cuts out its run), so ragged batches and a
 // single long sequence fill the device alike; an item cut by a run boundary
 // leaves partial (O, m, l) in the workspace for tree_combine_kernel.
-constexpr int kTreeThreads = 512;   // WG0, WG1 softmax; WG2 loads; warp 12 issues the MMAs, warp 13 deals the pieces
+constexpr int kTreeThreads = 512;   // WG0, WG1 softmax; WG2 loads; warp 12 issues the MMAs, warp 13 deals
+                                    // the pieces, warp 14 fetches the rows that WG2 converts (F32, int8)
 constexpr int kTreeMmaWarp = 12;
 constexpr int kTreePieceWarp = 13;
+constexpr int kTreeRawWarp = 14;
 constexpr int kTreeLoadWarp = 8;
 constexpr unsigned kTreeSpin = 1u << 26;
 constexpr int kTreeRows = 256;      // query vectors of a partial slot
@@ -203,6 +205,7 @@ struct TreeForm {  // KV: 0 F32, 1 F16, 2 int8
     static constexpr int kQTile = 2 * kQPart;
     static constexpr int kSlotPart = kHalves * kBn * 128;
     static constexpr int kSlot = kParts * kSlotPart;     // one K or V tile
+    static constexpr int kItemWeight = 8;                // an item's own cost (Q, merge, output), in tiles
     static constexpr int kElem = KV == 0 ? 4 : KV == 1 ? 2 : 1;
     static constexpr int kRaw = KV == 1 ? 0 : kBn * DP * kElem;  // one unconverted tile
     static constexpr int kRawDepth = KV == 1 ? 0 : DP == 64 ? 4 : KV == 0 ? 2 : 3;
@@ -250,18 +253,22 @@ struct TreeMeta {  // at kOffMeta
     std::uint64_t v_ready[kMetaRing];  // a tile's V scales and vbad are in place
     std::uint64_t q_full, merge_ready, merge_read, drain;
     std::uint64_t piece_full[kPieceRing], piece_empty[kPieceRing];
+    std::uint64_t raw_full[4], raw_empty[4];
     union {
         TreePiece piece[kPieceRing];
         long long warp_sum[16];  // while the run is cut out
     };
     alignas(16) unsigned valid[kMetaRing][4];   // columns of a tile that hold a row
     alignas(16) float vmax[kMetaRing][4];       // largest V scale per load warp
-    unsigned vbad[kMetaRing][4];    // nodes whose V (kept out of the products: 0 * inf) is not finite
-    long long total, excl0, excl1;
-    int seq0, seq1;
+    union {
+        unsigned vbad[kMetaRing][4];  // nodes whose V (kept out of the products: 0 * inf) is not finite
+        struct {                      // while the run is cut out
+            long long total, excl0, excl1;
+            int seq0, seq1, bad;
+        };
+    };
     unsigned tmem;
     int abort_flag;
-    int bad;
 };
 static_assert(sizeof(TreeMeta) <= kTreeMetaBytes);
 
@@ -357,6 +364,11 @@ __device__ __forceinline__ void cp16(unsigned dst, const void* src, unsigned byt
 }
 __device__ __forceinline__ void cp4(unsigned dst, const void* src, unsigned bytes) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bulk_load(unsigned dst, const void* src, unsigned bytes, unsigned bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"(bar)
+                 : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -492,7 +504,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
 #pragma unroll 1
         for (int i = 0; i < kPieceRing; ++i) {
             bar_init(&M.piece_full[i], 1);
-            bar_init(&M.piece_empty[i], 13);  // 8 softmax warps, 4 load warps, the MMA thread
+            bar_init(&M.piece_empty[i], KV == 1 ? 13 : 14);  // 8 softmax warps, 4 load warps, MMA, row fetch
+            bar_init(&M.raw_full[i], KV == 2 ? 33 : 1);
+            bar_init(&M.raw_empty[i], 4);
         }
         bar_init(&M.q_full, 8);
         bar_init(&M.merge_ready, 4);
@@ -511,7 +525,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
         TreeSeq q;
         if (s >= a.n_seq) return 0;
         if (!tree_seq<F>(a, s, q)) M.bad = 1;
-        return q.total ? q.total * q.weight : 0;
+        return q.total ? q.total * q.weight + (long long)q.groups * a.hkv * F::kItemWeight : 0;
     };
     long long mine = 0;
 #pragma unroll 1
@@ -569,16 +583,24 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
     if (warp == kTreePieceWarp) {
         // --------------------------------------------------------- pieces
         if (lane == 0) {
-            const int seq1 = M.seq1;
+            const int seq1 = M.seq1, seq0 = M.seq0;  // read before the first piece: their place is used again
+            const long long excl1 = M.excl1, excl0 = M.excl0;
             TreeSeq q;
             tree_seq<F>(a, seq1, q);
-            const long long u1 = min(q.total, (w1 - M.excl1 + q.weight - 1) / q.weight);
-            tree_seq<F>(a, M.seq0, q);
-            long long u = (w0 - M.excl0 + q.weight - 1) / q.weight;
+            // Item i of a sequence takes the weights from i (tiles weight + kItemWeight)
+            // on, its tile t starts at t weight of them; a tile belongs to the
+            // CTA whose run holds its start.
+            const auto tile_at = [&](long long w) {
+                const long long each = q.tiles * q.weight + F::kItemWeight, i = w / each;
+                return i * q.tiles + min(q.tiles, (w - i * each + q.weight - 1) / q.weight);
+            };
+            const long long u1 = min(q.total, tile_at(w1 - excl1));
+            tree_seq<F>(a, seq0, q);
+            long long u = tile_at(w0 - excl0);
             unsigned count = 0, tile_base = 0;
             bool go = true;
 #pragma unroll 1
-            for (int seq = M.seq0; go; ++count) {
+            for (int seq = seq0; go; ++count) {
                 long long end = seq == seq1 ? u1 : q.total;
 #pragma unroll 1
                 while (u >= end && seq < seq1) {
@@ -619,7 +641,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                 bar_arrive(&M.piece_full[ring]);
                 tile_base += unsigned(t1 - t0);
                 if (t0 == 0 && t1 < q.tiles) {  // continues in other CTAs: up to the one its last tile starts in
-                    const long long last = M.excl1 + (item * q.tiles + q.tiles - 1) * q.weight;
+                    const long long last = excl1 + item * (q.tiles * q.weight + F::kItemWeight) + (q.tiles - 1) * q.weight;
                     TreeRec rec;
                     rec.c0 = q.c0;
                     rec.row0 = row0;
@@ -644,6 +666,15 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                M.piece[i % kPieceRing].rows != 0;
     };
     const auto release_piece = [&](unsigned i) { bar_arrive(&M.piece_empty[i % kPieceRing]); };
+
+    const int row_bytes = a.dim * F::kElem, chunks = row_bytes >> 4;
+    const unsigned char* pool = static_cast<const unsigned char*>(a.kv);
+    // Index p of a piece's sequence (cached positions, then nodes): its K row in the pool (-1: none).
+    const auto row_of = [&](const TreePiece& w, int p, int& flags) -> long long {
+        if (p >= w.len + w.n) return -1;
+        const long long at = tree_row(a, w.s, w.c0, w.len, p, flags);
+        return at < 0 ? -1 : at + (long long)w.head * a.bt;
+    };
 
     if (warp < kTreeLoadWarp) {
         // ------------------------------------------------ softmax warpgroups
@@ -979,17 +1010,6 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
         constexpr int kRowsPerWarp = F::kBn / 4;
         unsigned empty_phase = 0xffffffffu;
         int slot = 0, flags = 0;
-        const int row_bytes = a.dim * F::kElem, chunks = row_bytes >> 4;
-        const unsigned char* pool = static_cast<const unsigned char*>(a.kv);
-        // This lane's row of a tile: its K row in the pool (-1: none).
-        // V of a tile uses the row that K left behind: by the order of the
-        // entries it is the last or the last but one.
-        const auto row_of = [&](const TreePiece& w, int j) -> long long {
-            const int p = (w.t0 + j) * F::kBn + lw * kRowsPerWarp + (lane % kRowsPerWarp);
-            if (p >= w.len + w.n) return -1;
-            const long long at = tree_row(a, w.s, w.c0, w.len, p, flags);
-            return at < 0 ? -1 : at + (long long)w.head * a.bt;
-        };
         if constexpr (KV == 1) {
             bool go = true, prev_pair = false;
             int pend[2], n_pend = 0;
@@ -1018,9 +1038,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                     const int j = walk.entry(e, is_v);
                     if (!is_v) {
                         row_prev = row_cur;
-                        row_cur = row_of(walk, j);
+                        row_cur = row_of(walk, (walk.t0 + j) * F::kBn + lw * 32 + lane, flags);
                         k_last = j;
                     }
+                    // V of a tile uses the row that K left behind: by the order of the
+                    // entries it is the last or the last but one
                     const long long k_row = j == k_last ? row_cur : row_prev;
                     const unsigned have = __ballot_sync(0xffffffffu, k_row >= 0);
                     if (slot >= F::kBase && wait_q) {
@@ -1122,65 +1144,21 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                 if (lane == 0) release_piece(piece);
             }
             drain();
+            // on the way out after an error: the slots' own copies first
+#pragma unroll 1
+            for (int i = 0; i < F::kBase + F::kExtra && *abort_flag; ++i)
+#pragma unroll 1
+                for (unsigned k = 0; k < (1u << 20) && !bar_test(&M.full[i], empty_phase >> i & 1); ++k) {
+                }
         } else {
-            // Raw rows land in a small ring by cp.async, each 16 bytes in the
-            // place of the thread that converts them, so a thread waits only
-            // for its own copies.
+            // Rows that the row fetch warp (below) has put into the raw ring
+            // become F16 operands.
             bool go = true;
-            unsigned piece_issue = 0xffffffffu;  // the piece that is being fetched
-            int e_issue = 0, loads_issue = 0, k_last = -1;
-            long long row_cur = -1, row_prev = -1;
-            bool more = true;
-            int raw_in = 0, raw_out = 0;
+            int raw = 0;
+            unsigned raw_phase = 0;
             constexpr int kLanes = DP * F::kElem / 16, kStep = 32 / kLanes;  // lanes per row, rows per instruction
             constexpr int kIters = kRowsPerWarp / kStep;
             const int ch = lane % kLanes;
-            const auto issue = [&]() {
-                if (e_issue == loads_issue) {
-                    more = __all_sync(0xffffffffu, get_piece(++piece_issue));
-                    if (!more) return;
-                    e_issue = 0;
-                    loads_issue = 2 * (M.piece[piece_issue % kPieceRing].t1 - M.piece[piece_issue % kPieceRing].t0);
-                    k_last = -1;
-                }
-                const TreePiece& ahead = M.piece[piece_issue % kPieceRing];
-                bool is_v;
-                const int j = ahead.entry(e_issue++, is_v);
-                if (!is_v) {
-                    row_prev = row_cur;
-                    row_cur = row_of(ahead, j);
-                    k_last = j;
-                }
-                const long long mine_row = j == k_last ? row_cur : row_prev;
-                const unsigned have = __ballot_sync(0xffffffffu, mine_row >= 0);
-                if (!is_v && lane == 0) {
-                    unsigned* valid = M.valid[(ahead.tile_base + j) % kMetaRing];
-                    if constexpr (F::kBn == 128)
-                        valid[lw] = have;
-                    else
-                        reinterpret_cast<unsigned short*>(valid)[lw] = (unsigned short)(have & 0xffffu);
-                }
-                const unsigned dst = smem + F::kOffRaw + raw_in * F::kRaw + lw * (F::kRaw / 4);
-                const long long shift = is_v ? a.kind_rows : 0;
-#pragma unroll 4
-                for (int i = 0; i < kIters; ++i) {
-                    const int rr = i * kStep + lane / kLanes;
-                    const long long at = __shfl_sync(0xffffffffu, mine_row, rr);
-                    const bool ok = at >= 0 && ch < chunks;
-                    cp16(dst + (i * 32 + lane) * 16, ok ? pool + (at + shift) * row_bytes + ch * 16 : pool, ok ? 16u : 0u);
-                }
-                if constexpr (KV == 2) {  // this lane's row scale, straight into its column
-                    const int ring = int((ahead.tile_base + j) % F::kScaleRing);
-                    const unsigned to = smem + F::kOffScale + ((ring * 2 + is_v) * F::kBn + lw * 32 + lane) * 4;
-                    cp4(to, mine_row >= 0 ? a.scales + (mine_row + shift) : a.scales, mine_row >= 0 ? 4u : 0u);
-                }
-                cp_commit();
-                raw_in = raw_in + 1 == F::kRawDepth ? 0 : raw_in + 1;
-            };
-            for (int i = 0; i < F::kRawDepth - 1; ++i) {
-                if (more) issue();
-                if (!more) cp_commit();  // keeps the count of groups
-            }
             for (unsigned piece = 0; go; ++piece) {
                 if (!__all_sync(0xffffffffu, get_piece(piece))) break;
                 const TreePiece& walk = M.piece[piece % kPieceRing];
@@ -1188,9 +1166,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                 for (int e = 0; e < loads && go; ++e) {
                     bool is_v;
                     const int j = walk.entry(e, is_v);
-                    if (more) issue();
-                    if (!more) cp_commit();
-                    cp_wait<F::kRawDepth - 1>();
+                    go = __all_sync(0xffffffffu, bar_wait(&M.raw_full[raw], (raw_phase >> raw) & 1, abort_flag, a.status));
+                    raw_phase ^= 1u << raw;
+                    if (!go) break;
                     const unsigned parity = (empty_phase >> slot) & 1;
                     go = __all_sync(0xffffffffu, bar_wait(&M.empty[slot], parity, abort_flag, a.status));
                     if (!go) break;
@@ -1201,8 +1179,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                     float* scale_col = reinterpret_cast<float*>(tree_smem + F::kOffScale) +
                                        (int((walk.tile_base + j) % F::kScaleRing) * 2 + is_v) * F::kBn;
                     unsigned char* out = tree_smem + slot_at(slot);
-                    const uint4* raw = reinterpret_cast<const uint4*>(tree_smem + F::kOffRaw + raw_out * F::kRaw +
-                                                                      lw * (F::kRaw / 4));
+                    const uint4* src = reinterpret_cast<const uint4*>(tree_smem + F::kOffRaw + raw * F::kRaw + lw * (F::kRaw / 4));
                     float big = 0.f;
                     bool bad = false;
                     unsigned bad_rows = 0;
@@ -1219,7 +1196,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
 #pragma unroll 4
                         for (int i = 0; i < kIters; ++i) {
                             const int rt = lw * 32 + i * kStep + lane / kLanes;
-                            const uint4 v = raw[i * 32 + lane];
+                            const uint4 v = ch < chunks ? src[i * 32 + lane] : make_uint4(0, 0, 0, 0);
                             const unsigned w[4] = {v.x, v.y, v.z, v.w};
                             unsigned h[8];
 #pragma unroll
@@ -1242,10 +1219,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                             }
                         }
                     } else {
-#pragma unroll 2
+#pragma unroll 4
                         for (int i = 0; i < kIters; ++i) {
                             const int rw = i * kStep + lane / kLanes, rt = lw * kRowsPerWarp + rw;
-                            uint4 raw_v = raw[i * 32 + lane];
+                            const uint4 raw_v = ch < chunks ? src[i * 32 + lane] : make_uint4(0, 0, 0, 0);
                             float v[4] = {__uint_as_float(raw_v.x), __uint_as_float(raw_v.y), __uint_as_float(raw_v.z),
                                           __uint_as_float(raw_v.w)};
                             if (is_v && p0 + rt >= walk.len) {
@@ -1281,18 +1258,18 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                         for (int d = 16; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
                         if (lane == 0) M.vmax[meta][lw] = big;
                     }
-                    raw_out = raw_out + 1 == F::kRawDepth ? 0 : raw_out + 1;
                     proxy_fence();
                     __syncwarp();
                     if (lane == 0) {
+                        bar_arrive(&M.raw_empty[raw]);
                         if (is_v) bar_arrive(&M.v_ready[meta]);
                         bar_arrive(&M.full[slot]);
                     }
+                    raw = raw + 1 == F::kRawDepth ? 0 : raw + 1;
                     slot = slot + 1 == F::kBase ? 0 : slot + 1;
                 }
                 if (lane == 0) release_piece(piece);
             }
-            cp_wait<0>();
         }
         if (flags) atomicOr(a.status, flags);
     } else if (warp == kTreeMmaWarp) {
@@ -1392,6 +1369,132 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
         }
         __syncwarp();
     }
+    if (KV != 1 && warp == kTreeRawWarp) {
+        // --------------------------------------- rows of F32 and int8 pools
+        // 32 rows at a time: cached positions of whole boxes by TMA, any
+        // others row by row with bulk copies; rows that hold nothing are zero.
+        constexpr int kSlabs = F::kBn / 32, kPitch = DP * F::kElem;
+        bool go = true;
+        int raw = 0, flags = 0;
+        unsigned empty_phase = 0xffffffffu;
+        for (unsigned piece = 0; go; ++piece) {
+            if (!__all_sync(0xffffffffu, get_piece(piece))) break;
+            const TreePiece& walk = M.piece[piece % kPieceRing];
+            const int loads = 2 * (walk.t1 - walk.t0);
+            long long cur[kSlabs], prev[kSlabs];
+            long long box_cur = 0, box_prev = 0;
+            int k_last = -1, ahead = 0, ahead_j = -1;  // ahead: the table entry of this lane's box in tile ahead_j
+            int k_box = -1;
+            const int boxes = a.box_rows ? F::kBn / a.box_rows : 0;
+            const auto entry_of = [&](int j) -> int {
+                const int p = (walk.t0 + j) * F::kBn + lane * a.box_rows;
+                return a.tables[(long long)walk.s * a.stride + div_bt(a, p)];
+            };
+#pragma unroll
+            for (int i = 0; i < kSlabs; ++i) cur[i] = prev[i] = -1;
+#pragma unroll 1
+            for (int e = 0; e < loads; ++e) {
+                bool is_v;
+                const int j = walk.entry(e, is_v);
+                const unsigned tile = walk.tile_base + j;
+                if (boxes && (walk.t0 + j + 1) * F::kBn <= walk.len) {
+                    if (!is_v) {
+                        box_prev = box_cur;
+                        box_cur = -1;
+                        if (lane < boxes) {
+                            const int block = ahead_j == j ? ahead : entry_of(j);
+                            const int p = (walk.t0 + j) * F::kBn + lane * a.box_rows;
+                            if (unsigned(block) < unsigned(a.max_blocks))
+                                box_cur = block * a.block_rows + a.layer_rows + (long long)walk.head * a.bt + (p - int(div_bt(a, p)) * a.bt);
+                            ahead_j = j + 1;
+                            if ((walk.t0 + j + 2) * F::kBn <= walk.len && walk.t0 + j + 1 < walk.t1) ahead = entry_of(j + 1);
+                            else ahead_j = -1;
+                        }
+                    }
+                    const long long at = is_v && j != k_box ? box_prev : box_cur;
+                    if (!is_v) k_box = j;
+                    if (__all_sync(0xffffffffu, lane >= boxes || at >= 0)) {
+                        go = __all_sync(0xffffffffu, bar_wait(&M.raw_empty[raw], (empty_phase >> raw) & 1, abort_flag, a.status));
+                        if (!go) break;
+                        empty_phase ^= 1u << raw;
+                        if (!is_v && lane < 4) M.valid[tile % kMetaRing][lane] = 0xffffffffu;
+                        const unsigned full = sm_addr(&M.raw_full[raw]);
+                        if (lane == 0)
+                            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full),
+                                         "r"(F::kBn * (DP * F::kElem + (KV == 2 ? 4 : 0)))
+                                         : "memory");
+                        __syncwarp();
+                        if (lane < boxes) {
+                            const long long row = at + (is_v ? a.kind_rows : 0);
+                            tma_load_2d(smem + F::kOffRaw + raw * F::kRaw + lane * a.box_rows * kPitch, &kv_map, 0, int(row), full);
+                            if constexpr (KV == 2)
+                                bulk_load(smem + F::kOffScale + ((tile % F::kScaleRing * 2 + is_v) * F::kBn + lane * a.box_rows) * 4,
+                                          a.scales + row, a.box_rows * 4, full);
+                        }
+                        if constexpr (KV == 2) bar_arrive(&M.raw_full[raw]);
+                        raw = raw + 1 == F::kRawDepth ? 0 : raw + 1;
+                        continue;
+                    }
+                }
+                if (j != k_last && (!is_v || j != k_last - 1)) {
+#pragma unroll
+                    for (int i = 0; i < kSlabs; ++i) {
+                        prev[i] = cur[i];
+                        cur[i] = row_of(walk, (walk.t0 + j) * F::kBn + 32 * i + lane, flags);
+                    }
+                    k_last = j;
+                }
+                go = __all_sync(0xffffffffu, bar_wait(&M.raw_empty[raw], (empty_phase >> raw) & 1, abort_flag, a.status));
+                if (!go) break;
+                empty_phase ^= 1u << raw;
+                const unsigned dst = F::kOffRaw + raw * F::kRaw;
+                int bytes = 0;
+#pragma unroll
+                for (int i = 0; i < kSlabs; ++i) {
+                    const long long at = j == k_last ? cur[i] : prev[i];
+                    const unsigned have = __ballot_sync(0xffffffffu, at >= 0);
+                    if (!is_v && lane == 0) M.valid[tile % kMetaRing][i] = have;
+                    if (at < 0)
+                        for (int k = 0; k < chunks; ++k)
+                            *reinterpret_cast<uint4*>(tree_smem + dst + (32 * i + lane) * kPitch + 16 * k) = make_uint4(0, 0, 0, 0);
+                    bytes += __popc(have) * row_bytes;
+                }
+                __syncwarp();
+                const unsigned full = sm_addr(&M.raw_full[raw]);
+                if (lane == 0)
+                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full), "r"(bytes) : "memory");
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < kSlabs; ++i) {
+                    const long long at = j == k_last ? cur[i] : prev[i], row = at + (is_v ? a.kind_rows : 0);
+                    const unsigned to = smem + dst + (32 * i + lane) * kPitch;
+                    const bool slab = a.box_rows && __all_sync(0xffffffffu, at >= 0) &&
+                                      (walk.t0 + j) * F::kBn + 32 * i + 32 <= walk.len;
+                    if (slab) {
+                        if ((lane & (a.box_rows - 1)) == 0) tma_load_2d(to, &kv_map, 0, int(row), full);
+                    } else if (at >= 0) {
+                        bulk_load(to, pool + row * row_bytes, row_bytes, full);
+                    }
+                    if constexpr (KV == 2)  // the row's scale, straight into its column
+                        cp4(smem + F::kOffScale + ((tile % F::kScaleRing * 2 + is_v) * F::kBn + 32 * i + lane) * 4,
+                            at >= 0 ? a.scales + row : a.scales, at >= 0 ? 4u : 0u);
+                }
+                if constexpr (KV == 2)
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full) : "memory");
+                __syncwarp();
+                raw = raw + 1 == F::kRawDepth ? 0 : raw + 1;
+            }
+            if (lane == 0 && go) release_piece(piece);
+        }
+        // every copy of this warp has landed before the memory is given back
+#pragma unroll 1
+        for (int i = 0; i < F::kRawDepth; ++i)
+#pragma unroll 1
+            for (unsigned k = 0; k < kTreeSpin && !bar_test(&M.raw_full[i], empty_phase >> i & 1); ++k) {
+            }
+        if (KV == 2) cp_wait<0>();
+        if (flags) atomicOr(a.status, flags);
+    }
     tm_before();
     __syncthreads();
     if (warp == kTreeMmaWarp) {
@@ -1452,19 +1555,20 @@ void run_tree_mma(const TreeAttn& a, void* workspace, cudaStream_t s) {
     auto* recs = static_cast<TreeRec*>(workspace);
     auto* partial = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + 4096);
     TVARA_CUDA(cudaFuncSetAttribute(tree_mma_kernel<KV, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem));
-    // F16 pools of whole 128-byte row halves and blocks of a multiple of 8
-    // positions: cached positions come by TMA, whose boxes never cross a block
+    // head_dim 64 or 128 and blocks of a multiple of 8 positions: cached
+    // positions come by TMA, whose boxes never cross a block
     CUtensorMap map{};
     TreeAttn job = a;
     job.box_rows = 0;
     const unsigned long long rows = (unsigned long long)a.max_blocks * a.block_rows;
-    if (KV == 1 && a.dim % 64 == 0 && a.bt % 8 == 0 && rows < 0x7fffffffull) {
+    if (a.dim % 64 == 0 && a.bt % 8 == 0 && rows < 0x7fffffffull && reinterpret_cast<std::uintptr_t>(a.scales) % 16 == 0) {
         job.box_rows = a.bt % 32 == 0 ? 32 : a.bt % 16 == 0 ? 16 : 8;
         const cuuint64_t dims[2] = {cuuint64_t(a.dim), cuuint64_t(rows)};
-        const cuuint64_t strides[1] = {cuuint64_t(a.dim) * 2};
-        const cuuint32_t box[2] = {64, cuuint32_t(job.box_rows)}, ones[2] = {1, 1};
-        if (tensor_map_encoder()(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(a.kv), dims, strides, box, ones,
-                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+        const cuuint64_t strides[1] = {cuuint64_t(a.dim) * F::kElem};
+        const cuuint32_t box[2] = {cuuint32_t(KV == 1 ? 64 : a.dim), cuuint32_t(job.box_rows)}, ones[2] = {1, 1};
+        const auto type = KV == 0 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : KV == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+        if (tensor_map_encoder()(&map, type, 2, const_cast<void*>(a.kv), dims, strides, box, ones,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, KV == 1 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
             throw std::runtime_error("cuTensorMapEncodeTiled failed for the KV pool");
     }
