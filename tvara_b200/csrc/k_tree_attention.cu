@@ -263,7 +263,7 @@ struct TreeMeta {  // at kOffMeta
     union {
         unsigned vbad[kMetaRing][4];  // nodes whose V (kept out of the products: 0 * inf) is not finite
         struct {                      // while the run is cut out
-            long long total, excl0, excl1;
+            long long excl0, excl1;
             int seq0, seq1, bad;
         };
     };
@@ -514,62 +514,66 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
         bar_init(&M.drain, 1);
         M.abort_flag = 0;
         M.bad = 0;
-        M.total = 0;
         M.seq0 = M.seq1 = a.n_seq;
         M.excl0 = M.excl1 = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
-    // The run of tiles: weights are scanned in sequence order by every CTA.
-    const auto weight_of = [&](int s) -> long long {
-        TreeSeq q;
-        if (s >= a.n_seq) return 0;
-        if (!tree_seq<F>(a, s, q)) M.bad = 1;
-        return q.total ? q.total * q.weight + (long long)q.groups * a.hkv * F::kItemWeight : 0;
-    };
-    long long mine = 0;
-#pragma unroll 1
-    for (int s = tid; s < a.n_seq; s += kTreeThreads) mine += weight_of(s);
-    if (mine) atomicAdd(reinterpret_cast<unsigned long long*>(&M.total), (unsigned long long)mine);
-    __syncthreads();
-    const long long total = M.total;
-    if (blockIdx.x == 0 && tid == 0 && M.bad) atomicOr(a.status, kTreeBadLengths);
-    const int ctas = int(max(1ll, min((long long)gridDim.x, total / min_weight)));
+    // The run of tiles: weights are scanned in sequence order by every CTA
+    // (twice if they are more than the threads: for the sum, then for the cuts).
     const int cta = blockIdx.x;
+    long long total = 0, w0 = 0, w1 = 0;
+    int ctas = 1;
+    const bool once = a.n_seq <= kTreeThreads;
+#pragma unroll 1
+    for (int pass = once ? 1 : 0; pass < 2; ++pass) {
+        long long carry = 0;
+#pragma unroll 1
+        for (int base = 0; base < a.n_seq; base += kTreeThreads) {
+            TreeSeq q;
+            q.total = 0;
+            if (base + tid < a.n_seq && !tree_seq<F>(a, base + tid, q)) M.bad = 1;
+            const long long w = q.total ? q.total * q.weight + (long long)q.groups * a.hkv * F::kItemWeight : 0;
+            long long scan = w;
+#pragma unroll 1
+            for (int d = 1; d < 32; d <<= 1) {
+                const long long up = __shfl_up_sync(0xffffffffu, scan, d);
+                if (lane >= d) scan += up;
+            }
+            if (lane == 31) M.warp_sum[warp] = scan;
+            __syncthreads();
+            long long before = carry, all = 0;
+#pragma unroll 4
+            for (int i = 0; i < kTreeThreads / 32; ++i) {
+                const long long x = M.warp_sum[i];
+                before += i < warp ? x : 0;
+                all += x;
+            }
+            carry += all;
+            if (once) total = carry;
+            if (pass) {
+                if (once || base == 0) {
+                    ctas = int(max(1ll, min((long long)gridDim.x, total / min_weight)));
+                    w0 = total * cta / ctas;
+                    w1 = total * (cta + 1) / ctas;
+                }
+                const long long excl = before + scan - w;
+                if (w && excl <= w0 && w0 < excl + w) {
+                    M.seq0 = base + tid;
+                    M.excl0 = excl;
+                }
+                if (w && excl < w1 && w1 <= excl + w) {
+                    M.seq1 = base + tid;
+                    M.excl1 = excl;
+                }
+            }
+            __syncthreads();
+        }
+        total = carry;
+    }
+    if (cta == 0 && tid == 0 && M.bad) atomicOr(a.status, kTreeBadLengths);
     if (tid == 0) recs[cta].pieces = 0;
     if (cta >= ctas || total == 0) return;
-    const long long w0 = total * cta / ctas, w1 = total * (cta + 1) / ctas;
-    long long carry = 0;
-#pragma unroll 1
-    for (int base = 0; base < a.n_seq; base += kTreeThreads) {
-        const long long w = weight_of(base + tid);
-        long long scan = w;
-#pragma unroll 1
-        for (int d = 1; d < 32; d <<= 1) {
-            const long long up = __shfl_up_sync(0xffffffffu, scan, d);
-            if (lane >= d) scan += up;
-        }
-        if (lane == 31) M.warp_sum[warp] = scan;
-        __syncthreads();
-        long long before = carry, all = 0;
-#pragma unroll 1
-        for (int i = 0; i < kTreeThreads / 32; ++i) {
-            if (i < warp) before += M.warp_sum[i];
-            all += M.warp_sum[i];
-        }
-        const long long excl = before + scan - w;
-        if (w && excl <= w0 && w0 < excl + w) {
-            M.seq0 = base + tid;
-            M.excl0 = excl;
-        }
-        if (w && excl < w1 && w1 <= excl + w) {
-            M.seq1 = base + tid;
-            M.excl1 = excl;
-        }
-        carry += all;
-        __syncthreads();
-        if (carry >= w1) break;
-    }
     if (warp == kTreeMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sm_addr(&M.tmem)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -578,6 +582,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
     __syncthreads();
     tm_after();
     const unsigned tmem = M.tmem;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     volatile int* abort_flag = &M.abort_flag;
     if (warp >= kTreeMmaWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
     if (warp == kTreePieceWarp) {
@@ -696,9 +701,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
             const int first_node = unsigned(first_row + wq * 32) / unsigned(group);  // of the warp's vectors
             const int first_g = first_row + wq * 32 - first_node * group;
             const bool live = r < tile_rows, warp_live = wq * 32 < tile_rows;
-            // The warp's query vectors, one at a time across its lanes: scaled
-            // below 2^15, split, into this stream's Q tile; lane i keeps the
-            // score factor of vector i.
+            // The warp's query vectors, scaled below 2^15 and split, into this
+            // stream's Q tile; lane i keeps the score factor of vector i.
             float c = 0.f;
             if (warp_live) {
                 // raw rows first, all in flight, each in the 512 (256) bytes its two halves will take
@@ -709,10 +713,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                 const float* src = a.q + (long long)(q.c0 + first_node) * a.ldq + (long long)(q.head * group + g) * a.dim + lane * 4;
                 const long long turn = a.ldq - (long long)(group - 1) * a.dim;  // to the next node's first head
                 if (writes) {
-                    const unsigned to = sm_addr(tile) + (lane >> 3) * 16384 + ((lane & 7) << 4);
+                    const unsigned to = sm_addr(tile) + (lane >> 3) * 16384;
 #pragma unroll 1
                     for (int i = 0; i < most; ++i) {
-                        if (lane < DP / 4) cp16(to + i * 128, lane < quads ? src : a.q, lane < quads ? 16u : 0u);
+                        if (lane < DP / 4)
+                            cp16(to + i * 128 + (((lane & 7) ^ (i & 7)) << 4), lane < quads ? src : a.q, lane < quads ? 16u : 0u);
                         const bool last = g + 1 == group;
                         src += last ? turn : a.dim;
                         g = last ? 0 : g + 1;
@@ -720,24 +725,31 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                     cp_commit();
                     cp_wait<0>();
                     __syncwarp();
-#pragma unroll 4
-                    for (int i = 0; i < most; ++i) {
-                        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (lane < DP / 4) x = *reinterpret_cast<const float4*>(tile + (lane >> 3) * 16384 + i * 128 + ((lane & 7) << 4));
-                        float top = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
-                        top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-                        const int up = lift(top);
-                        if (lane == i) c = score_unit * two_to(-up);
-                        const float f = two_to(up);
-                        uint2 hi, lo;
-                        split_exact(x.x * f, x.y * f, hi.x, lo.x);
-                        split_exact(x.z * f, x.w * f, hi.y, lo.y);
-                        __syncwarp();  // the row is read
-                        const int ch = lane >> 1, at = (ch >> 3) * 16384 + i * 128 + (((ch & 7) ^ (i & 7)) << 4) + (lane & 1) * 8;
-                        if (lane < DP / 4) {
-                            *reinterpret_cast<uint2*>(tile + at) = hi;
-                            *reinterpret_cast<uint2*>(tile + F::kQPart + at) = lo;
-                        }
+                    // then lane i takes row i (the accumulators' registers are free yet)
+                    unsigned char* mine = tile + lane * 128;
+                    float tops[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int i = 0; i < DP / 4; ++i) {
+                        const float4 x = *reinterpret_cast<const float4*>(mine + (i >> 3) * 16384 + (((i & 7) ^ (lane & 7)) << 4));
+                        o[4 * i] = x.x;
+                        o[4 * i + 1] = x.y;
+                        o[4 * i + 2] = x.z;
+                        o[4 * i + 3] = x.w;
+                        tops[i & 3] = max3(tops[i & 3], fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+                    }
+                    const int up = lift(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
+                    c = live ? score_unit * two_to(-up) : 0.f;
+                    const float f = two_to(up);
+#pragma unroll
+                    for (int i = 0; i < DP / 8; ++i) {
+                        uint4 hi, lo;
+                        split_exact(o[8 * i] * f, o[8 * i + 1] * f, hi.x, lo.x);
+                        split_exact(o[8 * i + 2] * f, o[8 * i + 3] * f, hi.y, lo.y);
+                        split_exact(o[8 * i + 4] * f, o[8 * i + 5] * f, hi.z, lo.z);
+                        split_exact(o[8 * i + 6] * f, o[8 * i + 7] * f, hi.w, lo.w);
+                        unsigned char* at = mine + (i >> 3) * 16384 + (((i & 7) ^ (lane & 7)) << 4);
+                        *reinterpret_cast<uint4*>(at) = hi;
+                        *reinterpret_cast<uint4*>(at + F::kQPart) = lo;
                     }
                     if (!q.pair) {  // for the other stream, in its idle tensor memory
                         asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(lane_base + 384),
@@ -1508,6 +1520,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
 // Block (b, y) takes rows 8 y .. 8 y + 7 of the item that starts in CTA b.
 template <int DP>
 __global__ void __launch_bounds__(256) tree_combine_kernel(TreeAttn a, const float* partial, const TreeRec* recs) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the tiles are still being worked on
     const TreeRec rec = recs[blockIdx.x];
     const int row = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (rec.pieces < 2 || row >= rec.rows) return;
@@ -1516,22 +1529,29 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(TreeAttn a, const flo
     const long long slot_floats = (long long)kTreeRows * (DP + 2);
     const auto slot_of = [&](int i) { return partial + (2ll * (blockIdx.x + i) + (i == 0)) * slot_floats; };
     float top = -INFINITY;
-#pragma unroll 1
-    for (int i = 0; i < rec.pieces; ++i) top = fmaxf(top, slot_of(i)[kTreeRows * DP + pr]);
-    float l = 0.f, o[kPer] = {};
-    if (top != -INFINITY) {
-#pragma unroll 2
-        for (int i = 0; i < rec.pieces; ++i) {
-            const float* slot = slot_of(i);
-            const float f = ex2(slot[kTreeRows * DP + pr] - top);
-            l += slot[kTreeRows * DP + kTreeRows + pr] * f;
+    for (int i = lane; i < rec.pieces; i += 32) top = fmaxf(top, slot_of(i)[kTreeRows * DP + pr]);
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) o[e] += slot[pr * DP + e * 32 + lane] * f;
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    float l = 0.f, o[kPer] = {};
+    for (int base = 0; base < rec.pieces; base += 32) {
+        float f = 0.f;
+        if (base + lane < rec.pieces) {
+            const float* slot = slot_of(base + lane);
+            // nothing seen (or nothing but NaN scores): the sums decide
+            f = top == -INFINITY ? 1.f : ex2(slot[kTreeRows * DP + pr] - top);
+            l += slot[kTreeRows * DP + kTreeRows + pr] * f;
         }
-    } else {  // nothing seen, or nothing but NaN scores
-#pragma unroll 1
-        for (int i = 0; i < rec.pieces; ++i) l += slot_of(i)[kTreeRows * DP + kTreeRows + pr];
+        const int here = min(32, rec.pieces - base);
+#pragma unroll 4
+        for (int i = 0; i < here; ++i) {
+            const float fi = __shfl_sync(0xffffffffu, f, i);
+            const float* slot = slot_of(base + i);
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) o[e] += slot[pr * DP + e * 32 + lane] * fi;
+        }
     }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
     const int vec = rec.row0 + row, node = unsigned(vec) / unsigned(group), head = rec.head * group + vec - node * group;
     float* dst = a.out + (long long)(rec.c0 + node) * a.ldo + (long long)head * a.dim;
 #pragma unroll
@@ -1574,7 +1594,21 @@ void run_tree_mma(const TreeAttn& a, void* workspace, cudaStream_t s) {
     }
     tree_mma_kernel<KV, DP><<<ctas, kTreeThreads, F::kSmem, s>>>(map, job, partial, recs, 2);
     TVARA_LAUNCHED();
-    tree_combine_kernel<DP><<<dim3(unsigned(ctas), kTreeRows / 8), 256, 0, s>>>(a, partial, recs);
+    // launched early (its blocks wait for the first kernel's end), and with the
+    // same shared-memory split, so that the SMs need not be drained between
+    TVARA_CUDA(cudaFuncSetAttribute(tree_combine_kernel<DP>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                    cudaSharedmemCarveoutMaxShared));
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(unsigned(ctas), kTreeRows / 8);
+    config.blockDim = dim3(256);
+    config.stream = s;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    TVARA_CUDA(cudaLaunchKernelEx(&config, tree_combine_kernel<DP>, a, static_cast<const float*>(partial),
+                                  static_cast<const TreeRec*>(recs)));
     TVARA_LAUNCHED();
 }
 
