@@ -249,11 +249,10 @@ struct TreePiece {
 
 struct TreeMeta {  // at kOffMeta
     std::uint64_t full[8], empty[8];
-    std::uint64_t s_full[2], p_full[2], o_full[2];
     std::uint64_t v_ready[kMetaRing];  // a tile's V scales and vbad are in place
+    std::uint64_t raw_full[4], raw_empty[4], piece_full[kPieceRing], piece_empty[kPieceRing];
+    std::uint64_t s_full[2], p_full[2], o_full[2];
     std::uint64_t q_full, merge_ready, merge_read, drain;
-    std::uint64_t piece_full[kPieceRing], piece_empty[kPieceRing];
-    std::uint64_t raw_full[4], raw_empty[4];
     union {
         TreePiece piece[kPieceRing];
         long long warp_sum[16];  // while the run is cut out
@@ -270,10 +269,13 @@ struct TreeMeta {  // at kOffMeta
     unsigned tmem;
     int abort_flag;
 };
+constexpr int kTreeBars = 50;
+static_assert(kMetaRing == 8 && kPieceRing == 4 && offsetof(TreeMeta, drain) == (kTreeBars - 1) * 8);
 static_assert(sizeof(TreeMeta) <= kTreeMetaBytes);
 
 struct TreeRec {  // an item that continues in the next CTAs, by the CTA it starts in
     int c0, row0, rows, split, head, pieces;
+    int streams;  // slot halves that hold parts of the same vectors (1: of different ones)
 };
 
 __device__ __forceinline__ unsigned sm_addr(const void* p) { return unsigned(__cvta_generic_to_shared(p)); }
@@ -429,6 +431,11 @@ __device__ __forceinline__ void split_weight(f32x2 p, unsigned& hi, unsigned& lo
     lo = half2_of(fma2(h, pair_of(-1.f, -1.f), p));
 }
 
+// Quotients of non-negative numbers, mostly below 2^32.
+__device__ __forceinline__ long long quotient(long long x, long long y) {
+    return (x | y) >> 32 ? x / y : (long long)(unsigned(x) / unsigned(y));
+}
+
 // What every role knows of a sequence, and its tiles in the global order
 // (KV heads outermost, then groups of query vectors, then tiles).
 struct TreeSeq {
@@ -487,36 +494,27 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int group = a.group;
 
-    if (tid == 0) {
-#pragma unroll 1
-        for (int i = 0; i < 8; ++i) {
-            bar_init(&M.full[i], 4);
-            bar_init(&M.empty[i], 1);
-        }
-#pragma unroll 1
-        for (int i = 0; i < kMetaRing; ++i) bar_init(&M.v_ready[i], 4);
-#pragma unroll 1
-        for (int i = 0; i < 2; ++i) {
-            bar_init(&M.s_full[i], 1);
-            bar_init(&M.p_full[i], 4);
-            bar_init(&M.o_full[i], 1);
-        }
-#pragma unroll 1
-        for (int i = 0; i < kPieceRing; ++i) {
-            bar_init(&M.piece_full[i], 1);
-            bar_init(&M.piece_empty[i], KV == 1 ? 13 : 14);  // 8 softmax warps, 4 load warps, MMA, row fetch
-            bar_init(&M.raw_full[i], KV == 2 ? 33 : 1);
-            bar_init(&M.raw_empty[i], 4);
-        }
-        bar_init(&M.q_full, 8);
-        bar_init(&M.merge_ready, 4);
-        bar_init(&M.merge_read, 4);
-        bar_init(&M.drain, 1);
+    if (tid < kTreeBars) {  // TreeMeta begins with its barriers
+        const int i = tid;
+        bar_init(&M.full[0] + i, i < 8    ? 4                   // full: load warps
+                                 : i < 16 ? 1                   // empty: MMA commits
+                                 : i < 24 ? 4                   // v_ready: load warps
+                                 : i < 32 ? (i & 4 ? 4 : KV == 2 ? 33 : 1)  // raw_full, raw_empty
+                                 : i < 40 ? (i & 4 ? (KV == 1 ? 13 : 14) : 1)  // piece_full, piece_empty: 8 softmax
+                                                                               // warps, 4 load warps, MMA, row fetch
+                                 : i < 42 ? 1                   // s_full
+                                 : i < 44 ? 4                   // p_full
+                                 : i < 46 ? 1                   // o_full
+                                 : i < 47 ? 8                   // q_full
+                                 : i < 49 ? 4                   // merge_ready, merge_read
+                                          : 1);                 // drain
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (tid == 64) {
         M.abort_flag = 0;
         M.bad = 0;
         M.seq0 = M.seq1 = a.n_seq;
         M.excl0 = M.excl1 = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
     // The run of tiles: weights are scanned in sequence order by every CTA
@@ -553,9 +551,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
             if (once) total = carry;
             if (pass) {
                 if (once || base == 0) {
-                    ctas = int(max(1ll, min((long long)gridDim.x, total / min_weight)));
-                    w0 = total * cta / ctas;
-                    w1 = total * (cta + 1) / ctas;
+                    ctas = int(max(1ll, min((long long)gridDim.x, quotient(total, min_weight))));
+                    w0 = quotient(total * cta, ctas);
+                    w1 = quotient(total * (cta + 1), ctas);
                 }
                 const long long excl = before + scan - w;
                 if (w && excl <= w0 && w0 < excl + w) {
@@ -596,8 +594,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
             // on, its tile t starts at t weight of them; a tile belongs to the
             // CTA whose run holds its start.
             const auto tile_at = [&](long long w) {
-                const long long each = q.tiles * q.weight + F::kItemWeight, i = w / each;
-                return i * q.tiles + min(q.tiles, (w - i * each + q.weight - 1) / q.weight);
+                const long long each = q.tiles * q.weight + F::kItemWeight, i = quotient(w, each), left = w - i * each;
+                return i * q.tiles + min(q.tiles, q.weight == 2 ? (left + 1) >> 1 : left);
             };
             const long long u1 = min(q.total, tile_at(w1 - excl1));
             tree_seq<F>(a, seq0, q);
@@ -622,12 +620,12 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                     bar_arrive(&M.piece_full[ring]);
                     break;
                 }
-                const long long item = u / q.tiles;
+                const long long item = quotient(u, q.tiles);
                 const int t0 = int(u - item * q.tiles), t1 = int(min(q.tiles, t0 + (end - u)));
                 u += t1 - t0;
-                const int head = int(item / q.groups), grp = int(item - (long long)head * q.groups);
+                const int head = int(unsigned(item) / unsigned(q.groups)), grp = int(item - (long long)head * q.groups);
                 // groups of nearly equal size, and M tiles of nearly equal size
-                const int vectors = q.n * group, per = (vectors + q.groups - 1) / q.groups;
+                const int vectors = q.n * group, per = unsigned(vectors + q.groups - 1) / unsigned(q.groups);
                 const int row0 = grp * per, rows = min(per, vectors - row0);
                 p.s = seq;
                 p.c0 = q.c0;
@@ -653,7 +651,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                     rec.rows = rows;
                     rec.split = p.split;
                     rec.head = head;
-                    rec.pieces = int(((last + 1) * ctas + total - 1) / total - 1) - cta + 1;
+                    rec.pieces = int(quotient((last + 1) * ctas + total - 1, total) - 1) - cta + 1;
+                    rec.streams = q.pair ? 1 : 2;
                     recs[cta] = rec;
                 }
             }
@@ -781,8 +780,6 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
             for (int j = q.pair ? 0 : stream; j < tiles && go; j += q.pair ? 1 : 2, ++n_s) {
                 const unsigned t = q.tile_base + j;
                 go = bar_wait(&M.s_full[stream], n_s & 1, abort_flag, a.status);
-                if (KV != 1 || (q.t0 + j + 1) * F::kBn > q.len)  // scales of V, nodes with a non-finite V
-                    go = go && bar_wait(&M.v_ready[t % kMetaRing], (t / kMetaRing) & 1, abort_flag, a.status);
                 go = __all_sync(0xffffffffu, go);
                 if (!go) break;
                 tm_after();
@@ -821,10 +818,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                         }
                         if (!all) {
                             unsigned see = M.valid[ring][k];
-                            if (nodes) {
-                                see &= node_bits(a, q.c0, q.n, live ? node : 0, p0 + 32 * k - q.len);
-                                if (see & M.vbad[ring][k]) l = NAN;  // the row's result is not finite
-                            }
+                            if (nodes) see &= node_bits(a, q.c0, q.n, live ? node : 0, p0 + 32 * k - q.len);
 #pragma unroll
                             for (int i = 0; i < F::kBn / 32; ++i) seen[i] = k == i ? see : seen[i];
 #pragma unroll
@@ -841,6 +835,15 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                     keep = mn == -INFINITY ? 1.f : ex2(m - mn);
                     m = mn;
                     l *= keep;
+                    if (KV != 1 || nodes) {  // scales of V, nodes with a non-finite V
+                        go = __all_sync(0xffffffffu, bar_wait(&M.v_ready[t % kMetaRing], (t / kMetaRing) & 1, abort_flag, a.status));
+                        if (!go) break;
+                        if (nodes) {
+#pragma unroll
+                            for (int k = 0; k < F::kBn / 32; ++k)
+                                if (seen[k] & M.vbad[ring][k]) l = NAN;  // the row's result is not finite
+                        }
+                    }
                     float v_unit = 1.f;
                     if constexpr (KV != 1) {
                         const float4 big4 = *reinterpret_cast<const float4*>(M.vmax[ring]);
@@ -924,11 +927,28 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
 #pragma unroll
                 for (int i = 0; i < DP; ++i) o[i] *= vref;
             }
+            // The part of an item that other CTAs continue: (O, m, l) of each
+            // stream into the workspace, one thread a row, rows side by side.
+            // The CTA's slot 1 holds an item that begins here, slot 0 one that
+            // began earlier; stream 1 uses the upper half of a slot.
+            if (!q.whole && live) {
+                float* slot = partial + (long long)(2 * cta + (q.t0 == 0)) * kTreeRows * (DP + 2);
+                const int pr = stream * 128 + r;
+#pragma unroll
+                for (int i = 0; i < DP / 4; ++i)
+                    *reinterpret_cast<float4*>(slot + (i * kTreeRows + pr) * 4) =
+                        make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                slot[kTreeRows * DP + pr] = m;
+                slot[kTreeRows * DP + kTreeRows + pr] = l;
+            }
             if (!q.pair) {
-                // the odd tiles' (O, m, l) through stream 1's tensor memory
+                // A whole item: the odd tiles' (O, m, l) through stream 1's tensor
+                // memory.  Either way each stream learns that the other is done
+                // with the shared Q tile.
+                const bool merge = q.whole && warp_live && tiles > 1;
                 const unsigned b_o = lane_base + 256 + 128, b_ml = lane_base + 128;
                 if (stream) {
-                    if (warp_live && tiles > 1) {
+                    if (merge) {
 #pragma unroll
                         for (int k = 0; k < DP / 16; ++k) {
                             unsigned x[16];
@@ -948,7 +968,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                 } else {
                     go = __all_sync(0xffffffffu, bar_wait(&M.merge_ready, q.count & 1, abort_flag, a.status));
                     tm_after();
-                    if (go && warp_live && tiles > 1) {
+                    if (go && merge) {
                         unsigned ml[16];
                         tm_ld16(b_ml, ml);
                         const float m2 = __uint_as_float(ml[0]), l2 = __uint_as_float(ml[1]);
@@ -956,13 +976,16 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                         const float ka = mn == -INFINITY ? 0.f : ex2(m - mn), kb = mn == -INFINITY ? 0.f : ex2(m2 - mn);
                         m = mn;
                         l = l * ka + l2 * kb;
+                        const f32x2 ka2 = pair_of(ka, ka), kb2 = pair_of(kb, kb);
 #pragma unroll
                         for (int k = 0; k < DP / 32; ++k) {
                             unsigned x[32];
                             tm_ld32(b_o + 32 * k, x);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                o[32 * k + i] = fmaf(o[32 * k + i], ka, __uint_as_float(x[i]) * kb);
+                            for (int i = 0; i < 32; i += 2)
+                                halves_of(fma2(pair_of(o[32 * k + i], o[32 * k + i + 1]), ka2,
+                                               mul2(pair_of(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), kb2)),
+                                          o[32 * k + i], o[32 * k + i + 1]);
                         }
                     }
                     tm_before();
@@ -974,41 +997,28 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                 if (lane == 0) bar_arrive(stream ? &M.merge_ready : &M.merge_read);
             }
             if (!go) break;
-            if (warp_live && (q.pair || stream == 0)) {
+            if (q.whole && warp_live && (q.pair || stream == 0)) {
                 // Rows through the Q tile, whose MMAs are done (the places of this
                 // warp's own vectors), so that each is written by a whole warp.
                 unsigned char* tile = tree_smem + (q.pair && stream ? F::kQTile : 0) + wq * 4096;
                 const auto stage = [&](int row, int ch) {
                     return reinterpret_cast<float4*>(tile + (ch >> 3) * 16384 + row * 128 + (((ch & 7) ^ (row & 7)) << 4));
                 };
-                float f = 1.f;
-                if (q.whole) f = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
+                const float f = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
                 for (int i = 0; i < DP / 4; ++i)  // lane is the row
                     *stage(lane, i) = make_float4(o[4 * i] * f, o[4 * i + 1] * f, o[4 * i + 2] * f, o[4 * i + 3] * f);
-                // the CTA's slot 1 holds an item that begins here, slot 0 one that began earlier
-                float* part = partial + (long long)(2 * cta + (q.t0 == 0)) * kTreeRows * (DP + 2);
-                const int pr = stream * 128 + r;
-                if (!q.whole && live) {
-                    part[kTreeRows * DP + pr] = m;
-                    part[kTreeRows * DP + kTreeRows + pr] = l;
-                }
                 __syncwarp();
-                const int most = min(32, tile_rows - wq * 32);
-                {
-                    const int width = q.whole ? a.dim >> 2 : DP / 4;
-                    int g = q.whole ? first_g : 0;
-                    float* dst = q.whole ? a.out + (long long)(q.c0 + first_node) * a.ldo + (long long)(q.head * group + g) * a.dim
-                                         : part + (stream * 128 + wq * 32) * DP;
-                    const int heads = q.whole ? group : 1;
-                    const long long step = q.whole ? a.dim : DP, turn = q.whole ? a.ldo - (long long)(group - 1) * a.dim : DP;
-#pragma unroll 2
-                    for (int i = 0; i < most; ++i) {
-                        if (lane < width) reinterpret_cast<float4*>(dst)[lane] = *stage(i, lane);
-                        const bool last = g + 1 == heads;
-                        dst += last ? turn : step;
-                        g = last ? 0 : g + 1;
-                    }
+                const int most = min(32, tile_rows - wq * 32), width = a.dim >> 2;
+                int g = first_g;
+                float* dst = a.out + (long long)(q.c0 + first_node) * a.ldo + (long long)(q.head * group + g) * a.dim + lane * 4;
+                const long long turn = a.ldo - (long long)(group - 1) * a.dim;
+#pragma unroll 4
+                for (int i = 0; i < most; ++i) {
+                    if (lane < width) *reinterpret_cast<float4*>(dst) = *stage(i, lane);
+                    const bool last = g + 1 == group;
+                    dst += last ? turn : a.dim;
+                    g = last ? 0 : g + 1;
                 }
             }
             proxy_fence();  // the Q tile's next readers and writers
@@ -1170,7 +1180,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
             unsigned raw_phase = 0;
             constexpr int kLanes = DP * F::kElem / 16, kStep = 32 / kLanes;  // lanes per row, rows per instruction
             constexpr int kIters = kRowsPerWarp / kStep;
-            const int ch = lane % kLanes;
+            const int ch = lane % kLanes, row_in = lane / kLanes;
+            static_assert(kStep <= 8 && kIters % 4 == 0);
             for (unsigned piece = 0; go; ++piece) {
                 if (!__all_sync(0xffffffffu, get_piece(piece))) break;
                 const TreePiece& walk = M.piece[piece % kPieceRing];
@@ -1187,27 +1198,25 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                     empty_phase ^= 1u << slot;
                     const int meta = int((walk.tile_base + j) % kMetaRing);
                     const int p0 = (walk.t0 + j) * F::kBn;
-                    const bool node_row = p0 + lw * kRowsPerWarp + (lane % kRowsPerWarp) >= walk.len;
+                    const bool node_values = is_v && p0 + F::kBn > walk.len;  // V of nodes may be masked: finite in the products
                     float* scale_col = reinterpret_cast<float*>(tree_smem + F::kOffScale) +
                                        (int((walk.tile_base + j) % F::kScaleRing) * 2 + is_v) * F::kBn;
                     unsigned char* out = tree_smem + slot_at(slot);
-                    const uint4* src = reinterpret_cast<const uint4*>(tree_smem + F::kOffRaw + raw * F::kRaw + lw * (F::kRaw / 4));
+                    uint4* src = reinterpret_cast<uint4*>(tree_smem + F::kOffRaw + raw * F::kRaw + lw * (F::kRaw / 4));
                     float big = 0.f;
-                    bool bad = false;
                     unsigned bad_rows = 0;
                     if constexpr (KV == 2) {
                         if (is_v) {
                             float* mine_s = scale_col + lw * 32 + lane;
                             float sc = *mine_s;
-                            if (node_row && !isfinite(sc)) {
-                                bad = true;
-                                *mine_s = sc = 0.f;
-                            }
+                            const bool bad = node_values && p0 + lw * 32 + lane >= walk.len && !isfinite(sc);
+                            if (bad) *mine_s = sc = 0.f;
+                            bad_rows = __ballot_sync(0xffffffffu, bad);
                             big = fabsf(sc);
                         }
-#pragma unroll 4
+                        unsigned char* dst = out + (lw * 32 + row_in) * 128;
+#pragma unroll
                         for (int i = 0; i < kIters; ++i) {
-                            const int rt = lw * 32 + i * kStep + lane / kLanes;
                             const uint4 v = ch < chunks ? src[i * 32 + lane] : make_uint4(0, 0, 0, 0);
                             const unsigned w[4] = {v.x, v.y, v.z, v.w};
                             unsigned h[8];
@@ -1225,47 +1234,65 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
 #pragma unroll
                             for (int x = 0; x < 2; ++x) {
                                 const int hc = 2 * ch + x;  // 16-byte chunk of the F16 row
-                                *reinterpret_cast<uint4*>(out + (hc >> 3) * (F::kBn * 128) + rt * 128 +
-                                                          (((hc & 7) ^ (rt & 7)) << 4)) =
+                                *reinterpret_cast<uint4*>(dst + (hc >> 3) * (F::kBn * 128) + i * kStep * 128 +
+                                                          (((hc & 7) ^ row_in ^ ((i * kStep) & 7)) << 4)) =
                                     make_uint4(h[4 * x], h[4 * x + 1], h[4 * x + 2], h[4 * x + 3]);
                             }
                         }
                     } else {
-#pragma unroll 4
-                        for (int i = 0; i < kIters; ++i) {
-                            const int rw = i * kStep + lane / kLanes, rt = lw * kRowsPerWarp + rw;
-                            const uint4 raw_v = ch < chunks ? src[i * 32 + lane] : make_uint4(0, 0, 0, 0);
-                            float v[4] = {__uint_as_float(raw_v.x), __uint_as_float(raw_v.y), __uint_as_float(raw_v.z),
-                                          __uint_as_float(raw_v.w)};
-                            if (is_v && p0 + rt >= walk.len) {
-#pragma unroll
-                                for (int x = 0; x < 4; ++x)
-                                    if (!isfinite(v[x])) v[x] = 0.f, bad = true;
+                        if (node_values) {
+#pragma unroll 1
+                            for (int i = 0; i < kIters; ++i) {
+                                const int rw = i * kStep + row_in;
+                                const uint4 v = src[i * 32 + lane];
+                                const bool bad = ch < chunks && p0 + lw * kRowsPerWarp + rw >= walk.len &&
+                                                 !(isfinite(__uint_as_float(v.x)) && isfinite(__uint_as_float(v.y)) &&
+                                                   isfinite(__uint_as_float(v.z)) && isfinite(__uint_as_float(v.w)));
+                                const unsigned hit = __ballot_sync(0xffffffffu, bad);
+                                if (bad) src[i * 32 + lane] = make_uint4(0, 0, 0, 0);
+                                if (hit & (kLanes == 32 ? 0xffffffffu : 0xffffu)) bad_rows |= 1u << (i * kStep);
+                                if (kLanes == 16 && hit >> 16) bad_rows |= 2u << (i * kStep);
                             }
-                            const unsigned hit = __ballot_sync(0xffffffffu, bad);
-                            bad = false;
-                            if (hit) bad_rows |= kLanes == 32 ? 1u << i : ((hit & 0xffffu) ? 1u << (2 * i) : 0u) | ((hit >> 16) ? 2u << (2 * i) : 0u);
-                            float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+                        }
+                        unsigned char* dst = out + (lw * kRowsPerWarp + row_in) * 128 + (ch >> 4) * (F::kBn * 128) + (ch & 1) * 8;
+                        const int col = ((ch >> 1) & 7) ^ row_in;
+                        const unsigned peers = kLanes == 32 ? 0xffffffffu : lane < 16 ? 0xffffu : 0xffff0000u;  // lanes of a row
 #pragma unroll
-                            for (int d = kLanes / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                            const int up = lift(top);
-                            const float f = two_to(up), back = two_to(-up);
-                            if (ch == 0) scale_col[rt] = back;
-                            big = fmaxf(big, top > 0.f ? back : 0.f);
-                            uint2 hi, lo;
-                            split_exact(v[0] * f, v[1] * f, hi.x, lo.x);
-                            split_exact(v[2] * f, v[3] * f, hi.y, lo.y);
-                            const int at = (ch >> 4) * (F::kBn * 128) + rt * 128 + ((((ch >> 1) & 7) ^ (rt & 7)) << 4) + (ch & 1) * 8;
-                            *reinterpret_cast<uint2*>(out + at) = hi;
-                            *reinterpret_cast<uint2*>(out + F::kSlotPart + at) = lo;
+                        for (int i0 = 0; i0 < kIters; i0 += 4) {
+                            float v[4][4], tops[4];
+#pragma unroll
+                            for (int b = 0; b < 4; ++b) {
+                                const uint4 x = ch < chunks ? src[(i0 + b) * 32 + lane] : make_uint4(0, 0, 0, 0);
+                                v[b][0] = __uint_as_float(x.x);
+                                v[b][1] = __uint_as_float(x.y);
+                                v[b][2] = __uint_as_float(x.z);
+                                v[b][3] = __uint_as_float(x.w);
+                                tops[b] = max3(fmaxf(fabsf(v[b][0]), fabsf(v[b][1])), fabsf(v[b][2]), fabsf(v[b][3]));
+                            }
+#pragma unroll
+                            for (int b = 0; b < 4; ++b) tops[b] = __uint_as_float(__reduce_max_sync(peers, __float_as_uint(tops[b])));
+#pragma unroll
+                            for (int b = 0; b < 4; ++b) {
+                                const int i = i0 + b, up = lift(tops[b]);
+                                const float f = two_to(up), back = two_to(-up);
+                                if (ch == 0) scale_col[lw * kRowsPerWarp + i * kStep + row_in] = back;
+                                big = fmaxf(big, tops[b] > 0.f ? back : 0.f);
+                                uint2 hi, lo;
+                                split_exact(v[b][0] * f, v[b][1] * f, hi.x, lo.x);
+                                split_exact(v[b][2] * f, v[b][3] * f, hi.y, lo.y);
+                                unsigned char* at = dst + i * kStep * 128 + ((col ^ ((i * kStep) & 7)) << 4);
+                                *reinterpret_cast<uint2*>(at) = hi;
+                                *reinterpret_cast<uint2*>(at + F::kSlotPart) = lo;
+                            }
                         }
                     }
                     if (is_v) {
-                        if constexpr (KV == 2) {
-                            const unsigned rows = __ballot_sync(0xffffffffu, bad);
-                            if (lane == 0) M.vbad[meta][lw] = rows;
-                        } else if (lane == 0)
-                            reinterpret_cast<unsigned short*>(M.vbad[meta])[lw] = (unsigned short)bad_rows;
+                        if (lane == 0) {
+                            if constexpr (KV == 2)
+                                M.vbad[meta][lw] = bad_rows;
+                            else
+                                reinterpret_cast<unsigned short*>(M.vbad[meta])[lw] = (unsigned short)bad_rows;
+                        }
 #pragma unroll
                         for (int d = 16; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
                         if (lane == 0) M.vmax[meta][lw] = big;
@@ -1517,46 +1544,56 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
 
 // Items cut by run boundaries: out = sum_i O_i 2^(m_i - M) / sum_i l_i 2^(m_i - M)
 // over the pieces in order (a fixed order, so results repeat bit for bit).
-// Block (b, y) takes rows 8 y .. 8 y + 7 of the item that starts in CTA b.
+// Block (b, y) takes rows 32 y .. 32 y + 31 of the item that starts in CTA b:
+// columns 32 z .. 32 z + 31: lanes are rows, warps groups of four columns.
 template <int DP>
 __global__ void __launch_bounds__(256) tree_combine_kernel(TreeAttn a, const float* partial, const TreeRec* recs) {
+    __shared__ float4 stage[32][9];
     asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the tiles are still being worked on
     const TreeRec rec = recs[blockIdx.x];
-    const int row = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (rec.pieces < 2 || row >= rec.rows) return;
-    const int pr = row < rec.split ? row : 128 + row - rec.split, group = a.group;
-    constexpr int kPer = DP / 32;
-    const long long slot_floats = (long long)kTreeRows * (DP + 2);
-    const auto slot_of = [&](int i) { return partial + (2ll * (blockIdx.x + i) + (i == 0)) * slot_floats; };
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.y * 32 + lane;
+    if (rec.pieces < 2 || int(blockIdx.y) * 32 >= rec.rows) return;
+    const int mine = min(row, rec.rows - 1);  // idle lanes repeat the last row
+    const int pr = mine < rec.split ? mine : 128 + mine - rec.split, parts = rec.pieces * rec.streams;
+    const int group4 = blockIdx.z * 8 + warp;
+    const auto slot_of = [&](int i, int& at) {  // part i: its slot, and the row's place in it
+        const int piece = rec.streams == 2 ? i >> 1 : i;
+        at = rec.streams == 2 ? (i & 1) * 128 + pr : pr;
+        return partial + (2ll * (int(blockIdx.x) + piece) + (piece == 0)) * kTreeRows * (DP + 2);
+    };
     float top = -INFINITY;
-    for (int i = lane; i < rec.pieces; i += 32) top = fmaxf(top, slot_of(i)[kTreeRows * DP + pr]);
-#pragma unroll
-    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    float l = 0.f, o[kPer] = {};
-    for (int base = 0; base < rec.pieces; base += 32) {
-        float f = 0.f;
-        if (base + lane < rec.pieces) {
-            const float* slot = slot_of(base + lane);
-            // nothing seen (or nothing but NaN scores): the sums decide
-            f = top == -INFINITY ? 1.f : ex2(slot[kTreeRows * DP + pr] - top);
-            l += slot[kTreeRows * DP + kTreeRows + pr] * f;
-        }
-        const int here = min(32, rec.pieces - base);
 #pragma unroll 4
-        for (int i = 0; i < here; ++i) {
-            const float fi = __shfl_sync(0xffffffffu, f, i);
-            const float* slot = slot_of(base + i);
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) o[e] += slot[pr * DP + e * 32 + lane] * fi;
-        }
+    for (int i = 0; i < parts; ++i) {
+        int at;
+        const float* slot = slot_of(i, at);
+        top = fmaxf(top, slot[kTreeRows * DP + at]);
     }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-    const int vec = rec.row0 + row, node = unsigned(vec) / unsigned(group), head = rec.head * group + vec - node * group;
-    float* dst = a.out + (long long)(rec.c0 + node) * a.ldo + (long long)head * a.dim;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e)
-        if (e * 32 + lane < a.dim) dst[e * 32 + lane] = l == 0.f && top == -INFINITY ? 0.f : o[e] / l;
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) {
+        int at;
+        const float* slot = slot_of(i, at);
+        // nothing seen (or nothing but NaN scores): the sums decide
+        const float f = top == -INFINITY ? 1.f : ex2(slot[kTreeRows * DP + at] - top);
+        const float4 x = *reinterpret_cast<const float4*>(slot + (group4 * kTreeRows + at) * 4);
+        l += slot[kTreeRows * DP + kTreeRows + at] * f;
+        o.x += x.x * f;
+        o.y += x.y * f;
+        o.z += x.z * f;
+        o.w += x.w * f;
+    }
+    const float f = l == 0.f && top == -INFINITY ? 0.f : 1.f / l;
+    stage[lane][warp] = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+    __syncthreads();
+    // eight lanes write a row's 32 columns
+    const int i = threadIdx.x >> 3, col = threadIdx.x & 7;
+    if (int(blockIdx.y) * 32 + i < rec.rows && (int(blockIdx.z) * 8 + col) * 4 < a.dim) {
+        const int vec = rec.row0 + blockIdx.y * 32 + i, node = unsigned(vec) / unsigned(a.group);
+        const int head = rec.head * a.group + vec - node * a.group;
+        float* dst = a.out + (long long)(rec.c0 + node) * a.ldo + (long long)head * a.dim;
+        reinterpret_cast<float4*>(dst)[blockIdx.z * 8 + col] = stage[i][col];
+    }
 }
 
 int tree_ctas() {
@@ -1566,14 +1603,14 @@ int tree_ctas() {
     return sms;
 }
 
-constexpr int kTreeMaxCtas = 148;
+constexpr int kTreeMaxCtas = 148, kTreeRecBytes = 8192;
 
 template <int KV, int DP>
 void run_tree_mma(const TreeAttn& a, void* workspace, cudaStream_t s) {
     using F = TreeForm<KV, DP>;
     const int ctas = std::min(tree_ctas(), kTreeMaxCtas);
     auto* recs = static_cast<TreeRec*>(workspace);
-    auto* partial = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + 4096);
+    auto* partial = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + kTreeRecBytes);
     TVARA_CUDA(cudaFuncSetAttribute(tree_mma_kernel<KV, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem));
     // head_dim 64 or 128 and blocks of a multiple of 8 positions: cached
     // positions come by TMA, whose boxes never cross a block
@@ -1599,7 +1636,7 @@ void run_tree_mma(const TreeAttn& a, void* workspace, cudaStream_t s) {
     TVARA_CUDA(cudaFuncSetAttribute(tree_combine_kernel<DP>, cudaFuncAttributePreferredSharedMemoryCarveout,
                                     cudaSharedmemCarveoutMaxShared));
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(unsigned(ctas), kTreeRows / 8);
+    config.gridDim = dim3(unsigned(ctas), kTreeRows / 32, DP / 32);
     config.blockDim = dim3(256);
     config.stream = s;
     cudaLaunchAttribute early{};
@@ -1623,9 +1660,9 @@ bool tree_mma_takes(const TreeAttn& a) {
 }  // namespace
 
 std::size_t tree_attention_workspace(const TreeAttn& a) {
-    static_assert(sizeof(TreeRec) * kTreeMaxCtas <= 4096);
+    static_assert(sizeof(TreeRec) * kTreeMaxCtas <= kTreeRecBytes);
     const int dp = a.dim <= 64 ? 64 : 128;
-    return a.dim <= 128 ? 4096 + std::size_t(2) * kTreeMaxCtas * kTreeRows * (dp + 2) * 4 : 256;
+    return a.dim <= 128 ? kTreeRecBytes + std::size_t(2) * kTreeMaxCtas * kTreeRows * (dp + 2) * 4 : 256;
 }
 
 void launch_tree_attention(const TreeAttn& a, void* workspace, cudaStream_t s) {
