@@ -188,7 +188,8 @@ constexpr int kTreeMmaWarp = 12;
 constexpr int kTreePieceWarp = 13;
 constexpr int kTreeRawWarp = 14;
 constexpr int kTreeLoadWarp = 8;
-constexpr unsigned kTreeSpin = 1u << 26;
+constexpr unsigned kTreeNap = 2000;                       // ns a wait may sleep at a time
+constexpr unsigned long long kTreeLimit = 4000000000ull;  // ns after which a wait gives up
 constexpr int kTreeRows = 256;      // query vectors of a partial slot
 constexpr int kPieceRing = 4;
 constexpr int kMetaRing = 8;        // tiles of column masks and int8 scales kept
@@ -208,6 +209,8 @@ struct TreeForm {  // KV: 0 F32, 1 F16, 2 int8
     static constexpr int kItemWeight = 8;                // an item's own cost (Q, merge, output), in tiles
     static constexpr int kElem = KV == 0 ? 4 : KV == 1 ? 2 : 1;
     static constexpr int kRaw = KV == 1 ? 0 : kBn * DP * kElem;  // one unconverted tile
+    static constexpr int kRawPitch = DP * kElem < 128 ? DP * kElem : 128;  // its rows lie in parts of this many bytes,
+    static constexpr int kRawParts = DP * kElem / kRawPitch;               // part after part
     static constexpr int kRawDepth = KV == 1 ? 0 : DP == 64 ? 4 : KV == 0 ? 2 : 3;
     static constexpr int kBase = KV == 1 ? (DP == 64 ? 6 : 3) : (DP == 64 ? 4 : 3);  // ring slots
     static constexpr int kExtra = kPairs ? 2 : 0;        // more of them in the second Q tile when it is not used
@@ -268,6 +271,7 @@ struct TreeMeta {  // at kOffMeta
     };
     unsigned tmem;
     int abort_flag;
+    unsigned char swizzled[4];      // per raw slot: its rows came by TMA
 };
 constexpr int kTreeBars = 50;
 static_assert(kMetaRing == 8 && kPieceRing == 4 && offsetof(TreeMeta, drain) == (kTreeBars - 1) * 8);
@@ -288,22 +292,31 @@ __device__ __forceinline__ void bar_arrive(std::uint64_t* b) {
 __device__ __forceinline__ bool bar_test(std::uint64_t* b, unsigned parity) {
     unsigned ok;
     asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
         : "=r"(ok)
-        : "r"(sm_addr(b)), "r"(parity)
+        : "r"(sm_addr(b)), "r"(parity), "r"(kTreeNap)
         : "memory");
     return ok != 0;
 }
+__device__ __forceinline__ unsigned long long now_ns() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+    return t;
+}
 // Bounded; false after the limit or when another role gave up.
 __device__ __forceinline__ bool bar_wait(std::uint64_t* b, unsigned parity, volatile int* abort_flag, int* status) {
+    if (bar_test(b, parity)) return true;
+    const unsigned long long since = now_ns();
 #pragma unroll 1
-    for (unsigned i = 0; i < kTreeSpin; ++i) {
-        if (bar_test(b, parity)) return true;
+    while (!bar_test(b, parity)) {
         if (*abort_flag) return false;
+        if (now_ns() - since > kTreeLimit) {
+            *abort_flag = 1;
+            atomicOr(status, kTreeTimeout);
+            return false;
+        }
     }
-    *abort_flag = 1;
-    atomicOr(status, kTreeTimeout);
-    return false;
+    return true;
 }
 __device__ __forceinline__ bool elect_one() {
     unsigned p;
@@ -582,6 +595,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
     const unsigned tmem = M.tmem;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     volatile int* abort_flag = &M.abort_flag;
+    volatile int never = 0;  // waits for copies in flight do not end with the others
     if (warp >= kTreeMmaWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
     if (warp == kTreePieceWarp) {
         // --------------------------------------------------------- pieces
@@ -1029,7 +1043,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
         // ------------------------------------------------------------ loads
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         const int lw = warp - kTreeLoadWarp;
-        constexpr int kRowsPerWarp = F::kBn / 4;
+
         unsigned empty_phase = 0xffffffffu;
         int slot = 0, flags = 0;
         if constexpr (KV == 1) {
@@ -1169,19 +1183,17 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
             // on the way out after an error: the slots' own copies first
 #pragma unroll 1
             for (int i = 0; i < F::kBase + F::kExtra && *abort_flag; ++i)
-#pragma unroll 1
-                for (unsigned k = 0; k < (1u << 20) && !bar_test(&M.full[i], empty_phase >> i & 1); ++k) {
-                }
+                bar_wait(&M.full[i], empty_phase >> i & 1, &never, a.status);
         } else {
             // Rows that the row fetch warp (below) has put into the raw ring
             // become F16 operands.
             bool go = true;
             int raw = 0;
             unsigned raw_phase = 0;
-            constexpr int kLanes = DP * F::kElem / 16, kStep = 32 / kLanes;  // lanes per row, rows per instruction
-            constexpr int kIters = kRowsPerWarp / kStep;
-            const int ch = lane % kLanes, row_in = lane / kLanes;
-            static_assert(kStep <= 8 && kIters % 4 == 0);
+            // int8: a lane per row; F32: a lane per half of a row.  With the
+            // swizzle of the TMA boxes a warp reads and writes without bank conflicts.
+            const int row = KV == 2 ? lw * 32 + lane : lw * 16 + (lane & 15);
+            const int f16_swizzle = row & 7;
             for (unsigned piece = 0; go; ++piece) {
                 if (!__all_sync(0xffffffffu, get_piece(piece))) break;
                 const TreePiece& walk = M.piece[piece % kPieceRing];
@@ -1202,22 +1214,23 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                     float* scale_col = reinterpret_cast<float*>(tree_smem + F::kOffScale) +
                                        (int((walk.tile_base + j) % F::kScaleRing) * 2 + is_v) * F::kBn;
                     unsigned char* out = tree_smem + slot_at(slot);
-                    uint4* src = reinterpret_cast<uint4*>(tree_smem + F::kOffRaw + raw * F::kRaw + lw * (F::kRaw / 4));
+                    unsigned char* src = tree_smem + F::kOffRaw + raw * F::kRaw + row * F::kRawPitch;
+                    const int swizzle = M.swizzled[raw] ? (F::kRawPitch == 128 ? row & 7 : row >> 1 & 3) : 0;
+                    const bool node_row = node_values && p0 + row >= walk.len;
                     float big = 0.f;
                     unsigned bad_rows = 0;
+                    unsigned char* dst = out + row * 128;
                     if constexpr (KV == 2) {
                         if (is_v) {
-                            float* mine_s = scale_col + lw * 32 + lane;
-                            float sc = *mine_s;
-                            const bool bad = node_values && p0 + lw * 32 + lane >= walk.len && !isfinite(sc);
-                            if (bad) *mine_s = sc = 0.f;
+                            float sc = scale_col[row];
+                            const bool bad = node_row && !isfinite(sc);
+                            if (bad) scale_col[row] = sc = 0.f;
                             bad_rows = __ballot_sync(0xffffffffu, bad);
                             big = fabsf(sc);
                         }
-                        unsigned char* dst = out + (lw * 32 + row_in) * 128;
 #pragma unroll
-                        for (int i = 0; i < kIters; ++i) {
-                            const uint4 v = ch < chunks ? src[i * 32 + lane] : make_uint4(0, 0, 0, 0);
+                        for (int i = 0; i < DP / 16; ++i) {
+                            const uint4 v = i < chunks ? *reinterpret_cast<const uint4*>(src + ((i ^ swizzle) << 4)) : make_uint4(0, 0, 0, 0);
                             const unsigned w[4] = {v.x, v.y, v.z, v.w};
                             unsigned h[8];
 #pragma unroll
@@ -1232,59 +1245,62 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                                 h[2 * x + 1] = *reinterpret_cast<const unsigned*>(&a1);
                             }
 #pragma unroll
-                            for (int x = 0; x < 2; ++x) {
-                                const int hc = 2 * ch + x;  // 16-byte chunk of the F16 row
-                                *reinterpret_cast<uint4*>(dst + (hc >> 3) * (F::kBn * 128) + i * kStep * 128 +
-                                                          (((hc & 7) ^ row_in ^ ((i * kStep) & 7)) << 4)) =
+                            for (int x = 0; x < 2; ++x)
+                                *reinterpret_cast<uint4*>(dst + (i >> 2) * (F::kBn * 128) + ((((2 * i + x) & 7) ^ f16_swizzle) << 4)) =
                                     make_uint4(h[4 * x], h[4 * x + 1], h[4 * x + 2], h[4 * x + 3]);
-                            }
                         }
                     } else {
-                        if (node_values) {
+                        constexpr int kMine = F::kRawParts / 2;  // 128-byte parts of this lane's half
+                        const int part0 = (lane >> 4) * kMine;
+                        const auto quad = [&](int part, int i) -> uint4* {
+                            return reinterpret_cast<uint4*>(src + part * (F::kBn * 128) + ((i ^ swizzle) << 4));
+                        };
+                        unsigned top = 0;  // the largest magnitude, as bits: NaN and infinity are the largest
+#pragma unroll
+                        for (int k = 0; k < kMine; ++k)
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const uint4 v = (part0 + k) * 8 + i < chunks ? *quad(part0 + k, i) : make_uint4(0, 0, 0, 0);
+                                top = max(max(top, max(v.x & 0x7fffffffu, v.y & 0x7fffffffu)),
+                                          max(v.z & 0x7fffffffu, v.w & 0x7fffffffu));
+                            }
+                        top = max(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                        if (is_v) {
+                            const bool bad = node_row && top >= 0x7f800000u;
+                            bad_rows = __ballot_sync(0xffffffffu, bad) & 0xffffu;
+                            if (bad) {
+                                top = 0;
 #pragma unroll 1
-                            for (int i = 0; i < kIters; ++i) {
-                                const int rw = i * kStep + row_in;
-                                const uint4 v = src[i * 32 + lane];
-                                const bool bad = ch < chunks && p0 + lw * kRowsPerWarp + rw >= walk.len &&
-                                                 !(isfinite(__uint_as_float(v.x)) && isfinite(__uint_as_float(v.y)) &&
-                                                   isfinite(__uint_as_float(v.z)) && isfinite(__uint_as_float(v.w)));
-                                const unsigned hit = __ballot_sync(0xffffffffu, bad);
-                                if (bad) src[i * 32 + lane] = make_uint4(0, 0, 0, 0);
-                                if (hit & (kLanes == 32 ? 0xffffffffu : 0xffffu)) bad_rows |= 1u << (i * kStep);
-                                if (kLanes == 16 && hit >> 16) bad_rows |= 2u << (i * kStep);
+                                for (int i = 0; i < kMine * 8; ++i) *quad(part0 + (i >> 3), i & 7) = make_uint4(0, 0, 0, 0);
                             }
                         }
-                        unsigned char* dst = out + (lw * kRowsPerWarp + row_in) * 128 + (ch >> 4) * (F::kBn * 128) + (ch & 1) * 8;
-                        const int col = ((ch >> 1) & 7) ^ row_in;
-                        const unsigned peers = kLanes == 32 ? 0xffffffffu : lane < 16 ? 0xffffu : 0xffff0000u;  // lanes of a row
+                        const int up = lift(__uint_as_float(top));
+                        const float f = two_to(up), back = two_to(-up);
+                        if (lane < 16) scale_col[row] = back;
+                        big = top ? back : 0.f;
 #pragma unroll
-                        for (int i0 = 0; i0 < kIters; i0 += 4) {
-                            float v[4][4], tops[4];
+                        for (int k = 0; k < kMine; ++k)
 #pragma unroll
-                            for (int b = 0; b < 4; ++b) {
-                                const uint4 x = ch < chunks ? src[(i0 + b) * 32 + lane] : make_uint4(0, 0, 0, 0);
-                                v[b][0] = __uint_as_float(x.x);
-                                v[b][1] = __uint_as_float(x.y);
-                                v[b][2] = __uint_as_float(x.z);
-                                v[b][3] = __uint_as_float(x.w);
-                                tops[b] = max3(fmaxf(fabsf(v[b][0]), fabsf(v[b][1])), fabsf(v[b][2]), fabsf(v[b][3]));
+                            for (int i = 0; i < 8; i += 2) {
+                                float v[8];
+#pragma unroll
+                                for (int x = 0; x < 2; ++x) {
+                                    const uint4 w = (part0 + k) * 8 + i + x < chunks ? *quad(part0 + k, i + x) : make_uint4(0, 0, 0, 0);
+                                    v[4 * x] = __uint_as_float(w.x) * f;
+                                    v[4 * x + 1] = __uint_as_float(w.y) * f;
+                                    v[4 * x + 2] = __uint_as_float(w.z) * f;
+                                    v[4 * x + 3] = __uint_as_float(w.w) * f;
+                                }
+                                uint4 hi, lo;
+                                split_exact(v[0], v[1], hi.x, lo.x);
+                                split_exact(v[2], v[3], hi.y, lo.y);
+                                split_exact(v[4], v[5], hi.z, lo.z);
+                                split_exact(v[6], v[7], hi.w, lo.w);
+                                const int hc = (part0 + k) * 4 + i / 2;  // 16-byte chunk of the F16 row
+                                unsigned char* at = dst + (hc >> 3) * (F::kBn * 128) + (((hc & 7) ^ f16_swizzle) << 4);
+                                *reinterpret_cast<uint4*>(at) = hi;
+                                *reinterpret_cast<uint4*>(at + F::kSlotPart) = lo;
                             }
-#pragma unroll
-                            for (int b = 0; b < 4; ++b) tops[b] = __uint_as_float(__reduce_max_sync(peers, __float_as_uint(tops[b])));
-#pragma unroll
-                            for (int b = 0; b < 4; ++b) {
-                                const int i = i0 + b, up = lift(tops[b]);
-                                const float f = two_to(up), back = two_to(-up);
-                                if (ch == 0) scale_col[lw * kRowsPerWarp + i * kStep + row_in] = back;
-                                big = fmaxf(big, tops[b] > 0.f ? back : 0.f);
-                                uint2 hi, lo;
-                                split_exact(v[b][0] * f, v[b][1] * f, hi.x, lo.x);
-                                split_exact(v[b][2] * f, v[b][3] * f, hi.y, lo.y);
-                                unsigned char* at = dst + i * kStep * 128 + ((col ^ ((i * kStep) & 7)) << 4);
-                                *reinterpret_cast<uint2*>(at) = hi;
-                                *reinterpret_cast<uint2*>(at + F::kSlotPart) = lo;
-                            }
-                        }
                     }
                     if (is_v) {
                         if (lane == 0) {
@@ -1402,17 +1418,15 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
             }
             // nothing of this CTA's may be in flight when its memory is given back
             if (lane == 0) tree_commit_to(&M.drain);
-#pragma unroll 1
-            for (unsigned i = 0; i < kTreeSpin && !bar_test(&M.drain, 0); ++i) {
-            }
+            bar_wait(&M.drain, 0, &never, a.status);
         }
         __syncwarp();
     }
     if (KV != 1 && warp == kTreeRawWarp) {
         // --------------------------------------- rows of F32 and int8 pools
-        // 32 rows at a time: cached positions of whole boxes by TMA, any
-        // others row by row with bulk copies; rows that hold nothing are zero.
-        constexpr int kSlabs = F::kBn / 32, kPitch = DP * F::kElem;
+        // Tiles of cached positions by TMA, a lane per box; others row by row
+        // with bulk copies (rows that hold nothing are zero).
+        constexpr int kSlabs = F::kBn / 32, kPitch = F::kRawPitch;
         bool go = true;
         int raw = 0, flags = 0;
         unsigned empty_phase = 0xffffffffu;
@@ -1457,6 +1471,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                         if (!go) break;
                         empty_phase ^= 1u << raw;
                         if (!is_v && lane < 4) M.valid[tile % kMetaRing][lane] = 0xffffffffu;
+                        if (lane == 0) M.swizzled[raw] = 1;
+                        __syncwarp();
                         const unsigned full = sm_addr(&M.raw_full[raw]);
                         if (lane == 0)
                             asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full),
@@ -1465,7 +1481,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                         __syncwarp();
                         if (lane < boxes) {
                             const long long row = at + (is_v ? a.kind_rows : 0);
-                            tma_load_2d(smem + F::kOffRaw + raw * F::kRaw + lane * a.box_rows * kPitch, &kv_map, 0, int(row), full);
+#pragma unroll
+                            for (int part = 0; part < F::kRawParts; ++part)
+                                tma_load_2d(smem + F::kOffRaw + raw * F::kRaw + (part * F::kBn + lane * a.box_rows) * kPitch, &kv_map,
+                                            part * (kPitch / F::kElem), int(row), full);
                             if constexpr (KV == 2)
                                 bulk_load(smem + F::kOffScale + ((tile % F::kScaleRing * 2 + is_v) * F::kBn + lane * a.box_rows) * 4,
                                           a.scales + row, a.box_rows * 4, full);
@@ -1488,14 +1507,17 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                 empty_phase ^= 1u << raw;
                 const unsigned dst = F::kOffRaw + raw * F::kRaw;
                 int bytes = 0;
+                if (lane == 0) M.swizzled[raw] = 0;
 #pragma unroll
                 for (int i = 0; i < kSlabs; ++i) {
                     const long long at = j == k_last ? cur[i] : prev[i];
                     const unsigned have = __ballot_sync(0xffffffffu, at >= 0);
                     if (!is_v && lane == 0) M.valid[tile % kMetaRing][i] = have;
                     if (at < 0)
-                        for (int k = 0; k < chunks; ++k)
-                            *reinterpret_cast<uint4*>(tree_smem + dst + (32 * i + lane) * kPitch + 16 * k) = make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+                        for (int k = 0; k < F::kRawParts * kPitch / 16; ++k)
+                            *reinterpret_cast<uint4*>(tree_smem + dst + (k / (kPitch / 16) * F::kBn + 32 * i + lane) * kPitch +
+                                                      k % (kPitch / 16) * 16) = make_uint4(0, 0, 0, 0);
                     bytes += __popc(have) * row_bytes;
                 }
                 __syncwarp();
@@ -1507,13 +1529,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                 for (int i = 0; i < kSlabs; ++i) {
                     const long long at = j == k_last ? cur[i] : prev[i], row = at + (is_v ? a.kind_rows : 0);
                     const unsigned to = smem + dst + (32 * i + lane) * kPitch;
-                    const bool slab = a.box_rows && __all_sync(0xffffffffu, at >= 0) &&
-                                      (walk.t0 + j) * F::kBn + 32 * i + 32 <= walk.len;
-                    if (slab) {
-                        if ((lane & (a.box_rows - 1)) == 0) tma_load_2d(to, &kv_map, 0, int(row), full);
-                    } else if (at >= 0) {
-                        bulk_load(to, pool + row * row_bytes, row_bytes, full);
-                    }
+                    if (at >= 0)
+#pragma unroll 1
+                        for (int part = 0; part * kPitch < row_bytes; ++part)
+                            bulk_load(to + part * F::kBn * kPitch, pool + row * row_bytes + part * kPitch,
+                                      min(kPitch, row_bytes - part * kPitch), full);
                     if constexpr (KV == 2)  // the row's scale, straight into its column
                         cp4(smem + F::kOffScale + ((tile % F::kScaleRing * 2 + is_v) * F::kBn + 32 * i + lane) * 4,
                             at >= 0 ? a.scales + row : a.scales, at >= 0 ? 4u : 0u);
@@ -1528,9 +1548,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
         // every copy of this warp has landed before the memory is given back
 #pragma unroll 1
         for (int i = 0; i < F::kRawDepth; ++i)
-#pragma unroll 1
-            for (unsigned k = 0; k < kTreeSpin && !bar_test(&M.raw_full[i], empty_phase >> i & 1); ++k) {
-            }
+            bar_wait(&M.raw_full[i], empty_phase >> i & 1, &never, a.status);
         if (KV == 2) cp_wait<0>();
         if (flags) atomicOr(a.status, flags);
     }
@@ -1622,10 +1640,10 @@ void run_tree_mma(const TreeAttn& a, void* workspace, cudaStream_t s) {
         job.box_rows = a.bt % 32 == 0 ? 32 : a.bt % 16 == 0 ? 16 : 8;
         const cuuint64_t dims[2] = {cuuint64_t(a.dim), cuuint64_t(rows)};
         const cuuint64_t strides[1] = {cuuint64_t(a.dim) * F::kElem};
-        const cuuint32_t box[2] = {cuuint32_t(KV == 1 ? 64 : a.dim), cuuint32_t(job.box_rows)}, ones[2] = {1, 1};
+        const cuuint32_t box[2] = {cuuint32_t(KV == 1 ? 64 : F::kRawPitch / F::kElem), cuuint32_t(job.box_rows)}, ones[2] = {1, 1};
         const auto type = KV == 0 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : KV == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
         if (tensor_map_encoder()(&map, type, 2, const_cast<void*>(a.kv), dims, strides, box, ones,
-                                 CU_TENSOR_MAP_INTERLEAVE_NONE, KV == 1 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, KV != 1 && F::kRawPitch == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
             throw std::runtime_error("cuTensorMapEncodeTiled failed for the KV pool");
     }
