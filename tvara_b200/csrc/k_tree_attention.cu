@@ -370,6 +370,16 @@ __device__ __forceinline__ void tm_st16(unsigned addr, const unsigned (&r)[16]) 
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
+__device__ __forceinline__ void tm_st32(unsigned addr, const unsigned (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+        "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+        "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
+        "r"(r[30]), "r"(r[31])
+        : "memory");
+}
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tm_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -428,6 +438,12 @@ __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
     f32x2 r;
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
+}
+__device__ __forceinline__ void mul2_in(unsigned& x, unsigned& y, f32x2 f) {
+    float u, v;
+    halves_of(mul2(pair_of(__uint_as_float(x), __uint_as_float(y)), f), u, v);
+    x = __float_as_uint(u);
+    y = __float_as_uint(v);
 }
 __device__ __forceinline__ unsigned half2_of(f32x2 v) {
     float x, y;
@@ -787,7 +803,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                     c = __uint_as_float(x);
                 }
             }
-            float m = -INFINITY, l = 0.f, vref = 0.f;
+            float m = -INFINITY, l = 0.f;
+            float vref = 8.0779357e-28f;  // 2^-90: the weights' unit must not overflow
 #pragma unroll
             for (int i = 0; i < DP; ++i) o[i] = 0.f;
             const int tiles = q.t1 - q.t0;
@@ -823,11 +840,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                         if constexpr (KV != 1) {
 #pragma unroll
                             for (int i = 0; i < 32; i += 4) {
-                                const float4 f = *reinterpret_cast<const float4*>(k_scale + 32 * k + i);
-                                x[i] = __float_as_uint(__uint_as_float(x[i]) * f.x);
-                                x[i + 1] = __float_as_uint(__uint_as_float(x[i + 1]) * f.y);
-                                x[i + 2] = __float_as_uint(__uint_as_float(x[i + 2]) * f.z);
-                                x[i + 3] = __float_as_uint(__uint_as_float(x[i + 3]) * f.w);
+                                const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(k_scale + 32 * k + i);
+                                mul2_in(x[i], x[i + 1], f.x);
+                                mul2_in(x[i + 2], x[i + 3], f.y);
                             }
                         }
                         if (!all) {
@@ -839,16 +854,12 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                             for (int i = 0; i < 32; ++i)
                                 if (!(see >> i & 1)) x[i] = 0xff800000u;
                         }
+                        if constexpr (KV != 1) tm_st32(s_at + 32 * k, x);
 #pragma unroll
                         for (int i = 0; i < 32; i += 2)
                             tops[(i >> 1) & 3] = max3(tops[(i >> 1) & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
                     }
                     const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-                    const float mn = fmaxf(m, top * c);
-                    const float off = mn == -INFINITY ? 11.f : 11.f - mn;
-                    keep = mn == -INFINITY ? 1.f : ex2(m - mn);
-                    m = mn;
-                    l *= keep;
                     if (KV != 1 || nodes) {  // scales of V, nodes with a non-finite V
                         go = __all_sync(0xffffffffu, bar_wait(&M.v_ready[t % kMetaRing], (t / kMetaRing) & 1, abort_flag, a.status));
                         if (!go) break;
@@ -858,36 +869,30 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                                 if (seen[k] & M.vbad[ring][k]) l = NAN;  // the row's result is not finite
                         }
                     }
-                    float v_unit = 1.f;
+                    const float mn = fmaxf(m, top * c);
+                    float off = mn == -INFINITY ? 11.f : 11.f - mn;
+                    keep = mn == -INFINITY ? 1.f : ex2(m - mn);
+                    m = mn;
                     if constexpr (KV != 1) {
+                        // weights are kept in units of the largest V scale so far,
+                        // in O and l alike: times a V scale they stay below 2^11
                         const float4 big4 = *reinterpret_cast<const float4*>(M.vmax[ring]);
                         const float big = fmaxf(fmaxf(vref, fmaxf(big4.x, big4.y)), fmaxf(big4.z, big4.w));
-                        if (big > vref) {
-                            keep *= vref / big;
-                            vref = big;
-                        }
-                        v_unit = vref > 0.f ? 1.f / vref : 0.f;
+                        keep *= vref / big;
+                        vref = big;
+                        off -= __log2f(vref);
+                        tm_wait_st();
                     }
+                    l *= keep;
                     // P over S, sixteen positions (one K step of the MMA) at a
                     // time: hi in their first eight columns, lo in the others.
                     f32x2 sums[2] = {0, 0};
-                    const f32x2 c2 = pair_of(c, c), off2 = pair_of(off, off), unit2 = pair_of(v_unit, v_unit);
+                    const f32x2 c2 = pair_of(c, c), off2 = pair_of(off, off);
 #pragma unroll 1
                     for (int k = 0; k < F::kBn / 32; ++k) {
                         unsigned x[32];
                         tm_ld32(s_at + 32 * k, x);
-                        if constexpr (KV != 1) {
-#pragma unroll
-                            for (int i = 0; i < 32; i += 2) {
-                                float v0, v1;
-                                halves_of(mul2(pair_of(__uint_as_float(x[i]), __uint_as_float(x[i + 1])),
-                                               *reinterpret_cast<const f32x2*>(k_scale + 32 * k + i)),
-                                          v0, v1);
-                                x[i] = __float_as_uint(v0);
-                                x[i + 1] = __float_as_uint(v1);
-                            }
-                        }
-                        if (!all) {
+                        if (KV == 1 && !all) {
                             const unsigned see = see_of(k);
 #pragma unroll
                             for (int i = 0; i < 32; ++i)
@@ -897,16 +902,21 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                         for (int g = 0; g < 2; ++g) {
                             unsigned y[16];
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) {
+                            for (int i = 0; i < 8; i += 2) {
                                 const int at = 16 * g + 2 * i;
-                                const f32x2 v = pair_of(__uint_as_float(x[at]), __uint_as_float(x[at + 1]));
-                                float p0, p1;
-                                halves_of(fma2(v, c2, off2), p0, p1);
-                                f32x2 p = pair_of(ex2(p0), ex2(p1));
-                                sums[i & 1] = add2(sums[i & 1], p);
-                                if constexpr (KV != 1)
-                                    p = mul2(p, mul2(unit2, *reinterpret_cast<const f32x2*>(v_scale + 32 * k + at)));
+                                float p0, p1, p2, p3;
+                                halves_of(fma2(pair_of(__uint_as_float(x[at]), __uint_as_float(x[at + 1])), c2, off2), p0, p1);
+                                halves_of(fma2(pair_of(__uint_as_float(x[at + 2]), __uint_as_float(x[at + 3])), c2, off2), p2, p3);
+                                f32x2 p = pair_of(ex2(p0), ex2(p1)), r2 = pair_of(ex2(p2), ex2(p3));
+                                sums[0] = add2(sums[0], p);
+                                sums[1] = add2(sums[1], r2);
+                                if constexpr (KV != 1) {
+                                    const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(v_scale + 32 * k + at);
+                                    p = mul2(p, f.x);
+                                    r2 = mul2(r2, f.y);
+                                }
                                 split_weight(p, y[i], y[8 + i]);
+                                split_weight(r2, y[i + 1], y[9 + i]);
                             }
                             tm_st16(s_at + 32 * k + 16 * g, y);
                         }
@@ -937,10 +947,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                 }
             }
             if (!go) break;
-            if constexpr (KV != 1) {
-#pragma unroll
-                for (int i = 0; i < DP; ++i) o[i] *= vref;
-            }
+            if constexpr (KV != 1) m += __log2f(vref);  // the unit of O and l joins their reference
             // The part of an item that other CTAs continue: (O, m, l) of each
             // stream into the workspace, one thread a row, rows side by side.
             // The CTA's slot 1 holds an item that begins here, slot 0 one that
