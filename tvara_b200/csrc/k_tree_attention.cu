@@ -1204,10 +1204,14 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
             for (unsigned piece = 0; go; ++piece) {
                 if (!__all_sync(0xffffffffu, get_piece(piece))) break;
                 const TreePiece& walk = M.piece[piece % kPieceRing];
-                const int loads = 2 * (walk.t1 - walk.t0);
+                const int first_p = walk.t0 * F::kBn, len = walk.len, tiles = walk.t1 - walk.t0, ahead = min(2, tiles);
+                const unsigned tile_base = walk.tile_base;
+                const int loads = 2 * tiles;
                 for (int e = 0; e < loads && go; ++e) {
-                    bool is_v;
-                    const int j = walk.entry(e, is_v);
+                    // the order of TreePiece::entry, with one M tile
+                    const int f = e - ahead, both = 2 * (tiles - ahead);
+                    const bool is_v = f >= 0 && (f >= both || !(f & 1));
+                    const int j = f < 0 ? e : f < both ? (f >> 1) + (f & 1 ? ahead : 0) : f - (tiles - ahead);
                     go = __all_sync(0xffffffffu, bar_wait(&M.raw_full[raw], (raw_phase >> raw) & 1, abort_flag, a.status));
                     raw_phase ^= 1u << raw;
                     if (!go) break;
@@ -1215,15 +1219,15 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                     go = __all_sync(0xffffffffu, bar_wait(&M.empty[slot], parity, abort_flag, a.status));
                     if (!go) break;
                     empty_phase ^= 1u << slot;
-                    const int meta = int((walk.tile_base + j) % kMetaRing);
-                    const int p0 = (walk.t0 + j) * F::kBn;
-                    const bool node_values = is_v && p0 + F::kBn > walk.len;  // V of nodes may be masked: finite in the products
+                    const int meta = int((tile_base + j) % kMetaRing);
+                    const int p0 = first_p + j * F::kBn;
+                    const bool node_values = is_v && p0 + F::kBn > len;  // V of nodes may be masked: finite in the products
                     float* scale_col = reinterpret_cast<float*>(tree_smem + F::kOffScale) +
-                                       (int((walk.tile_base + j) % F::kScaleRing) * 2 + is_v) * F::kBn;
+                                       (int((tile_base + j) % F::kScaleRing) * 2 + is_v) * F::kBn;
                     unsigned char* out = tree_smem + slot_at(slot);
                     unsigned char* src = tree_smem + F::kOffRaw + raw * F::kRaw + row * F::kRawPitch;
                     const int swizzle = M.swizzled[raw] ? (F::kRawPitch == 128 ? row & 7 : row >> 1 & 3) : 0;
-                    const bool node_row = node_values && p0 + row >= walk.len;
+                    const bool node_row = node_values && p0 + row >= len;
                     float big = 0.f;
                     unsigned bad_rows = 0;
                     unsigned char* dst = out + row * 128;
@@ -1235,10 +1239,13 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                             bad_rows = __ballot_sync(0xffffffffu, bad);
                             big = fabsf(sc);
                         }
+                        uint4 row_codes[DP / 16];  // all read before any is written: no load waits behind a store
+#pragma unroll
+                        for (int i = 0; i < DP / 16; ++i)
+                            row_codes[i] = i < chunks ? *reinterpret_cast<const uint4*>(src + ((i ^ swizzle) << 4)) : make_uint4(0, 0, 0, 0);
 #pragma unroll
                         for (int i = 0; i < DP / 16; ++i) {
-                            const uint4 v = i < chunks ? *reinterpret_cast<const uint4*>(src + ((i ^ swizzle) << 4)) : make_uint4(0, 0, 0, 0);
-                            const unsigned w[4] = {v.x, v.y, v.z, v.w};
+                            const unsigned w[4] = {row_codes[i].x, row_codes[i].y, row_codes[i].z, row_codes[i].w};
                             unsigned h[8];
 #pragma unroll
                             for (int x = 0; x < 4; ++x) {
@@ -1286,13 +1293,17 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                         if (lane < 16) scale_col[row] = back;
                         big = top ? back : 0.f;
 #pragma unroll
-                        for (int k = 0; k < kMine; ++k)
+                        for (int k = 0; k < kMine; ++k) {
+                            uint4 quads[8];  // read before any is written: no load waits behind a store
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                quads[i] = (part0 + k) * 8 + i < chunks ? *quad(part0 + k, i) : make_uint4(0, 0, 0, 0);
 #pragma unroll
                             for (int i = 0; i < 8; i += 2) {
                                 float v[8];
 #pragma unroll
                                 for (int x = 0; x < 2; ++x) {
-                                    const uint4 w = (part0 + k) * 8 + i + x < chunks ? *quad(part0 + k, i + x) : make_uint4(0, 0, 0, 0);
+                                    const uint4 w = quads[i + x];
                                     v[4 * x] = __uint_as_float(w.x) * f;
                                     v[4 * x + 1] = __uint_as_float(w.y) * f;
                                     v[4 * x + 2] = __uint_as_float(w.z) * f;
@@ -1308,6 +1319,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                                 *reinterpret_cast<uint4*>(at) = hi;
                                 *reinterpret_cast<uint4*>(at + F::kSlotPart) = lo;
                             }
+                        }
                     }
                     if (is_v) {
                         if (lane == 0) {
