@@ -18,6 +18,7 @@ namespace {
 // search in shared memory.  All sequences are checked before anything is
 // written, by every CTA alike, so a refused plan writes nothing.
 constexpr int kPlanThreads = 512;
+constexpr int kPlanRun = 4;  // consecutive rows a thread takes when there are no trees
 enum { kPlanRows = 1, kPlanCounts = 2 };
 
 __device__ __forceinline__ int last_at_most(const int* sorted, int n, int x) {
@@ -36,13 +37,13 @@ __global__ void __launch_bounds__(kPlanThreads) tree_plan_kernel(TreePlan a, int
     extern __shared__ int plan_smem[];
     int* cu_s = plan_smem;                      // [n_seq + 1]
     int* first_s = plan_smem + a.n_seq + 1;     // [n_seq + 1]
+    int* parents_s = first_s + a.n_seq + 1;     // trees: parents of this CTA's rows, from their first sequence's start
     __shared__ int warp_sum[kPlanThreads / 32];
-    __shared__ unsigned long long need_total;
+    __shared__ long long warp_need[kPlanThreads / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (tid == 0) need_total = 0;
     const int free_count = *a.free_count;
     int bad = 0, carry = 0;
-    unsigned long long mine = 0;
+    long long mine = 0;
     if (free_count < 0 || free_count > a.free_capacity) bad = kTreeBadLengths;
     for (int base = 0; base < a.n_seq; base += kPlanThreads) {
         const int i = base + tid;
@@ -58,7 +59,7 @@ __global__ void __launch_bounds__(kPlanThreads) tree_plan_kernel(TreePlan a, int
             else
                 need = int(max(0ll, blocks - held));
         }
-        mine += unsigned(need);
+        mine += need;
         int scan = need;
         for (int d = 1; d < 32; d <<= 1) {
             const int up = __shfl_up_sync(0xffffffffu, scan, d);
@@ -78,9 +79,12 @@ __global__ void __launch_bounds__(kPlanThreads) tree_plan_kernel(TreePlan a, int
         carry += all;
         __syncthreads();
     }
-    if (mine) atomicAdd(&need_total, mine);
+    for (int d = 16; d; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
+    if (lane == 0) warp_need[warp] = mine;
     const int refused = __syncthreads_or(bad);
-    if (refused || need_total > (unsigned long long)free_count) {
+    long long need_total = 0;
+    for (int w = 0; w < kPlanThreads / 32; ++w) need_total += warp_need[w];
+    if (refused || need_total > free_count) {
         if (blockIdx.x == 0 && tid == 0) atomicOr(a.status, refused ? kTreeBadLengths : kTreeNoBlocks);
         return;
     }
@@ -105,45 +109,67 @@ __global__ void __launch_bounds__(kPlanThreads) tree_plan_kernel(TreePlan a, int
         if (unsigned(block) >= unsigned(a.max_blocks)) flags |= kTreeBadBlock;
         a.tables[(long long)s * a.stride + a.held[s] + j - first_s[s]] = block;
     }
-    for (int t = at; t < total; t += step) {
-        const int s = last_at_most(cu_s, a.n_seq, t);
-        const int i = t - cu_s[s], len = a.lengths[s], held = a.held[s];
-        const int p = len + i, entry = p / a.bt;
+    // the slot and position of row t of sequence s
+    const auto place = [&](int t, int s, int len, int held) {
+        const int p = len + t - cu_s[s], entry = unsigned(p) / unsigned(a.bt);
         const int block = entry < held ? a.tables[(long long)s * a.stride + entry]
                                        : a.free_blocks[free_count - 1 - (first_s[s] + entry - held)];
         const bool good = unsigned(block) < unsigned(a.max_blocks);
         if (!good) flags |= kTreeBadBlock;
         a.slots[t] = good ? (long long)block * a.bt + (p - entry * a.bt) : -1;
-        if (!a.parents) {
-            a.positions[t] = p;
-            continue;
-        }
-        // Up the tree: indices only fall, so each word of the mask is
-        // complete when the walk leaves it.
-        const int* parents = a.parents + cu_s[s];
-        unsigned long long* row = a.ancestors + (long long)t * a.words;
-        int word = i >> 6, depth = 0, node = i;
-        for (int w = a.words - 1; w > word; --w) row[w] = 0;
-        unsigned long long bits = 1ull << (i & 63);
-        for (;;) {
-            const int up = parents[node];
-            if (up < 0 || up >= node) {
-                if (up != -1) flags |= kTreeBadParent;
-                break;
+        return p;
+    };
+    if (!a.parents) {
+        for (int t0 = at * kPlanRun; t0 < total; t0 += step * kPlanRun) {
+            int s = last_at_most(cu_s, a.n_seq, t0), len = a.lengths[s], held = a.held[s];
+            for (int t = t0; t < min(t0 + kPlanRun, total); ++t) {
+                while (t >= cu_s[s + 1]) {
+                    ++s;
+                    len = a.lengths[s];
+                    held = a.held[s];
+                }
+                a.positions[t] = place(t, s, len, held);
             }
-            node = up;
-            ++depth;
-            while (word > (node >> 6)) {
+        }
+    } else {
+        for (int tile = int(blockIdx.x) * kPlanThreads; tile < total; tile += step) {
+            // the tile's rows and those before them back to their sequence's first
+            const int from = cu_s[last_at_most(cu_s, a.n_seq, tile)], to = min(tile + kPlanThreads, total);
+            __syncthreads();
+            for (int i = from + tid; i < to; i += kPlanThreads) parents_s[i - from] = a.parents[i];
+            __syncthreads();
+            const int t = tile + tid;
+            if (t >= to) continue;
+            const int s = last_at_most(cu_s, a.n_seq, t), len = a.lengths[s];
+            place(t, s, len, a.held[s]);
+            // Up the tree: indices only fall, so each word of the mask is
+            // complete when the walk leaves it.
+            const int* parents = parents_s + (cu_s[s] - from);
+            unsigned long long* row = a.ancestors + (long long)t * a.words;
+            const int i = t - cu_s[s];
+            int word = i >> 6, depth = 0, node = i;
+            for (int w = a.words - 1; w > word; --w) row[w] = 0;
+            unsigned long long bits = 1ull << (i & 63);
+            for (;;) {
+                const int up = parents[node];
+                if (up < 0 || up >= node) {
+                    if (up != -1) flags |= kTreeBadParent;
+                    break;
+                }
+                node = up;
+                ++depth;
+                while (word > (node >> 6)) {
+                    row[word--] = bits;
+                    bits = 0;
+                }
+                bits |= 1ull << (node & 63);
+            }
+            while (word >= 0) {
                 row[word--] = bits;
                 bits = 0;
             }
-            bits |= 1ull << (node & 63);
+            a.positions[t] = len + depth;
         }
-        while (word >= 0) {
-            row[word--] = bits;
-            bits = 0;
-        }
-        a.positions[t] = len + depth;
     }
     if (flags) atomicOr(a.status, flags);
 }
@@ -188,6 +214,7 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(TreeCommit 
     long long* to = from + a.max_nodes;      // [max_nodes]
     int* best = reinterpret_cast<int*>(to + a.max_nodes);  // [max_nodes + 1] first matching child of node - 1
     int* path = best + a.max_nodes + 1;      // [max_nodes]
+    unsigned* choice = reinterpret_cast<unsigned*>(path + a.max_nodes);  // [max_nodes]
     __shared__ int count_s;
     const int s = blockIdx.x, tid = threadIdx.x;
     const int c0 = a.cu[s], c1 = a.cu[s + 1], len = a.lengths[s];
@@ -198,18 +225,30 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(TreeCommit 
     }
     const int n = int(n64);
     const unsigned none = 0xffffffffu;
-    for (int i = tid; i <= n; i += kCommitThreads) best[i] = INT_MAX;
-    __syncthreads();
+    // everything that is known before the walk is fetched at once
     const unsigned first = a.first ? a.first[s] : none;
+    const long long* dest = a.dest ? a.dest : a.slots;
+    for (int i = tid; i < n; i += kCommitThreads) {
+        best[i] = INT_MAX;
+        choice[i] = a.choices[c0 + i];
+        if (a.pool) {
+            from[i] = a.slots[c0 + i];
+            to[i] = dest[c0 + i];
+        }
+    }
+    if (tid == 0) best[n] = INT_MAX;
+    const int parent0 = tid < n ? a.parents[c0 + tid] : 0;
+    const unsigned token0 = tid < n ? a.tokens[c0 + tid] : 0;
+    __syncthreads();
     int flags = 0;
     for (int i = tid; i < n; i += kCommitThreads) {
-        const int p = a.parents[c0 + i];
+        const int p = i == tid ? parent0 : a.parents[c0 + i];
         if (p < -1 || p >= i) {
             flags |= kTreeBadParent;
             continue;
         }
-        const unsigned want = p >= 0 ? a.choices[c0 + p] : first;
-        const bool match = !a.first && i == 0 ? true : want != none && a.tokens[c0 + i] == want;
+        const unsigned want = p >= 0 ? choice[p] : first;
+        const bool match = !a.first && i == 0 ? true : want != none && (i == tid ? token0 : a.tokens[c0 + i]) == want;
         if (match) atomicMin(&best[p + 1], i);
     }
     __syncthreads();
@@ -219,7 +258,7 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(TreeCommit 
         count_s = k;
         if (blockIdx.y == 0) {
             a.accepted[s] = k;
-            a.next[s] = at >= 0 ? a.choices[c0 + at] : first;
+            a.next[s] = at >= 0 ? choice[at] : first;
             a.lengths_out[s] = len + k;
         }
     }
@@ -228,16 +267,26 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(TreeCommit 
     if (blockIdx.y == 0)
         for (int i = tid; i < n; i += kCommitThreads) a.path[c0 + i] = i < rows ? path[i] : -1;
     if (a.pool && rows) {
-        const long long* dest = a.dest ? a.dest : a.slots;
         const long long limit = (long long)a.max_blocks * a.bt;
         const int runs = a.layers * 2 * a.hkv;
         const long long block_rows = (long long)runs * a.bt;
-        for (int k = tid; k < rows; k += kCommitThreads) {
-            const long long f = a.slots[c0 + path[k]], t = dest[c0 + k];
-            const bool good = f >= 0 && f < limit && t >= 0 && t < limit;
-            if (!good) flags |= kTreeBadBlock;
-            from[k] = good && f != t ? f / a.bt * block_rows + f % a.bt : -1;
-            to[k] = good ? t / a.bt * block_rows + t % a.bt : -1;
+        for (int k0 = 0; k0 < rows; k0 += kCommitThreads) {  // path[k] >= k: a pass reads before it writes
+            const int k = k0 + tid;
+            long long f = -1, t = -1;
+            if (k < rows) {
+                f = from[path[k]];
+                t = to[k];
+                const bool good = f >= 0 && f < limit && t >= 0 && t < limit;
+                if (!good) flags |= kTreeBadBlock;
+                const bool moves = good && f != t;
+                f = moves ? f / a.bt * block_rows + f % a.bt : -1;
+                t = moves ? t / a.bt * block_rows + t % a.bt : -1;
+            }
+            __syncthreads();
+            if (k < rows) {
+                from[k] = f;
+                to[k] = t;
+            }
         }
         __syncthreads();
         const int row_units = a.dim * a.elem / int(sizeof(U));
@@ -249,9 +298,11 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(TreeCommit 
 
 template <typename U>
 void run_commit(const TreeCommit& a, cudaStream_t s) {
-    const std::size_t smem = std::size_t(a.max_nodes) * 24 + 8;
+    const std::size_t smem = std::size_t(a.max_nodes) * 28 + 8;
     const long long units = (long long)a.layers * 2 * a.hkv * a.dim * a.elem / (long long)sizeof(U);
-    const long long slices = a.pool ? std::min<long long>((units + kCommitThreads - 1) / kCommitThreads, 256) : 1;
+    // every slice repeats the walk: no more of them than run at the same time
+    const long long room = std::max<long long>(1, 148 * 6 / a.n_seq);
+    const long long slices = a.pool ? std::min<long long>((units + kCommitThreads - 1) / kCommitThreads, room) : 1;
     tree_commit_kernel<U><<<dim3(unsigned(a.n_seq), unsigned(slices)), kCommitThreads, smem, s>>>(a);
     TVARA_LAUNCHED();
 }
@@ -259,9 +310,10 @@ void run_commit(const TreeCommit& a, cudaStream_t s) {
 }  // namespace
 
 void launch_tree_plan(const TreePlan& a, cudaStream_t s) {
-    const std::size_t smem = std::size_t(a.n_seq + 1) * 8;
-    TVARA_CUDA(cudaFuncSetAttribute(tree_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
-    const long long most = std::max<long long>(a.capacity, a.n_seq);
+    const std::size_t smem = std::size_t(a.n_seq + 1) * 8 + (a.parents ? (kPlanThreads + kTreeMaxNodes) * 4 : 0);
+    if (smem > 48 * 1024)
+        TVARA_CUDA(cudaFuncSetAttribute(tree_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+    const long long most = std::max<long long>(a.parents ? a.capacity : (a.capacity + kPlanRun - 1) / kPlanRun, a.n_seq);
     const int grid = int(std::clamp<long long>((most + kPlanThreads - 1) / kPlanThreads, 1, 296));
     // counts written over their own inputs wait until no CTA reads these
     const bool in_place = a.held_out == a.held || a.free_left == a.free_count;
