@@ -9,7 +9,6 @@
 
 #include <cuda_fp16.h>
 
-#include "split.cuh"
 #include "tma.cuh"
 #include "tree.cuh"
 
@@ -168,9 +167,8 @@ __global__ void __launch_bounds__(kAnyWarps * 32) tree_any_kernel(TreeAttn a) {
 // The tensor core's own F32 accumulation truncates, so it is kept to one
 // tile (the small lo products first) and the long sum over tiles is rounded
 // to nearest in registers; that costs one fused multiply-add per element.
-// F32 results from F16 operands: Q, P (and K, V of F32 pools) enter as exact
-// hi + lo F16 pairs of about 22 bits (split.cuh), int8 codes are exact in
-// F16; scales of int8 rows, and the powers of two that bring an F32 row below
+// F32 results from F16 operands: Q, P (and K, V of F32 pools) enter as hi +
+// lo F16 pairs of 22 bits, int8 codes are exact in F16; scales of int8 rows, and the powers of two that bring an F32 row below
 // 2^15, are applied to S columns and to P.
 //
 // Two softmax warpgroups ("streams") keep the tensor core busy: with one M
@@ -447,19 +445,20 @@ __device__ __forceinline__ void mul2_in(unsigned& x, unsigned& y, f32x2 f) {
     x = __float_as_uint(u);
     y = __float_as_uint(v);
 }
-__device__ __forceinline__ unsigned half2_of(f32x2 v) {
-    float x, y;
-    halves_of(v, x, y);
+// A pair of values below 2^16 as hi + lo, F16 each: hi is the value rounded to
+// 11 bits and lo what is left, so hi + lo carries 2^-22 of each value (not of
+// the largest: small softmax weights keep their digits), down to 2^-25 absolute.
+__device__ __forceinline__ void split_pair(float x, float y, unsigned& hi, unsigned& lo) {
     const __half2 h = __floats2half2_rn(x, y);
-    return *reinterpret_cast<const unsigned*>(&h);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const unsigned*>(&h);
+    lo = *reinterpret_cast<const unsigned*>(&l);
 }
-// A pair of weights in [0, 2^11] as hi (integers) + lo (|lo| <= 1/2): F16
-// each, lo's rounding is 2^-13, that is 2^-24 of the row's largest weight.
 __device__ __forceinline__ void split_weight(f32x2 p, unsigned& hi, unsigned& lo) {
-    const f32x2 up = pair_of(12582912.f, 12582912.f), down = pair_of(-12582912.f, -12582912.f);  // 1.5 * 2^23
-    const f32x2 h = add2(add2(p, up), down);
-    hi = half2_of(h);
-    lo = half2_of(fma2(h, pair_of(-1.f, -1.f), p));
+    float x, y;
+    halves_of(p, x, y);
+    split_pair(x, y, hi, lo);
 }
 
 // Quotients of non-negative numbers, mostly below 2^32.
@@ -774,10 +773,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
 #pragma unroll
                     for (int i = 0; i < DP / 8; ++i) {
                         uint4 hi, lo;
-                        split_exact(o[8 * i] * f, o[8 * i + 1] * f, hi.x, lo.x);
-                        split_exact(o[8 * i + 2] * f, o[8 * i + 3] * f, hi.y, lo.y);
-                        split_exact(o[8 * i + 4] * f, o[8 * i + 5] * f, hi.z, lo.z);
-                        split_exact(o[8 * i + 6] * f, o[8 * i + 7] * f, hi.w, lo.w);
+                        split_pair(o[8 * i] * f, o[8 * i + 1] * f, hi.x, lo.x);
+                        split_pair(o[8 * i + 2] * f, o[8 * i + 3] * f, hi.y, lo.y);
+                        split_pair(o[8 * i + 4] * f, o[8 * i + 5] * f, hi.z, lo.z);
+                        split_pair(o[8 * i + 6] * f, o[8 * i + 7] * f, hi.w, lo.w);
                         unsigned char* at = mine + (i >> 3) * 16384 + (((i & 7) ^ (lane & 7)) << 4);
                         *reinterpret_cast<uint4*>(at) = hi;
                         *reinterpret_cast<uint4*>(at + F::kQPart) = lo;
@@ -1312,10 +1311,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                                     v[4 * x + 3] = __uint_as_float(w.w) * f;
                                 }
                                 uint4 hi, lo;
-                                split_exact(v[0], v[1], hi.x, lo.x);
-                                split_exact(v[2], v[3], hi.y, lo.y);
-                                split_exact(v[4], v[5], hi.z, lo.z);
-                                split_exact(v[6], v[7], hi.w, lo.w);
+                                split_pair(v[0], v[1], hi.x, lo.x);
+                                split_pair(v[2], v[3], hi.y, lo.y);
+                                split_pair(v[4], v[5], hi.z, lo.z);
+                                split_pair(v[6], v[7], hi.w, lo.w);
                                 const int hc = (part0 + k) * 4 + i / 2;  // 16-byte chunk of the F16 row
                                 unsigned char* at = dst + (hc >> 3) * (F::kBn * 128) + (((hc & 7) ^ f16_swizzle) << 4);
                                 *reinterpret_cast<uint4*>(at) = hi;
