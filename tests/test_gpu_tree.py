@@ -187,6 +187,121 @@ def test_attention_captured_with_changing_lengths(capi):
     del graph
 
 
+@pytest.mark.parametrize("kv", ["f32", "f16", "i8"])
+@pytest.mark.parametrize("bt", [8, 16, 32, 48, 128, 12])
+def test_attention_wide_heads_by_block_size(capi, kv, bt):
+    """head_dim 128 with boxes of 8, 16 and 32 rows, and a size with none."""
+    rng = np.random.default_rng(100 + bt)
+    T.AttentionCase(rng, kv, [700, 129, 64], [33, 5, 40], 8, 2, 128, bt=bt, layers=3).upload().run(capi).check()
+
+
+@pytest.mark.parametrize("kv", ["f32", "f16", "i8"])
+@pytest.mark.parametrize("n_seq", [513, 2000])
+def test_attention_more_sequences_than_threads(capi, kv, n_seq):
+    rng = np.random.default_rng(n_seq)
+    lengths = [int(x) for x in rng.integers(0, 40, n_seq)]
+    nodes = [int(x) for x in rng.integers(0, 4, n_seq)]
+    T.AttentionCase(rng, kv, lengths, nodes, 4, 2, 64, layers=1, layer=0).upload().run(capi).check()
+
+
+@pytest.mark.parametrize("kv", ["f32", "f16", "i8"])
+def test_attention_one_long_sequence(capi, kv):
+    """One item cut into pieces for every SM."""
+    rng = np.random.default_rng(15)
+    T.AttentionCase(rng, kv, [30000], [3], 4, 1, 64, layers=1, layer=0).upload().run(capi).check()
+
+
+@pytest.mark.parametrize("q_scale,k_scale,v_scale", [(1e-6, 1, 1), (30, 1, 1), (1e-12, 1e12, 1e10), (1, 1, 1e-12)])
+def test_attention_f32_magnitudes(capi, q_scale, k_scale, v_scale):
+    """F32 values far outside F16's range: every row has its own power of two."""
+    rng = np.random.default_rng(16)
+    c = T.AttentionCase(rng, "f32", [300, 20], [20, 33], 8, 2, 64, q_scale=q_scale)
+    rows = np.exp(rng.uniform(-3, 3, c.pool.shape[0] * c.pool.shape[4])).reshape(c.pool.shape[0], 1, 1, c.pool.shape[4], 1)
+    rows = np.exp2(np.round(np.log2(rows))).astype(np.float32)  # uneven rows, by powers of two
+    c.pool[:, :, 0] *= (k_scale * rows).astype(np.float32)
+    c.pool[:, :, 1] *= (v_scale * rows).astype(np.float32)
+    for s, length in enumerate(c.lengths):
+        p = np.arange(length)
+        slot = np.concatenate([c.tables[s][p // c.bt].astype(np.int64) * c.bt + p % c.bt, c.slots[c.cu[s]:c.cu[s + 1]]])
+        for kind, to in ((0, c.k), (1, c.v)):
+            to[s] = np.moveaxis(c.pool[slot // c.bt, 1, kind, :, slot % c.bt].astype(np.float64), 1, 0)
+    c.upload().run(capi).check()
+
+
+@pytest.mark.parametrize("kv", ["f16", "i8"])
+def test_attention_and_commit_beyond_32_bit_offsets(capi, kv):
+    """Blocks more than 2^32 bytes (and 2^32 elements of int8) into the pool."""
+    import torch
+    rng = np.random.default_rng(17)
+    c = T.AttentionCase(rng, kv, [100, 33], [9, 20], 8, 2, 128, bt=16, layers=2)
+    per_block = int(np.prod(c.pool.shape[1:]))
+    far = (1 << 32) // per_block + 7
+    blocks = far + len(c.pool)
+    pool = torch.empty((blocks,) + c.pool.shape[1:], dtype=torch.from_numpy(c.pool).dtype, device="cuda")
+    pool[far:].copy_(torch.from_numpy(c.pool))
+    c.tables[c.tables >= 0] += far
+    c.slots[c.slots >= 0] += far * c.bt
+    c.upload()
+    c.dev.set(pool=pool, max_blocks=blocks)
+    scales = None
+    if kv == "i8":
+        scales = torch.empty((blocks,) + c.scales.shape[1:], device="cuda")
+        scales[far:].copy_(torch.from_numpy(c.scales))
+        c.dev.set(kv_scales=scales)
+    c.run(capi).check()
+    # move node 5's row of sequence 0 over node 0's
+    dev = T.Dev(B.TreeCommitArgs, kv_dtype=T.KV[kv][0], kv_heads=2, head_dim=128, block_tokens=16, layers=2, n_seq=1,
+                capacity=9, max_nodes=9, max_blocks=blocks)
+    parents = np.full(9, -1, np.int32)
+    dev.set(lengths=np.array([100], np.int32), cu_nodes=np.array([0, 9], np.int32), parents=parents,
+            tokens=np.arange(9, dtype=np.uint32), choices=np.full(9, 77, np.uint32), first=np.array([5], np.uint32),
+            slots=c.slots[:9].copy(), pool=pool, path=np.zeros(9, np.int32), accepted=np.zeros(1, np.int32),
+            next=np.zeros(1, np.uint32), lengths_out=np.zeros(1, np.int32), status=np.zeros(1, np.int32))
+    if scales is not None:
+        dev.set(kv_scales=scales)
+    check(capi, capi.tvara_tree_commit(dev.by, None))
+    assert dev.get("accepted")[0] == 1 and dev.get("status")[0] == 0
+    a, b = c.slots[5] - far * 16, c.slots[0]
+    want = c.pool[a // 16, :, :, :, a % 16]
+    assert np.array_equal(pool[int(b // 16), :, :, :, int(b % 16)].cpu().numpy().view(np.uint8), want.view(np.uint8))
+
+
+def test_attention_shared_prefix_and_shared_slots(capi):
+    """Sequences that share cached blocks, and nodes that share a slot."""
+    rng = np.random.default_rng(18)
+    c = T.AttentionCase(rng, "f16", [64, 64, 80], [9, 9, 4], 8, 2, 128, masks="any")
+    c.tables[1, :4] = c.tables[0, :4]
+    c.k[1][:, :64], c.v[1][:, :64] = c.k[0][:, :64], c.v[0][:, :64]
+    c.slots[c.cu[0] + 3] = c.slots[c.cu[0] + 8]
+    c.k[0][:, 64 + 3], c.v[0][:, 64 + 3] = c.k[0][:, 64 + 8], c.v[0][:, 64 + 8]
+    c.upload().run(capi).check()
+
+
+def test_attention_calls_on_two_streams(capi):
+    """Concurrent calls, each with its own workspace and status."""
+    import torch
+    cases = [T.AttentionCase(np.random.default_rng(s), kv, [900, 40], [20, 64], 8, 2, 128).upload()
+             for s, kv in ((1, "f16"), (2, "i8"), (3, "f32"), (4, "f16"))]
+    streams = [torch.cuda.Stream() for _ in cases]
+    sync()
+    for _ in range(3):
+        for c, s in zip(cases, streams):
+            c.run(capi, s.cuda_stream)
+            c.hold = getattr(c, "hold", []) + [c.workspace]
+    sync()
+    for c in cases:
+        c.check()
+
+
+def test_attention_refuses_an_unaligned_workspace(capi):
+    import torch
+    c = T.AttentionCase(np.random.default_rng(1), "f16", [9], [2], 4, 2, 64).upload()
+    size = capi.tvara_tree_attention_workspace(c.dev.by)
+    work = torch.empty(size + 16, dtype=torch.uint8, device="cuda")
+    assert capi.tvara_tree_attention(c.dev.by, work.data_ptr() + 4, size, None) == -1
+    assert b"aligned" in capi.tvara_last_error()
+
+
 # ----------------------------------------------------------------------- plan
 def plan_case(rng, lengths, nodes, bt, tree, spare_free=5, extra_held=0, max_nodes=None, spare_rows=2):
     n_seq = len(lengths)
