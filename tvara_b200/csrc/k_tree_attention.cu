@@ -1270,12 +1270,13 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                         const auto quad = [&](int part, int i) -> uint4* {
                             return reinterpret_cast<uint4*>(src + part * (F::kBn * 128) + ((i ^ swizzle) << 4));
                         };
+                        uint4 quads[8];    // one part at a time; all read before any is written
                         unsigned top = 0;  // the largest magnitude, as bits: NaN and infinity are the largest
 #pragma unroll
                         for (int k = 0; k < kMine; ++k)
 #pragma unroll
                             for (int i = 0; i < 8; ++i) {
-                                const uint4 v = (part0 + k) * 8 + i < chunks ? *quad(part0 + k, i) : make_uint4(0, 0, 0, 0);
+                                const uint4 v = quads[i] = (part0 + k) * 8 + i < chunks ? *quad(part0 + k, i) : make_uint4(0, 0, 0, 0);
                                 top = max(max(top, max(v.x & 0x7fffffffu, v.y & 0x7fffffffu)),
                                           max(v.z & 0x7fffffffu, v.w & 0x7fffffffu));
                             }
@@ -1285,8 +1286,12 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                             bad_rows = __ballot_sync(0xffffffffu, bad) & 0xffffu;
                             if (bad) {
                                 top = 0;
+                                if (kMine > 1)
 #pragma unroll 1
-                                for (int i = 0; i < kMine * 8; ++i) *quad(part0 + (i >> 3), i & 7) = make_uint4(0, 0, 0, 0);
+                                    for (int i = 0; i < kMine * 8; ++i) *quad(part0 + (i >> 3), i & 7) = make_uint4(0, 0, 0, 0);
+                                else
+#pragma unroll
+                                    for (int i = 0; i < 8; ++i) quads[i] = make_uint4(0, 0, 0, 0);
                             }
                         }
                         const int up = lift(__uint_as_float(top));
@@ -1295,10 +1300,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                         big = top ? back : 0.f;
 #pragma unroll
                         for (int k = 0; k < kMine; ++k) {
-                            uint4 quads[8];  // read before any is written: no load waits behind a store
+                            if (kMine > 1)
 #pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                quads[i] = (part0 + k) * 8 + i < chunks ? *quad(part0 + k, i) : make_uint4(0, 0, 0, 0);
+                                for (int i = 0; i < 8; ++i)
+                                    quads[i] = (part0 + k) * 8 + i < chunks ? *quad(part0 + k, i) : make_uint4(0, 0, 0, 0);
 #pragma unroll
                             for (int i = 0; i < 8; i += 2) {
                                 float v[8];
