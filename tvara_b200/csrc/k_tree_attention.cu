@@ -613,7 +613,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     volatile int* abort_flag = &M.abort_flag;
     volatile int never = 0;  // waits for copies in flight do not end with the others
-    if (warp >= kTreeMmaWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    if (warp >= kTreeMmaWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == kTreePieceWarp) {
         // --------------------------------------------------------- pieces
         if (lane == 0) {
@@ -713,7 +713,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
 
     if (warp < kTreeLoadWarp) {
         // ------------------------------------------------ softmax warpgroups
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
         const int stream = warp >> 2, wq = warp & 3, r = tid & 127;
         const unsigned lane_base = tmem + (unsigned(wq * 32) << 16);
         const unsigned s_at = lane_base + stream * 128, o_at = lane_base + 256 + stream * 128;
@@ -1049,7 +1049,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
         }
     } else if (warp < kTreeMmaWarp) {
         // ------------------------------------------------------------ loads
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         const int lw = warp - kTreeLoadWarp;
 
         unsigned empty_phase = 0xffffffffu;
