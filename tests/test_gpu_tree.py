@@ -277,6 +277,24 @@ def test_attention_shared_prefix_and_shared_slots(capi):
     c.upload().run(capi).check()
 
 
+@pytest.mark.parametrize("kv", ["f16", "f32"])
+@pytest.mark.parametrize("bt", [16, 12])
+def test_attention_alternating_tree_sizes(capi, kv, bt):
+    """Neighbouring sequences with one and with two tiles of query vectors, few
+    positions each, so that a CTA changes between the two many times; repeated
+    calls agree bit for bit."""
+    rng = np.random.default_rng(19)
+    nodes = [64 if i % 2 else 3 for i in range(120)]
+    lengths = [int(x) for x in rng.integers(0, 300, 120)]
+    c = T.AttentionCase(rng, kv, lengths, nodes, 8, 2, 128, bt=bt, layers=1, layer=0).upload().run(capi)
+    c.check()
+    first = c.dev.get("out").copy()
+    for _ in range(20):
+        c.dev.keep["out"].zero_()
+        c.run(capi)
+        assert np.array_equal(c.dev.get("out")[:c.total], first[:c.total])
+
+
 def test_attention_calls_on_two_streams(capi):
     """Concurrent calls, each with its own workspace and status."""
     import torch

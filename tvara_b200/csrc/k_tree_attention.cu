@@ -27,15 +27,15 @@ __device__ __forceinline__ bool tree_sequence_ok(const TreeAttn& a, int s, int& 
            len <= (long long)a.stride * a.bt && len <= 0x7fffffff - 2 * kTreeMaxNodes;
 }
 
-// Row (of dim elements) in the pool that holds K of head 0 of the layer for
-// index p of a sequence (cached positions, then nodes), or -1 with the status
-// bit for a block or slot outside the pool.
 // x / bt for x < 2^44 by the reciprocal 2^64 / bt rounded up (0 stands for
-// bt 1): it is too large by less than bt / 2^64 <= 2^-44, so the product is
-// off by less than one step of the quotient's fraction.
+// bt 1), which is too large by less than 2^-64: the product by less than
+// 2^-20, and the fraction of x / bt is at most 1 - 2^-20 (bt <= 2^20).
 __device__ __forceinline__ long long div_bt(const TreeAttn& a, long long x) {
     return a.bt_inverse ? (long long)__umul64hi((unsigned long long)x, a.bt_inverse) : x;
 }
+// Row (of dim elements) in the pool that holds K of head 0 of the layer for
+// index p of a sequence (cached positions, then nodes), or -1 with the status
+// bit for a block or slot outside the pool.
 __device__ __forceinline__ long long tree_row(const TreeAttn& a, int s, int c0, int len, int p, int& flags) {
     long long block, off;
     if (p < len) {
@@ -168,8 +168,9 @@ __global__ void __launch_bounds__(kAnyWarps * 32) tree_any_kernel(TreeAttn a) {
 // tile (the small lo products first) and the long sum over tiles is rounded
 // to nearest in registers; that costs one fused multiply-add per element.
 // F32 results from F16 operands: Q, P (and K, V of F32 pools) enter as hi +
-// lo F16 pairs of 22 bits, int8 codes are exact in F16; scales of int8 rows, and the powers of two that bring an F32 row below
-// 2^15, are applied to S columns and to P.
+// lo F16 pairs of 22 bits, int8 codes are exact in F16; the scales of int8
+// rows, and the powers of two that bring F32 rows below 2^15, are applied to
+// the columns of S and to P.
 //
 // Two softmax warpgroups ("streams") keep the tensor core busy: with one M
 // tile they take the even and the odd tiles of the same item, each with its
@@ -298,10 +299,26 @@ __device__ __forceinline__ bool bar_test(std::uint64_t* b, unsigned parity) {
         : "memory");
     return ok != 0;
 }
+__device__ __forceinline__ bool bar_done(std::uint64_t* b, unsigned parity) {  // without waiting
+    unsigned ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(sm_addr(b)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ unsigned long long now_ns() {
     unsigned long long t;
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
     return t;
+}
+// On the way out: copies in flight land within microseconds.
+__device__ __forceinline__ void bar_land(std::uint64_t* b, unsigned parity) {
+    const unsigned long long since = now_ns();
+#pragma unroll 1
+    while (!bar_test(b, parity) && now_ns() - since < 20000000ull) {
+    }
 }
 // Bounded; false after the limit or when another role gave up.
 __device__ __forceinline__ bool bar_wait(std::uint64_t* b, unsigned parity, volatile int* abort_flag, int* status) {
@@ -612,7 +629,6 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
     const unsigned tmem = M.tmem;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     volatile int* abort_flag = &M.abort_flag;
-    volatile int never = 0;  // waits for copies in flight do not end with the others
     if (warp >= kTreeMmaWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == kTreePieceWarp) {
         // --------------------------------------------------------- pieces
@@ -781,7 +797,15 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                         *reinterpret_cast<uint4*>(at) = hi;
                         *reinterpret_cast<uint4*>(at + F::kQPart) = lo;
                     }
-                    if (!q.pair) {  // for the other stream, in its idle tensor memory
+                    if (!q.pair) {
+                        // For the other stream, in its accumulator's place: free once that
+                        // stream is done with the piece before (which is known already,
+                        // unless that one had two M tiles).
+                        if (piece) {
+                            go = __all_sync(0xffffffffu, bar_wait(&M.merge_ready, (piece - 1) & 1, abort_flag, a.status));
+                            if (!go) break;
+                            tm_after();
+                        }
                         asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(lane_base + 384),
                                      "r"(__float_as_uint(c))
                                      : "memory");
@@ -1015,6 +1039,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                     if (lane == 0) bar_arrive(&M.merge_read);
                 }
             } else {  // both barriers count every piece
+                tm_before();
                 __syncwarp();
                 if (lane == 0) bar_arrive(stream ? &M.merge_ready : &M.merge_read);
             }
@@ -1096,7 +1121,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                         if (!go) break;
                     }
                     const unsigned parity = (empty_phase >> slot) & 1;
-                    if (!__all_sync(0xffffffffu, bar_test(&M.empty[slot], parity))) {
+                    if (!__all_sync(0xffffffffu, bar_done(&M.empty[slot], parity))) {
                         drain();  // nothing can be issued: hand over what has landed meanwhile
                         go = __all_sync(0xffffffffu, bar_wait(&M.empty[slot], parity, abort_flag, a.status));
                         if (!go) break;
@@ -1191,7 +1216,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
             // on the way out after an error: the slots' own copies first
 #pragma unroll 1
             for (int i = 0; i < F::kBase + F::kExtra && *abort_flag; ++i)
-                bar_wait(&M.full[i], empty_phase >> i & 1, &never, a.status);
+                bar_land(&M.full[i], empty_phase >> i & 1);
         } else {
             // Rows that the row fetch warp (below) has put into the raw ring
             // become F16 operands.
@@ -1443,7 +1468,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
             }
             // nothing of this CTA's may be in flight when its memory is given back
             if (lane == 0) tree_commit_to(&M.drain);
-            bar_wait(&M.drain, 0, &never, a.status);
+            bar_land(&M.drain, 0);
         }
         __syncwarp();
     }
@@ -1573,7 +1598,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
         // every copy of this warp has landed before the memory is given back
 #pragma unroll 1
         for (int i = 0; i < F::kRawDepth; ++i)
-            bar_wait(&M.raw_full[i], empty_phase >> i & 1, &never, a.status);
+            bar_land(&M.raw_full[i], empty_phase >> i & 1);
         if (KV == 2) cp_wait<0>();
         if (flags) atomicOr(a.status, flags);
     }
