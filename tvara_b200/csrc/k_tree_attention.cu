@@ -472,6 +472,20 @@ __device__ __forceinline__ void split_pair(float x, float y, unsigned& hi, unsig
     hi = *reinterpret_cast<const unsigned*>(&h);
     lo = *reinterpret_cast<const unsigned*>(&l);
 }
+// A pair below 2^15 as hi (a multiple of 16) + lo (|lo| <= 8): 2^-9 absolute,
+// in three packed additions.  Enough for K and V of F32 rows, whose largest
+// value lies in [2^14, 2^15); the products of their lo with that of Q or P,
+// which are left out, are 2^-23 of the value.
+__device__ __forceinline__ void split_fixed(f32x2 x, unsigned& hi, unsigned& lo) {
+    const f32x2 up = pair_of(201326592.f, 201326592.f), down = pair_of(-201326592.f, -201326592.f);  // 1.5 * 2^27
+    const f32x2 h = add2(add2(x, up), down), r = fma2(h, pair_of(-1.f, -1.f), x);
+    float a, b, c, d;
+    halves_of(h, a, b);
+    halves_of(r, c, d);
+    const __half2 hh = __floats2half2_rn(a, b), ll = __floats2half2_rn(c, d);
+    hi = *reinterpret_cast<const unsigned*>(&hh);
+    lo = *reinterpret_cast<const unsigned*>(&ll);
+}
 __device__ __forceinline__ void split_weight(f32x2 p, unsigned& hi, unsigned& lo) {
     float x, y;
     halves_of(p, x, y);
@@ -1223,9 +1237,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
             bool go = true;
             int raw = 0;
             unsigned raw_phase = 0;
-            // int8: a lane per row; F32: a lane per half of a row.  With the
+            // int8: a lane per row; F32: a lane per 128 bytes of a row.  With the
             // swizzle of the TMA boxes a warp reads and writes without bank conflicts.
-            const int row = KV == 2 ? lw * 32 + lane : lw * 16 + (lane & 15);
+            constexpr int kRound = 32 / F::kRawParts;  // rows a warp takes at a time
+            const int row = lw * (F::kBn / 4) + lane % kRound;
             const int f16_swizzle = row & 7;
             for (unsigned piece = 0; go; ++piece) {
                 if (!__all_sync(0xffffffffu, get_piece(piece))) break;
@@ -1253,14 +1268,13 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                     unsigned char* out = tree_smem + slot_at(slot);
                     unsigned char* src = tree_smem + F::kOffRaw + raw * F::kRaw + row * F::kRawPitch;
                     const int swizzle = M.swizzled[raw] ? (F::kRawPitch == 128 ? row & 7 : row >> 1 & 3) : 0;
-                    const bool node_row = node_values && p0 + row >= len;
                     float big = 0.f;
                     unsigned bad_rows = 0;
                     unsigned char* dst = out + row * 128;
                     if constexpr (KV == 2) {
                         if (is_v) {
                             float sc = scale_col[row];
-                            const bool bad = node_row && !isfinite(sc);
+                            const bool bad = node_values && p0 + row >= len && !isfinite(sc);
                             if (bad) scale_col[row] = sc = 0.f;
                             bad_rows = __ballot_sync(0xffffffffu, bad);
                             big = fabsf(sc);
@@ -1290,63 +1304,51 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                                     make_uint4(h[4 * x], h[4 * x + 1], h[4 * x + 2], h[4 * x + 3]);
                         }
                     } else {
-                        constexpr int kMine = F::kRawParts / 2;  // 128-byte parts of this lane's half
-                        const int part0 = (lane >> 4) * kMine;
-                        const auto quad = [&](int part, int i) -> uint4* {
-                            return reinterpret_cast<uint4*>(src + part * (F::kBn * 128) + ((i ^ swizzle) << 4));
-                        };
-                        uint4 quads[8];    // one part at a time; all read before any is written
-                        unsigned top = 0;  // the largest magnitude, as bits: NaN and infinity are the largest
-#pragma unroll
-                        for (int k = 0; k < kMine; ++k)
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                const uint4 v = quads[i] = (part0 + k) * 8 + i < chunks ? *quad(part0 + k, i) : make_uint4(0, 0, 0, 0);
-                                top = max(max(top, max(v.x & 0x7fffffffu, v.y & 0x7fffffffu)),
-                                          max(v.z & 0x7fffffffu, v.w & 0x7fffffffu));
-                            }
-                        top = max(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                        if (is_v) {
-                            const bool bad = node_row && top >= 0x7f800000u;
-                            bad_rows = __ballot_sync(0xffffffffu, bad) & 0xffffu;
-                            if (bad) {
-                                top = 0;
-                                if (kMine > 1)
+                        const int part = lane / kRound;
 #pragma unroll 1
-                                    for (int i = 0; i < kMine * 8; ++i) *quad(part0 + (i >> 3), i & 7) = make_uint4(0, 0, 0, 0);
-                                else
+                        for (int round = 0; round < F::kBn / 4; round += kRound) {
+                            const unsigned char* mine = src + part * (F::kBn * 128) + round * 128;  // (rounds of 8 or 16 rows
+                            uint4 quads[8];                                                         // keep the swizzle)
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                quads[i] = part * 8 + i < chunks ? *reinterpret_cast<const uint4*>(mine + ((i ^ swizzle) << 4)) : make_uint4(0, 0, 0, 0);
+                            if (node_values) {
+                                unsigned most = 0;  // magnitudes as bits: infinity and NaN are the largest
+#pragma unroll
+                                for (int i = 0; i < 8; ++i)
+                                    most = max(max(most, max(quads[i].x & 0x7fffffffu, quads[i].y & 0x7fffffffu)),
+                                               max(quads[i].z & 0x7fffffffu, quads[i].w & 0x7fffffffu));
+#pragma unroll
+                                for (int d = kRound; d < 32; d <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+                                const bool bad = p0 + row + round >= len && most >= 0x7f800000u;
+                                bad_rows |= (__ballot_sync(0xffffffffu, bad) & ((1u << kRound) - 1)) << round;
+                                if (bad)
 #pragma unroll
                                     for (int i = 0; i < 8; ++i) quads[i] = make_uint4(0, 0, 0, 0);
                             }
-                        }
-                        const int up = lift(__uint_as_float(top));
-                        const float f = two_to(up), back = two_to(-up);
-                        if (lane < 16) scale_col[row] = back;
-                        big = top ? back : 0.f;
+                            float tops[2] = {0.f, 0.f};
 #pragma unroll
-                        for (int k = 0; k < kMine; ++k) {
-                            if (kMine > 1)
+                            for (int i = 0; i < 8; ++i) {
+                                tops[0] = max3(tops[0], fabsf(__uint_as_float(quads[i].x)), fabsf(__uint_as_float(quads[i].y)));
+                                tops[1] = max3(tops[1], fabsf(__uint_as_float(quads[i].z)), fabsf(__uint_as_float(quads[i].w)));
+                            }
+                            float top = fmaxf(tops[0], tops[1]);
 #pragma unroll
-                                for (int i = 0; i < 8; ++i)
-                                    quads[i] = (part0 + k) * 8 + i < chunks ? *quad(part0 + k, i) : make_uint4(0, 0, 0, 0);
+                            for (int d = kRound; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                            const int up = lift(top);
+                            const float f = two_to(up), back = two_to(-up);
+                            if (lane < kRound) scale_col[row + round] = back;
+                            big = fmaxf(big, top > 0.f ? back : 0.f);
+                            const f32x2 f2 = pair_of(f, f);
 #pragma unroll
                             for (int i = 0; i < 8; i += 2) {
-                                float v[8];
-#pragma unroll
-                                for (int x = 0; x < 2; ++x) {
-                                    const uint4 w = quads[i + x];
-                                    v[4 * x] = __uint_as_float(w.x) * f;
-                                    v[4 * x + 1] = __uint_as_float(w.y) * f;
-                                    v[4 * x + 2] = __uint_as_float(w.z) * f;
-                                    v[4 * x + 3] = __uint_as_float(w.w) * f;
-                                }
                                 uint4 hi, lo;
-                                split_pair(v[0], v[1], hi.x, lo.x);
-                                split_pair(v[2], v[3], hi.y, lo.y);
-                                split_pair(v[4], v[5], hi.z, lo.z);
-                                split_pair(v[6], v[7], hi.w, lo.w);
-                                const int hc = (part0 + k) * 4 + i / 2;  // 16-byte chunk of the F16 row
-                                unsigned char* at = dst + (hc >> 3) * (F::kBn * 128) + (((hc & 7) ^ f16_swizzle) << 4);
+                                split_fixed(mul2(pair_of(__uint_as_float(quads[i].x), __uint_as_float(quads[i].y)), f2), hi.x, lo.x);
+                                split_fixed(mul2(pair_of(__uint_as_float(quads[i].z), __uint_as_float(quads[i].w)), f2), hi.y, lo.y);
+                                split_fixed(mul2(pair_of(__uint_as_float(quads[i + 1].x), __uint_as_float(quads[i + 1].y)), f2), hi.z, lo.z);
+                                split_fixed(mul2(pair_of(__uint_as_float(quads[i + 1].z), __uint_as_float(quads[i + 1].w)), f2), hi.w, lo.w);
+                                const int hc = part * 4 + i / 2;  // 16-byte chunk of the F16 row
+                                unsigned char* at = dst + round * 128 + (hc >> 3) * (F::kBn * 128) + (((hc & 7) ^ f16_swizzle) << 4);
                                 *reinterpret_cast<uint4*>(at) = hi;
                                 *reinterpret_cast<uint4*>(at + F::kSlotPart) = lo;
                             }
