@@ -17,6 +17,12 @@ namespace {
 // table entries are spread over the grid and find their sequence by a binary
 // search in shared memory.  All sequences are checked before anything is
 // written, by every CTA alike, so a refused plan writes nothing.
+//
+// Bound by latency, not bytes: a launch, one read of the lengths, the scan, a
+// search and, for trees, the walk up in shared memory.  One tree of 26 nodes
+// 7.6 us a call, 500 trees of up to 63 nodes 8.0 us, 511 prompts of up to 2,047
+// rows (6.3 MB) 10.2 us.  (Summing all needs with one contended shared-memory
+// atomic cost 12 us; a thread per prompt row instead of four, another 8 us.)
 constexpr int kPlanThreads = 512;
 constexpr int kPlanRun = 4;  // consecutive rows a thread takes when there are no trees
 enum { kPlanRows = 1, kPlanCounts = 2 };
@@ -184,6 +190,11 @@ __global__ void __launch_bounds__(kPlanThreads) tree_plan_kernel(TreePlan a, int
 // accepted row, kCommitRows rows in flight at a time.  In place, path[k] > k
 // or the rows coincide, and a batch is read before it is written, so
 // ascending batches never read a row that was overwritten.
+//
+// 48 sequences, 32 layers of 8 heads of 128 F16: 34 MB in 12.3 us (5.3 us at
+// the copy bandwidth); one sequence 6.6 us, a launch and four dependent
+// fetches.  Slices of one sequence beyond those that run at the same time only
+// repeat the walk (1,536 instead of 864 CTAs: 16.4 us).
 constexpr int kCommitThreads = 256;
 constexpr int kCommitRows = 8;
 

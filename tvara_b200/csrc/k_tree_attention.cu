@@ -181,6 +181,23 @@ __global__ void __launch_bounds__(kAnyWarps * 32) tree_any_kernel(TreeAttn a) {
 // (each CTA scans the lengths and cuts out its run), so ragged batches and a
 // single long sequence fill the device alike; an item cut by a run boundary
 // leaves partial (O, m, l) in the workspace for tree_combine_kernel.
+//
+// What bounds it.  A tile of 128 positions costs a stream 32 MMAs of 64
+// cycles (hi and lo of Q, and of P), of which the Q K^T half reads shared
+// memory at its full rate (8 KB in 64 cycles); softmax, acc and the waits in
+// between are hidden by the other stream.  F16 with two M tiles: 6,700 cycles
+// a tile for 4,096 of MMA (4 trees of up to 255 nodes over 8,000-30,000
+// positions: 560 us sustained, tensor pipe 65% busy).  F16 with one M tile:
+// about 3,200 cycles a tile, 2,835 of HBM; a ragged batch adds some 17,000 to
+// 25,000 cycles an item for Q, the pipeline's ends and the output (64 trees
+// over 200-4,000 positions: 265 us, 35% of the copy bandwidth, tensor pipe
+// 49%).  int8 and F32 pools: the conversion warps, whose loads wait behind the
+// MMAs' reads of shared memory (24 sequences int8: 206 us; 31 of the small
+// heads F32: 97 us).  Small calls: instruction fetch; code executed once costs
+// about a nanosecond per three instructions, so loops here stay rolled unless
+// registers force them open (unrolling everything was 181 KB and 3 times
+// slower on the batch).  Register shares of 200/64/48 or 184/96/48 for softmax,
+// loads and the rest were 2 to 10% slower than 192/72/56.
 constexpr int kTreeThreads = 512;   // WG0, WG1 softmax; WG2 loads; warp 12 issues the MMAs, warp 13 deals
                                     // the pieces, warp 14 fetches the rows that WG2 converts (F32, int8)
 constexpr int kTreeMmaWarp = 12;
@@ -205,9 +222,11 @@ struct TreeForm {  // KV: 0 F32, 1 F16, 2 int8
     static constexpr int kQTile = 2 * kQPart;
     static constexpr int kSlotPart = kHalves * kBn * 128;
     static constexpr int kSlot = kParts * kSlotPart;     // one K or V tile
-    // an item's own cost (Q, merge, output) in tiles; the best of 4, 6, 8, 11
-    // for ragged batches of each type (64 trees F16: 248, 244, 231, 233 us)
-    static constexpr int kItemWeight = KV == 0 ? 4 : KV == 1 ? 8 : 6;
+    // an item's own cost (Q, merge, output) in tiles, chosen on ragged batches
+    // of each type (64 trees F16 with 4, 6, 8, 11: 248, 244, 231, 233 us; 32
+    // sequences F32 of 128 values with 4, 7, 10: 187, 163, 161 us, 31 of 64
+    // values: 98, 93, 99 us; 24 sequences int8 with 4, 6, 9: 215, 212, 215 us)
+    static constexpr int kItemWeight = KV == 0 ? 7 : KV == 1 ? 8 : 6;
     static constexpr int kElem = KV == 0 ? 4 : KV == 1 ? 2 : 1;
     static constexpr int kRaw = KV == 1 ? 0 : kBn * DP * kElem;  // one unconverted tile
     static constexpr int kRawPitch = DP * kElem < 128 ? DP * kElem : 128;  // its rows lie in parts of this many bytes,
