@@ -248,8 +248,9 @@ TVARA_API int tvara_tree_attention(const tvara_tree_attention_args* args, void* 
  * matches.  With first NULL, node 0 is accepted as it is (the token already
  * emitted, its K and V not yet in the cache).  path[cu_nodes[s] + k] is the
  * k-th accepted node, -1 behind the last; accepted[s] counts them; next[s] is
- * the choice the walk ended with (0xFFFFFFFF when there is none);
- * lengths_out[s] = lengths[s] + accepted[s], and may be lengths itself.
+ * the choice the walk ended with (0xFFFFFFFF when there is none), and may be
+ * first itself; lengths_out[s] = lengths[s] + accepted[s], and may be lengths
+ * itself.  No other output may overlap an input.
  * With a pool, the K and V rows of the k-th accepted node (every layer and KV
  * head, int8 scales too) are copied from its slot to dest[cu_nodes[s] + k];
  * dest NULL means slots: the drafts were written behind the cached positions,

@@ -622,6 +622,17 @@ def test_commit_bad_parents_slots_and_lengths_are_reported(capi):
     assert np.array_equal(dev.get("pool")[t // 16, :, :, :, t % 16], pool[t // 16, :, :, :, t % 16])
 
 
+@pytest.mark.parametrize("kv", ["f16", "i8"])
+def test_commit_next_over_first_and_lengths_in_place(capi, kv):
+    """Many slices per sequence, all walking from `first` while `next` replaces it."""
+    for seed in range(5):
+        rng = np.random.default_rng(30 + seed)
+        dev, want = commit_case(rng, kv, [40, 64, 3], 16, 8, 128, 16, True, keep_going=1.0)
+        dev.set(next=dev.keep["first"], lengths_out=dev.keep["lengths"])
+        check(capi, capi.tvara_tree_commit(dev.by, None))
+        check_commit(dev, want)
+
+
 def test_commit_without_a_pool_only_walks(capi):
     rng = np.random.default_rng(7)
     dev, want = commit_case(rng, "f16", [30, 20], 2, 2, 64, 16, True)

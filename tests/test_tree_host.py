@@ -52,7 +52,8 @@ SIZES = [(dict(n_seq=0), "sequences"), (dict(n_seq=8193), "sequences"), (dict(ca
 @pytest.mark.parametrize("fields,text", SIZES + [
     (dict(parents=None), "go together"), (dict(ancestors=None), "go together"), (dict(table_stride=0), "table width"),
     (dict(slots=None), "arguments"), (dict(free_blocks=None), "arguments"), (dict(held_out=SOME + 4), "overlap"),
-    (dict(held_out=2 * SOME + 4), "overlap"), (dict(free_left=2 * SOME), "overlap")])
+    (dict(held_out=2 * SOME + 4), "overlap"), (dict(free_left=2 * SOME), "overlap"),
+    (dict(held_out=3 * SOME + 16), "overlap"), (dict(free_left=SOME), "overlap"), (dict(free_left=6 * SOME + 2), "overlap")])
 def test_plan_refusals(capi, fields, text):
     refused(capi, capi.tvara_tree_plan(C.byref(plan(**fields)), None), text)
 
@@ -88,6 +89,8 @@ def test_attention_workspace_is_required(capi):
     (dict(head_dim=0), "geometry"), (dict(layers=0), "geometry"), (dict(layers=65535, head_dim=65535), "geometry"),
     (dict(slots=None), "geometry"), (dict(parents=None), "arguments"), (dict(tokens=None), "arguments"),
     (dict(choices=None), "arguments"), (dict(path=None), "arguments"), (dict(accepted=None), "arguments"),
-    (dict(next=None), "arguments"), (dict(lengths_out=None), "arguments")])
+    (dict(next=None), "arguments"), (dict(lengths_out=None), "arguments"),
+    (dict(next=SOME), "overlap"), (dict(next=6 * SOME + 4), "overlap"), (dict(accepted=6 * SOME), "overlap"),
+    (dict(lengths_out=SOME + 8), "overlap"), (dict(accepted=2 * SOME + 16), "overlap")])
 def test_commit_refusals(capi, fields, text):
     refused(capi, capi.tvara_tree_commit(C.byref(commit(**fields)), None), text)

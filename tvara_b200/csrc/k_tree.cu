@@ -218,8 +218,12 @@ __device__ __forceinline__ void move_columns(U* base, int units, int row_units, 
     }
 }
 
+// parts: kCommitMove, kCommitAnswers, or both in one launch (the answers by
+// slice 0, which is safe as long as no other slice still reads what they overwrite).
+enum { kCommitMove = 1, kCommitAnswers = 2 };
+
 template <typename U>
-__global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(TreeCommit a) {
+__global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(TreeCommit a, int parts) {
     extern __shared__ long long commit_smem[];
     long long* from = commit_smem;           // [max_nodes] source row of accepted node k, -1: not moved
     long long* to = from + a.max_nodes;      // [max_nodes]
@@ -228,6 +232,8 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(TreeCommit 
     unsigned* choice = reinterpret_cast<unsigned*>(path + a.max_nodes);  // [max_nodes]
     __shared__ int count_s;
     const int s = blockIdx.x, tid = threadIdx.x;
+    const bool answers = (parts & kCommitAnswers) && blockIdx.y == 0;
+    // (lengths_out may be lengths: other slices see either value, and only ask whether it is negative)
     const int c0 = a.cu[s], c1 = a.cu[s + 1], len = a.lengths[s];
     const long long n64 = (long long)c1 - c0;
     if (c0 < 0 || n64 < 0 || n64 > a.max_nodes || c1 > a.capacity || len < 0) {
@@ -267,7 +273,7 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(TreeCommit 
         int k = 0, at = -1;
         while (best[at + 1] != INT_MAX) path[k++] = at = best[at + 1];
         count_s = k;
-        if (blockIdx.y == 0) {
+        if (answers) {
             a.accepted[s] = k;
             a.next[s] = at >= 0 ? choice[at] : first;
             a.lengths_out[s] = len + k;
@@ -275,9 +281,9 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(TreeCommit 
     }
     __syncthreads();
     const int rows = count_s;
-    if (blockIdx.y == 0)
+    if (answers)
         for (int i = tid; i < n; i += kCommitThreads) a.path[c0 + i] = i < rows ? path[i] : -1;
-    if (a.pool && rows) {
+    if (a.pool && rows && (parts & kCommitMove)) {
         const long long limit = (long long)a.max_blocks * a.bt;
         const int runs = a.layers * 2 * a.hkv;
         const long long block_rows = (long long)runs * a.bt;
@@ -314,8 +320,15 @@ void run_commit(const TreeCommit& a, cudaStream_t s) {
     // every slice repeats the walk: no more of them than run at the same time
     const long long room = std::max<long long>(1, 148 * 6 / a.n_seq);
     const long long slices = a.pool ? std::min<long long>((units + kCommitThreads - 1) / kCommitThreads, room) : 1;
-    tree_commit_kernel<U><<<dim3(unsigned(a.n_seq), unsigned(slices)), kCommitThreads, smem, s>>>(a);
+    // next written over first waits until no slice reads first any more
+    const bool apart = a.first && a.next == a.first && slices > 1;
+    tree_commit_kernel<U><<<dim3(unsigned(a.n_seq), unsigned(slices)), kCommitThreads, smem, s>>>(
+        a, apart ? kCommitMove : kCommitMove | kCommitAnswers);
     TVARA_LAUNCHED();
+    if (apart) {
+        tree_commit_kernel<U><<<dim3(unsigned(a.n_seq), 1), kCommitThreads, smem, s>>>(a, kCommitAnswers);
+        TVARA_LAUNCHED();
+    }
 }
 
 }  // namespace

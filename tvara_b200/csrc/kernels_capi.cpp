@@ -422,7 +422,9 @@ int tvara_tree_plan(const tvara_tree_plan_args* a, void* stream) {
         const std::size_t counts = a->n_seq * 4;
         if ((a->held_out != a->held && overlap(a->held_out, counts, a->held, counts)) ||
             overlap(a->held_out, counts, a->lengths, counts) || overlap(a->free_left, 4, a->held, counts) ||
-            overlap(a->held_out, counts, a->free_count, 4))
+            overlap(a->held_out, counts, a->free_count, 4) || overlap(a->held_out, counts, a->cu_nodes, counts + 4) ||
+            overlap(a->free_left, 4, a->lengths, counts) || overlap(a->free_left, 4, a->cu_nodes, counts + 4) ||
+            (a->free_left != a->free_count && overlap(a->free_left, 4, a->free_count, 4)))
             throw std::invalid_argument("plan outputs overlap its inputs");
         tvara::TreePlan j;
         j.bt = int(a->block_tokens);
@@ -480,6 +482,15 @@ int tvara_tree_commit(const tvara_tree_commit_args* a, void* stream) {
         if (!a->lengths || !a->cu_nodes || !a->accepted || !a->next || !a->lengths_out || !a->status ||
             (a->capacity && (!a->parents || !a->tokens || !a->choices || !a->path)))
             throw std::invalid_argument("invalid tree commit arguments");
+        const std::size_t per_seq = a->n_seq * 4;
+        const void* outs[] = {a->accepted, a->next, a->lengths_out};
+        for (const void* out : outs) {
+            // next may be first, lengths_out may be lengths; anything else would change what the walk reads
+            const bool over = overlap(out, per_seq, a->cu_nodes, per_seq + 4) ||
+                              (a->first && out != (out == a->next ? a->first : nullptr) && overlap(out, per_seq, a->first, per_seq)) ||
+                              (out != (out == a->lengths_out ? a->lengths : nullptr) && overlap(out, per_seq, a->lengths, per_seq));
+            if (over) throw std::invalid_argument("commit outputs overlap its inputs");
+        }
         tvara::TreeCommit j;
         if (a->pool) {
             if (a->kv_dtype > TVARA_KV_I8 || (a->kv_dtype == TVARA_KV_I8 && !a->kv_scales))
