@@ -157,6 +157,10 @@ TVARA_API int tvara_paged_attention_noalloc(const tvara_attention_args* args, vo
  * nodes a sequence (max_nodes, the width the ancestor masks are laid out for:
  * ceil(max_nodes / 64) words a row).
  *
+ * Arrays are aligned to their types, the workspace to 16 bytes.  Heads of at
+ * most 128 values, with rows of q, out and pool that are multiples of 16 bytes
+ * at 16-byte addresses, run on the tensor cores; others are much slower.
+ *
  * What the host can check is refused as by the calls above.  What only the
  * device sees sets bits of *status (device, one word, never cleared by these
  * calls: zero it once and look when convenient), and nothing outside the
@@ -214,7 +218,8 @@ TVARA_API int tvara_tree_plan(const tvara_tree_plan_args* args, void* stream);
  * Scores are q.k / sqrt(head_dim), query head h reads KV head
  * h / (heads / kv_heads), arithmetic and outputs are F32 to within rounding
  * for every pool type (as tvara_paged_attention).  A row that attends to
- * nothing is zero; masked K and V may hold anything, NaN included.  One
+ * nothing is zero; masked K and V may hold anything, NaN included.  Rows of
+ * out may not meet rows of q (column slices of one buffer are fine).  One
  * workspace serves one call at a time. */
 typedef struct tvara_tree_attention_args {
     uint32_t struct_size;         /* sizeof(tvara_tree_attention_args) */

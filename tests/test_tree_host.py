@@ -94,3 +94,47 @@ def test_attention_workspace_is_required(capi):
     (dict(lengths_out=SOME + 8), "overlap"), (dict(accepted=2 * SOME + 16), "overlap")])
 def test_commit_refusals(capi, fields, text):
     refused(capi, capi.tvara_tree_commit(C.byref(commit(**fields)), None), text)
+
+
+# Arrays are read by their own types: an address off by half of one would fault on the device.
+@pytest.mark.parametrize("call,fields", [
+    ("plan", dict(lengths=SOME + 2)), ("plan", dict(tables=7 * SOME + 2)), ("plan", dict(slots=8 * SOME + 4)),
+    ("plan", dict(ancestors=10 * SOME + 4)), ("plan", dict(status=13 * SOME + 1)),
+    ("attention", dict(q=SOME + 2)), ("attention", dict(out=2 * SOME + 2)), ("attention", dict(pool=3 * SOME + 1)),
+    ("attention", dict(kv_dtype=0, pool=3 * SOME + 2)), ("attention", dict(kv_dtype=2, kv_scales=4 * SOME + 2)),
+    ("attention", dict(slots=8 * SOME + 4)), ("attention", dict(ancestors=9 * SOME + 4)),
+    ("attention", dict(cu_nodes=7 * SOME + 3)),
+    ("commit", dict(tokens=4 * SOME + 2)), ("commit", dict(slots=7 * SOME + 4)), ("commit", dict(dest=8 * SOME + 4)),
+    ("commit", dict(pool=9 * SOME + 1)), ("commit", dict(kv_dtype=2, kv_scales=10 * SOME + 2)),
+    ("commit", dict(path=11 * SOME + 2))])
+def test_misaligned_arrays(capi, call, fields):
+    if call == "attention":
+        status = capi.tvara_tree_attention(C.byref(attention(**fields)), C.c_void_p(SOME), 1 << 40, None)
+    else:
+        status = {"plan": capi.tvara_tree_plan, "commit": capi.tvara_tree_commit}[call](
+            C.byref({"plan": plan, "commit": commit}[call](**fields)), None)
+    refused(capi, status, "aligned")
+
+
+@pytest.mark.parametrize("name", ["parents", "tokens", "choices"])
+def test_commit_path_apart_from_what_the_walk_reads(capi, name):
+    at = [n for n, k in B.TreeCommitArgs._fields_ if k is C.c_void_p].index(name) + 1
+    refused(capi, capi.tvara_tree_commit(C.byref(commit(path=at * SOME + 396)), None), "overlap")
+    refused(capi, capi.tvara_tree_commit(C.byref(commit(path=at * SOME - 396)), None), "overlap")
+
+
+# Rows of 512 floats out of 100; q begins at SOME.
+@pytest.mark.parametrize("fields", [
+    dict(out=SOME), dict(out=SOME + 2044), dict(out=SOME - 2044), dict(out=SOME + 99 * 2048 + 2044),
+    dict(q_stride=1024, out_stride=1024, out=SOME + 2044), dict(q_stride=1024, out_stride=1024, out=SOME + 5 * 4096 - 2044),
+    dict(q_stride=1024, out_stride=1028, out=SOME + 2048)])
+def test_attention_out_apart_from_q(capi, fields):
+    refused(capi, capi.tvara_tree_attention(C.byref(attention(**fields)), C.c_void_p(50 * SOME), 1 << 40, None), "overlap")
+
+
+# Column slices of one buffer are apart: such a call is refused only for its missing workspace.
+@pytest.mark.parametrize("fields", [
+    dict(q_stride=1024, out_stride=1024, out=SOME + 2048), dict(q_stride=1024, out_stride=1024, out=SOME - 2048),
+    dict(q_stride=1536, out_stride=1536, out=SOME + 4096), dict(out=SOME + 100 * 2048), dict(out=SOME - 100 * 2048)])
+def test_attention_out_beside_q(capi, fields):
+    refused(capi, capi.tvara_tree_attention(C.byref(attention(**fields)), None, 0, None), "workspace")

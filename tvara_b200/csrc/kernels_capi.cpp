@@ -6,6 +6,7 @@
 #include <cstring>
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 #include <string>
 #include <vector>
 
@@ -357,6 +358,25 @@ bool overlap(const void* a, std::size_t na, const void* b, std::size_t nb) {
     return x < y + nb && y < x + na;
 }
 
+// Arrays are read by their own types; an address off by half of one would fault on the device.
+void check_aligned(std::size_t bytes, std::initializer_list<const void*> arrays) {
+    for (const void* at : arrays)
+        if (reinterpret_cast<std::uintptr_t>(at) % bytes) throw std::invalid_argument("arrays are not aligned to their type");
+}
+
+// Rows of `width` floats: out may be written while q is still read, so no row
+// of one may meet a row of the other; column slices of one buffer are apart.
+bool rows_overlap(const float* q, std::size_t q_stride, const float* out, std::size_t out_stride, std::size_t rows,
+                  std::size_t width) {
+    using wide = unsigned __int128;
+    const wide x = reinterpret_cast<std::uintptr_t>(q), y = reinterpret_cast<std::uintptr_t>(out);
+    const wide nx = ((wide(rows) - 1) * q_stride + width) * 4, ny = ((wide(rows) - 1) * out_stride + width) * 4;
+    if (x >= y + ny || y >= x + nx) return false;
+    if (q_stride != out_stride) return true;
+    const wide stride = wide(q_stride) * 4, off = y >= x ? (y - x) % stride : (stride - (x - y) % stride) % stride;
+    return off < wide(width) * 4 || off > stride - wide(width) * 4;
+}
+
 tvara::TreeAttn tree_attention_job(const tvara_tree_attention_args* a) {
     if (!a || a->struct_size < sizeof(tvara_tree_attention_args))
         throw std::invalid_argument("invalid tree attention arguments");
@@ -426,6 +446,9 @@ int tvara_tree_plan(const tvara_tree_plan_args* a, void* stream) {
             overlap(a->free_left, 4, a->lengths, counts) || overlap(a->free_left, 4, a->cu_nodes, counts + 4) ||
             (a->free_left != a->free_count && overlap(a->free_left, 4, a->free_count, 4)))
             throw std::invalid_argument("plan outputs overlap its inputs");
+        check_aligned(4, {a->lengths, a->held, a->cu_nodes, a->parents, a->free_blocks, a->free_count, a->tables,
+                          a->positions, a->held_out, a->free_left, a->status});
+        check_aligned(8, {a->slots, a->ancestors});
         tvara::TreePlan j;
         j.bt = int(a->block_tokens);
         j.n_seq = int(a->n_seq);
@@ -466,6 +489,12 @@ int tvara_tree_attention(const tvara_tree_attention_args* a, void* workspace, si
             throw std::invalid_argument("invalid tree attention arguments");
         if (a->kv_dtype == TVARA_KV_I8 && !a->kv_scales)
             throw std::invalid_argument("invalid KV dtype or missing int8 scales");
+        check_aligned(4, {a->q, a->out, a->tables, a->lengths, a->cu_nodes, a->status, j.scales});
+        check_aligned(8, {a->slots, a->ancestors});
+        check_aligned(j.kv_kind == 0 ? 4 : j.kv_kind == 1 ? 2 : 1, {a->pool});
+        if (a->capacity &&
+            rows_overlap(a->q, a->q_stride, a->out, a->out_stride, a->capacity, std::size_t(a->heads) * a->head_dim))
+            throw std::invalid_argument("attention output rows overlap the query rows");
         if (!workspace || workspace_bytes < tvara::tree_attention_workspace(j))
             throw std::invalid_argument("attention workspace too small");
         if (reinterpret_cast<std::uintptr_t>(workspace) % 16) throw std::invalid_argument("attention workspace is not 16-byte aligned");
@@ -491,6 +520,13 @@ int tvara_tree_commit(const tvara_tree_commit_args* a, void* stream) {
                               (out != (out == a->lengths_out ? a->lengths : nullptr) && overlap(out, per_seq, a->lengths, per_seq));
             if (over) throw std::invalid_argument("commit outputs overlap its inputs");
         }
+        const std::size_t per_row = a->capacity * 4;
+        for (const void* in : std::initializer_list<const void*>{a->parents, a->tokens, a->choices})
+            if (a->capacity && (overlap(a->path, per_row, in, per_row) || overlap(a->accepted, per_seq, in, per_row) ||
+                                overlap(a->next, per_seq, in, per_row) || overlap(a->lengths_out, per_seq, in, per_row)))
+                throw std::invalid_argument("commit outputs overlap its inputs");
+        check_aligned(4, {a->lengths, a->cu_nodes, a->parents, a->tokens, a->choices, a->first, a->path, a->accepted,
+                          a->next, a->lengths_out, a->status});
         tvara::TreeCommit j;
         if (a->pool) {
             if (a->kv_dtype > TVARA_KV_I8 || (a->kv_dtype == TVARA_KV_I8 && !a->kv_scales))
@@ -505,10 +541,13 @@ int tvara_tree_commit(const tvara_tree_commit_args* a, void* stream) {
             j.bt = int(a->block_tokens);
             j.layers = int(a->layers);
             j.max_blocks = int(a->max_blocks);
+            check_aligned(8, {a->slots, a->dest});
+            check_aligned(std::size_t(j.elem), {a->pool});
             j.pool = a->pool;
             j.scales = a->kv_dtype == TVARA_KV_I8 ? a->kv_scales : nullptr;
             j.slots = reinterpret_cast<const long long*>(a->slots);
             j.dest = reinterpret_cast<const long long*>(a->dest);
+            check_aligned(4, {j.scales});
         }
         j.n_seq = int(a->n_seq);
         j.capacity = int(a->capacity);
