@@ -291,7 +291,6 @@ struct TreeMeta {  // at kOffMeta
     };
     unsigned tmem;
     int abort_flag;
-    unsigned char swizzled[4];      // per raw slot: its rows came by TMA
 };
 constexpr int kTreeBars = 50;
 static_assert(kMetaRing == 8 && kPieceRing == 4 && offsetof(TreeMeta, drain) == (kTreeBars - 1) * 8);
@@ -579,7 +578,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
         bar_init(&M.full[0] + i, i < 8    ? 4                   // full: load warps
                                  : i < 16 ? 1                   // empty: MMA commits
                                  : i < 24 ? 4                   // v_ready: load warps
-                                 : i < 32 ? (i & 4 ? 4 : KV == 2 ? 33 : 1)  // raw_full, raw_empty
+                                 : i < 32 ? (i & 4 ? 4 : 33)          // raw_full: the row fetch warp and its copies; raw_empty
                                  : i < 40 ? (i & 4 ? (KV == 1 ? 13 : 14) : 1)  // piece_full, piece_empty: 8 softmax
                                                                                // warps, 4 load warps, MMA, row fetch
                                  : i < 42 ? 1                   // s_full
@@ -1286,7 +1285,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                                        (int((tile_base + j) % F::kScaleRing) * 2 + is_v) * F::kBn;
                     unsigned char* out = tree_smem + slot_at(slot);
                     unsigned char* src = tree_smem + F::kOffRaw + raw * F::kRaw + row * F::kRawPitch;
-                    const int swizzle = M.swizzled[raw] ? (F::kRawPitch == 128 ? row & 7 : row >> 1 & 3) : 0;
+                    const int swizzle = F::kRawPitch == 128 ? row & 7 : row >> 1 & 3;
                     float big = 0.f;
                     unsigned bad_rows = 0;
                     unsigned char* dst = out + row * 128;
@@ -1495,9 +1494,14 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
     }
     if (KV != 1 && warp == kTreeRawWarp) {
         // --------------------------------------- rows of F32 and int8 pools
-        // Tiles of cached positions by TMA, a lane per box; others row by row
-        // with bulk copies (rows that hold nothing are zero).
+        // Tiles of cached positions by TMA, a lane per box; others in pieces of
+        // 16 bytes, whole rows to an instruction, into the same swizzle (rows
+        // that hold nothing are zero).  Bulk copies of 128 bytes a lane, which
+        // issue one after another and land without the swizzle, were slower (one
+        // tree of 60 nodes on 300 positions, 32/8 heads of 128: F32 53.5 -> 41.2 us,
+        // int8 33.0 -> 30.8; 24 sequences int8 205 -> 196).
         constexpr int kSlabs = F::kBn / 32, kPitch = F::kRawPitch;
+        constexpr int kLanes = F::kRawParts * kPitch / 16, kStep = 32 / kLanes;  // lanes per row, rows per instruction
         bool go = true;
         int raw = 0, flags = 0;
         unsigned empty_phase = 0xffffffffu;
@@ -1542,7 +1546,6 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                         if (!go) break;
                         empty_phase ^= 1u << raw;
                         if (!is_v && lane < 4) M.valid[tile % kMetaRing][lane] = 0xffffffffu;
-                        if (lane == 0) M.swizzled[raw] = 1;
                         __syncwarp();
                         const unsigned full = sm_addr(&M.raw_full[raw]);
                         if (lane == 0)
@@ -1560,7 +1563,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                                 bulk_load(smem + F::kOffScale + ((tile % F::kScaleRing * 2 + is_v) * F::kBn + lane * a.box_rows) * 4,
                                           a.scales + row, a.box_rows * 4, full);
                         }
-                        if constexpr (KV == 2) bar_arrive(&M.raw_full[raw]);
+                        bar_arrive(&M.raw_full[raw]);
                         raw = raw + 1 == F::kRawDepth ? 0 : raw + 1;
                         continue;
                     }
@@ -1576,41 +1579,28 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                 go = __all_sync(0xffffffffu, bar_wait(&M.raw_empty[raw], (empty_phase >> raw) & 1, abort_flag, a.status));
                 if (!go) break;
                 empty_phase ^= 1u << raw;
-                const unsigned dst = F::kOffRaw + raw * F::kRaw;
-                int bytes = 0;
-                if (lane == 0) M.swizzled[raw] = 0;
-#pragma unroll
-                for (int i = 0; i < kSlabs; ++i) {
-                    const long long at = j == k_last ? cur[i] : prev[i];
-                    const unsigned have = __ballot_sync(0xffffffffu, at >= 0);
-                    if (!is_v && lane == 0) M.valid[tile % kMetaRing][i] = have;
-                    if (at < 0)
-#pragma unroll 1
-                        for (int k = 0; k < F::kRawParts * kPitch / 16; ++k)
-                            *reinterpret_cast<uint4*>(tree_smem + dst + (k / (kPitch / 16) * F::kBn + 32 * i + lane) * kPitch +
-                                                      k % (kPitch / 16) * 16) = make_uint4(0, 0, 0, 0);
-                    bytes += __popc(have) * row_bytes;
-                }
-                __syncwarp();
-                const unsigned full = sm_addr(&M.raw_full[raw]);
-                if (lane == 0)
-                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full), "r"(bytes) : "memory");
-                __syncwarp();
+                const unsigned dst = smem + F::kOffRaw + raw * F::kRaw, full = sm_addr(&M.raw_full[raw]);
+                const int ch = lane % kLanes, column = ch % (kPitch / 16);
 #pragma unroll
                 for (int i = 0; i < kSlabs; ++i) {
                     const long long at = j == k_last ? cur[i] : prev[i], row = at + (is_v ? a.kind_rows : 0);
-                    const unsigned to = smem + dst + (32 * i + lane) * kPitch;
-                    if (at >= 0)
-#pragma unroll 1
-                        for (int part = 0; part * kPitch < row_bytes; ++part)
-                            bulk_load(to + part * F::kBn * kPitch, pool + row * row_bytes + part * kPitch,
-                                      min(kPitch, row_bytes - part * kPitch), full);
+                    const unsigned have = __ballot_sync(0xffffffffu, at >= 0);
+                    if (!is_v && lane == 0) M.valid[tile % kMetaRing][i] = have;
                     if constexpr (KV == 2)  // the row's scale, straight into its column
                         cp4(smem + F::kOffScale + ((tile % F::kScaleRing * 2 + is_v) * F::kBn + 32 * i + lane) * 4,
                             at >= 0 ? a.scales + row : a.scales, at >= 0 ? 4u : 0u);
+#pragma unroll 4
+                    for (int r0 = 0; r0 < 32; r0 += kStep) {
+                        const int rr = r0 + lane / kLanes, rt = 32 * i + rr;
+                        const long long from = __shfl_sync(0xffffffffu, row, rr);
+                        const bool ok = (have >> rr & 1) && ch < chunks;
+                        const int swizzle = kPitch == 128 ? rt & 7 : rt >> 1 & 3;
+                        cp16(dst + (ch / (kPitch / 16) * F::kBn + rt) * kPitch + ((column ^ swizzle) << 4),
+                             ok ? pool + from * row_bytes + ch * 16 : pool, ok ? 16u : 0u);
+                    }
                 }
-                if constexpr (KV == 2)
-                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full) : "memory");
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full) : "memory");
+                if (lane == 0) bar_arrive(&M.raw_full[raw]);
                 __syncwarp();
                 raw = raw + 1 == F::kRawDepth ? 0 : raw + 1;
             }
@@ -1620,7 +1610,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
 #pragma unroll 1
         for (int i = 0; i < F::kRawDepth; ++i)
             bar_land(&M.raw_full[i], empty_phase >> i & 1);
-        if (KV == 2) cp_wait<0>();
+        cp_wait<0>();
         if (flags) atomicOr(a.status, flags);
     }
     tm_before();
