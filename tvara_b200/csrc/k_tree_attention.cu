@@ -192,8 +192,8 @@ __global__ void __launch_bounds__(kAnyWarps * 32) tree_any_kernel(TreeAttn a) {
 // 25,000 cycles an item for Q, the pipeline's ends and the output (64 trees
 // over 200-4,000 positions: 265 us, 35% of the copy bandwidth, tensor pipe
 // 49%).  int8 and F32 pools: the conversion warps, whose loads wait behind the
-// MMAs' reads of shared memory (24 sequences int8: 206 us; 31 of the small
-// heads F32: 97 us).  Small calls: instruction fetch; code executed once costs
+// MMAs' reads of shared memory (24 sequences int8: 197 us, 206 sustained; 31
+// of the small heads F32: 89 us).  Small calls: instruction fetch; code executed once costs
 // about a nanosecond per three instructions, so loops here stay rolled unless
 // registers force them open (unrolling everything was 181 KB and 3 times
 // slower on the batch).  Register shares of 200/64/48 or 184/96/48 for softmax,
@@ -223,10 +223,12 @@ struct TreeForm {  // KV: 0 F32, 1 F16, 2 int8
     static constexpr int kSlotPart = kHalves * kBn * 128;
     static constexpr int kSlot = kParts * kSlotPart;     // one K or V tile
     // an item's own cost (Q, merge, output) in tiles, chosen on ragged batches
-    // of each type (64 trees F16 with 4, 6, 8, 11: 248, 244, 231, 233 us; 32
-    // sequences F32 of 128 values with 4, 7, 10: 187, 163, 161 us, 31 of 64
-    // values: 98, 93, 99 us; 24 sequences int8 with 4, 6, 9: 215, 212, 215 us)
-    static constexpr int kItemWeight = KV == 0 ? 7 : KV == 1 ? 8 : 6;
+    // of each type (64 trees F16 with 4, 6, 8, 11: 248, 244, 231, 233 us; F32
+    // heads of 128 with 4, 7, 9: 32 sequences 152, 141, 139 us, 8 sequences 68,
+    // 64, 75; F32 heads of 64 with 3, 4, 7: 31 sequences 88, 86, 93 us, 12
+    // sequences 74, 77, 79; int8 with 5, 6, 7: 24 sequences 197, 195, 199 us,
+    // 64 sequences 62, 66, 68, 16 sequences 63, 66, 63)
+    static constexpr int kItemWeight = KV == 0 ? (DP == 64 ? 3 : 7) : KV == 1 ? 8 : 5;
     static constexpr int kElem = KV == 0 ? 4 : KV == 1 ? 2 : 1;
     static constexpr int kRaw = KV == 1 ? 0 : kBn * DP * kElem;  // one unconverted tile
     static constexpr int kRawPitch = DP * kElem < 128 ? DP * kElem : 128;  // its rows lie in parts of this many bytes,
@@ -1683,6 +1685,9 @@ int tree_ctas() {
 }
 
 constexpr int kTreeMaxCtas = 148, kTreeRecBytes = 8192;
+// Weight of the shortest run: one tree of 26 nodes on 1,900 positions with 2, 3,
+// 4, 6, 10: 28.9, 28.9, 30.5, 30.4, 39.2 us; alike for other small calls.
+constexpr int kTreeMinRun = 2;
 
 template <int KV, int DP>
 void run_tree_mma(const TreeAttn& a, void* workspace, cudaStream_t s) {
@@ -1708,7 +1713,7 @@ void run_tree_mma(const TreeAttn& a, void* workspace, cudaStream_t s) {
                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
             throw std::runtime_error("cuTensorMapEncodeTiled failed for the KV pool");
     }
-    tree_mma_kernel<KV, DP><<<ctas, kTreeThreads, F::kSmem, s>>>(map, job, partial, recs, 2);
+    tree_mma_kernel<KV, DP><<<ctas, kTreeThreads, F::kSmem, s>>>(map, job, partial, recs, kTreeMinRun);
     TVARA_LAUNCHED();
     // launched early; its blocks wait for the first kernel's end (one token F32:
     // 18.5 us in place of 19.7, one tree of 26 nodes F16: 28.9 in place of 31.0)
