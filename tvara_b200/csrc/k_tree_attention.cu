@@ -1114,7 +1114,13 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
         unsigned empty_phase = 0xffffffffu;
         int slot = 0, flags = 0;
         if constexpr (KV == 1) {
-            bool go = true, prev_pair = false;
+            bool go = true;
+            // The extra slots lie in the second Q tile, which a piece with two M
+            // tiles uses until its last output row has been staged there.  `tail` is
+            // the latest such piece that this warp has not seen released yet: it
+            // stays set over any number of pieces that fit the other slots.
+            constexpr unsigned kNoPiece = 0xffffffffu;
+            unsigned tail = kNoPiece;
             int pend[2], n_pend = 0;
             const auto signal = [&](int s) {
                 proxy_fence();
@@ -1132,7 +1138,6 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                 const bool pair = walk.pair;
                 const int ns = pair ? F::kBase : F::kBase + F::kExtra;
                 if (slot >= ns) slot = 0;
-                bool wait_q = prev_pair && !pair;  // extra slots lie in the second Q tile: its last use first
                 const int loads = 2 * (walk.t1 - walk.t0);
                 long long row_cur = -1, row_prev = -1;
                 int k_last = -1;
@@ -1148,11 +1153,19 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                     // entries it is the last or the last but one
                     const long long k_row = j == k_last ? row_cur : row_prev;
                     const unsigned have = __ballot_sync(0xffffffffu, k_row >= 0);
-                    if (slot >= F::kBase && wait_q) {
-                        drain();
-                        go = __all_sync(0xffffffffu, bar_wait(&M.q_full, piece & 1, abort_flag, a.status));
-                        wait_q = false;
-                        if (!go) break;
+                    if (slot >= F::kBase && tail != kNoPiece) {
+                        // Piece `tail` released by every role.  Its phase of the ring's
+                        // barrier is the present or the last one, so the parity says
+                        // which: piece tail - kPieceRing was released before `tail` was
+                        // dealt, and once tail + kPieceRing has been dealt, as this
+                        // warp then knows, nothing is left to wait for.
+                        if (piece - tail < unsigned(kPieceRing)) {
+                            drain();
+                            go = __all_sync(0xffffffffu, bar_wait(&M.piece_empty[tail % kPieceRing], (tail / kPieceRing) & 1,
+                                                                  abort_flag, a.status));
+                            if (!go) break;
+                        }
+                        tail = kNoPiece;
                     }
                     const unsigned parity = (empty_phase >> slot) & 1;
                     if (!__all_sync(0xffffffffu, bar_done(&M.empty[slot], parity))) {
@@ -1243,7 +1256,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                     }
                     slot = slot + 1 == ns ? 0 : slot + 1;
                 }
-                prev_pair = pair;
+                if (pair) tail = piece;
                 if (lane == 0) release_piece(piece);
             }
             drain();
