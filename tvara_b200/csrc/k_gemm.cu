@@ -1696,8 +1696,6 @@ __global__ void __launch_bounds__(kQ4kpThreads, 1)
                         break;
                     }
                     const uint4 w = *reinterpret_cast<const uint4*>(pk_ring + ps * F::kPkBytes + r * 16);
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&pk_empty[ps]);
                     ++pq;
                     if ((p & 7) == 0 && p > 0) {
                         sc_cur = sc_next;
@@ -1743,6 +1741,13 @@ __global__ void __launch_bounds__(kQ4kpThreads, 1)
                     } else {
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     }
+                    // The packed slot goes back only now, when the stores above have
+                    // used the codes: an arrival right behind the load does not wait
+                    // for the load's data, and the next copy (async proxy) then
+                    // overtook the read of single rows while the epilogue kept the
+                    // memory pipe busy (9 of 65 products of 512 tokens were wrong).
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&pk_empty[ps]);
                 } else if (kTmemA) {
                     // min term: this row's 32 split minima of the chunk (qmin_hi on even
                     // steps, qmin_lo on odd ones) into the slot; zero past the row's units
