@@ -1369,9 +1369,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
 #pragma unroll
                             for (int d = kRound; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
                             const int up = lift(top);
-                            const float f = two_to(up), back = two_to(-up);
+                            // a row of zeros has scale 0: with 1 its weight, which is in units of the
+                            // other rows' scales, overflows F16, and inf * 0 is NaN
+                            const float f = two_to(up), back = top > 0.f ? two_to(-up) : 0.f;
                             if (lane < kRound) scale_col[row + round] = back;
-                            big = fmaxf(big, top > 0.f ? back : 0.f);
+                            big = fmaxf(big, back);
                             const f32x2 f2 = pair_of(f, f);
 #pragma unroll
                             for (int i = 0; i < 8; i += 2) {
