@@ -447,7 +447,7 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
     return r;
 }
-__device__ __forceinline__ float two_to(int e) { return __uint_as_float(unsigned(127 + e) << 23); }  // |e| <= 126
+__device__ __forceinline__ float two_to(int e) { return __uint_as_float(unsigned(127 + e) << 23); }  // -126 <= e <= 127
 // The power of two that brings a largest |value| into [2^14, 2^15).
 __device__ __forceinline__ int lift(float top) {
     const int e = int((__float_as_uint(top) >> 23) & 255) - 127;
@@ -818,7 +818,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                         tops[i & 3] = max3(tops[i & 3], fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
                     }
                     const int up = lift(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
-                    c = live ? score_unit * two_to(-up) : 0.f;
+                    // (K scales of F32 rows are 2^14 lower: their product with S must not overflow)
+                    c = live ? score_unit * two_to((KV == 0 ? 14 : 0) - up) : 0.f;
                     const float f = two_to(up);
 #pragma unroll
                     for (int i = 0; i < DP / 8; ++i) {
@@ -929,7 +930,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                         }
                     }
                     const float mn = fmaxf(m, top * c);
-                    float off = mn == -INFINITY ? 11.f : 11.f - mn;
+                    float off = mn == -INFINITY ? 11.f : 11.f - mn, v_unit = 0.f;
                     keep = mn == -INFINITY ? 1.f : ex2(m - mn);
                     m = mn;
                     if constexpr (KV != 1) {
@@ -939,7 +940,26 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                         const float big = fmaxf(fmaxf(vref, fmaxf(big4.x, big4.y)), fmaxf(big4.z, big4.w));
                         keep *= vref / big;
                         vref = big;
-                        off -= __log2f(vref);
+                        v_unit = __log2f(vref);
+                        off -= v_unit;
+                        tm_wait_st();
+                    }
+                    // Beyond 2^22 the reference is so coarse that the exact product
+                    // less it could reach past F16's range: scores rounded to F32,
+                    // less their maximum, go back into S.
+                    if (__any_sync(0xffffffffu, fabsf(mn) >= 4194304.f && mn != -INFINITY)) {
+                        const bool far = fabsf(mn) >= 4194304.f && mn != -INFINITY;
+                        if (far) off = 11.f - v_unit;
+                        const float back = 1.f / c;
+#pragma unroll 1
+                        for (int k = 0; k < F::kBn / 16; ++k) {
+                            unsigned x[16];
+                            tm_ld16(s_at + 16 * k, x);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+                                if (far) x[i] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(x[i]), c), mn) * back);
+                            tm_st16(s_at + 16 * k, x);
+                        }
                         tm_wait_st();
                     }
                     l *= keep;
@@ -1372,7 +1392,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                             // a row of zeros has scale 0: with 1 its weight, which is in units of the
                             // other rows' scales, overflows F16, and inf * 0 is NaN
                             const float f = two_to(up), back = top > 0.f ? two_to(-up) : 0.f;
-                            if (lane < kRound) scale_col[row + round] = back;
+                            if (lane < kRound) scale_col[row + round] = is_v ? back : back * two_to(-14);
                             big = fmaxf(big, back);
                             const f32x2 f2 = pair_of(f, f);
 #pragma unroll
