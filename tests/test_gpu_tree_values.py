@@ -4,6 +4,7 @@ far above or below the others, seen or masked."""
 import numpy as np
 import pytest
 
+from tests import tree_bounds
 from tests import tree_cases as T
 
 pytestmark = pytest.mark.gpu
@@ -45,6 +46,74 @@ def test_all_values_zero(capi, kv):
             set_row(c, s, index, 1, 0, 0.0)
     c.upload().run(capi).check()
     assert (c.dev.get("out")[:c.total, :c.heads * c.d] == 0).all()
+
+
+LARGE = [1e4, 1e8, 1e10, 1e12, 1e20, 1e30]
+
+
+@pytest.mark.parametrize("kv", ["f32", "i8"])
+@pytest.mark.parametrize("large", LARGE)
+def test_masked_node_with_large_values(capi, kv, large):
+    """A node that most rows do not see holds finite V far above the rest."""
+    rng = np.random.default_rng(52)
+    c = T.AttentionCase(rng, kv, [90, 0, 300], [40, 20, 7], 8, 2, 128, masks="any")
+    for s, node in ((0, 7), (0, 33), (1, 2), (2, 6)):
+        length = c.lengths[s]
+        c.mask[s][:, length + node] = False
+        c.mask[s][node, length + node] = True  # itself only
+        row = rng.integers(-127, 128, c.d) if kv == "i8" else rng.standard_normal(c.d) * large
+        for kind in (0, 1):
+            set_row(c, s, length + node, kind, row, large)
+        r = slice(c.cu[s], c.cu[s + 1])
+        c.words[r] = T.mask_words(c.mask[s][:, length:], c.words.shape[1])
+    tree_bounds.check_case(c.upload().run(capi), tree_bounds.rows_and_bound_by_element)
+
+
+def test_masked_node_with_nan_scales(capi):
+    rng = np.random.default_rng(53)
+    c = T.AttentionCase(rng, "i8", [90, 0], [40, 20], 8, 2, 64, masks="any")
+    unseen = []
+    for s, node, scale in ((0, 7, np.nan), (0, 33, np.inf), (1, 2, -np.inf)):
+        c.mask[s][:, c.lengths[s] + node] = False
+        slot = c.slots[c.cu[s] + node]
+        c.scales[slot // c.bt, 1, :, :, slot % c.bt] = scale
+        unseen.append((s, c.lengths[s] + node))
+    for s, index in unseen:
+        c.k[s][:, index] = c.v[s][:, index] = 0
+        c.words[c.cu[s]:c.cu[s + 1]] = T.mask_words(c.mask[s][:, c.lengths[s]:], c.words.shape[1])
+    tree_bounds.check_case(c.upload().run(capi), tree_bounds.rows_and_bound_by_element)
+
+
+@pytest.mark.parametrize("kv", ["f32", "i8"])
+@pytest.mark.parametrize("large", LARGE)
+def test_seen_position_of_large_values_and_no_weight(capi, kv, large):
+    """Cached positions with V far above the rest and scores far below: what
+    they add is small, and the others keep their digits."""
+    rng = np.random.default_rng(54)
+    c = T.AttentionCase(rng, kv, [90, 700], [9, 30], 8, 2, 64)
+    c.q = np.abs(c.q)
+    far = 1.6 * (np.log(large) + 10) / (0.8 * 1.5 * 8)  # scores near -1.6 (ln large + 10)
+    for s, index in ((0, 5), (0, 64), (1, 3), (1, 699)):
+        set_row(c, s, index, 0, -127 if kv == "i8" else -far, far / 127)
+        row = rng.integers(-127, 128, c.d) if kv == "i8" else rng.standard_normal(c.d) * large
+        set_row(c, s, index, 1, row, large / 127)
+    tree_bounds.check_case(c.upload().run(capi), tree_bounds.rows_and_bound_by_element)
+
+
+@pytest.mark.parametrize("q_scale,k_scale,v_scale", [(1e-28, 1e28, 1), (1e28, 1e-28, 1e-20), (1e-20, 1e20, 1e36)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_f32_extreme_magnitudes(capi, q_scale, k_scale, v_scale, d):
+    """Ordinary scores from factors far from one."""
+    rng = np.random.default_rng(56)
+    c = T.AttentionCase(rng, "f32", [300, 20], [20, 33], 8, 2, d, q_scale=q_scale)
+    c.pool[:, :, 0] *= np.float32(k_scale)
+    c.pool[:, :, 1] *= np.float32(v_scale)
+    for s, length in enumerate(c.lengths):
+        p = np.arange(length)
+        slot = np.concatenate([c.tables[s][p // c.bt].astype(np.int64) * c.bt + p % c.bt, c.slots[c.cu[s]:c.cu[s + 1]]])
+        for kind, to in ((0, c.k), (1, c.v)):
+            to[s] = np.moveaxis(c.pool[slot // c.bt, 1, kind, :, slot % c.bt].astype(np.float64), 1, 0)
+    tree_bounds.check_case(c.upload().run(capi), tree_bounds.rows_and_bound_by_element)
 
 
 @pytest.mark.parametrize("kv,q_scale,k_scale", [

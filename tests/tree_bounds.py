@@ -27,7 +27,45 @@ def rows_and_bound(q, k, v, mask, group):
     return out, tol
 
 
-def check_case(case):
+def rows_and_bound_by_element(q, k, v, mask, group):
+    """The same rows, with a bound for F32 and int8 pools that follows each
+    element of K and V, not its row's largest: an element enters as two F16 parts
+    with at most 2^-23 of itself left out (the first part is off by at most 2^-11
+    of the element, the second by 2^-12 of that), and the product of two second
+    parts, at most 2^-22 of the product, is left out.  A row is brought to a
+    largest value in [2^14, 2^15), so what F16 cannot hold, at most 2^-25, is
+    2^-39 of the row's largest.  With 3 d/16 + 1 truncating additions a score is
+    off by at most (3 d/16 + 5) 2^-23 of its sum of |q k|, and by 2^-39 of the
+    rows' largest times the other side's sum.  A weight is off by twice that and
+    2^-22 of the exponential; the weighted sum adds 24 additions' 2^-23 and the
+    parts' 2^-21.  Weight times row scale is below 2^11 and its largest is at
+    least 2^3 (a tile's scales within 2^6 of one another, two references rounded
+    up), where F16 leaves out 2^-25: 2^-28 of the largest weight times row
+    maximum (its power of two at most twice it: 2^-27), of either sign, six
+    deviations of sqrt(m) of them."""
+    import torch
+    n, heads, d = q.shape
+    out, tol = torch.zeros_like(q), torch.zeros_like(q)
+    seen = mask.repeat_interleave(group, 0)
+    some = seen.any(1)
+    for g in range(heads // group):
+        qg = q[:, g * group:(g + 1) * group].reshape(n * group, d)
+        s = (qg @ k[g].T / np.sqrt(d)).masked_fill(~seen, -torch.inf)
+        size = qg.abs() @ k[g].abs().T
+        floor = 2.0 ** -39 * (qg.abs().amax(1)[:, None] * k[g].abs().sum(1) + qg.abs().sum(1)[:, None] * k[g].abs().amax(1))
+        e = (((3 * -(-d // 16) + 5) * 2.0 ** -23 * size + floor) / np.sqrt(d)).masked_fill(~seen, 0.0).amax(1, keepdim=True)
+        w = torch.softmax(s, 1).masked_fill(~some[:, None], 0.0)
+        v_seen = v[g].masked_fill(~mask.any(0)[:, None], 0.0)
+        row = v_seen.abs().amax(1)
+        bound = (w @ v_seen.abs()) * (2 * e + 2.0 ** -22 + 24 * 2.0 ** -23 + 2.0 ** -21) \
+            + 2.0 ** -39 * (w @ row)[:, None] \
+            + 6 * seen.sum(1, keepdim=True).sqrt() * 2.0 ** -27 * (w * row).amax(1, keepdim=True) + 1e-37
+        out[:, g * group:(g + 1) * group] = (w @ v_seen).reshape(n, group, d)
+        tol[:, g * group:(g + 1) * group] = bound.masked_fill(~some[:, None], 0.0).reshape(n, group, d)
+    return out, tol
+
+
+def check_case(case, bound=rows_and_bound):
     """A tree_cases.AttentionCase that has run: every row within its bound, rows
     behind the last sequence as they were, no status bit."""
     import torch
@@ -40,7 +78,7 @@ def check_case(case):
         r = slice(int(case.cu[s]), int(case.cu[s + 1]))
         q = torch.from_numpy(case.q[r, :width].astype(np.float64)).cuda().reshape(n, case.heads, case.d)
         k, v = (torch.from_numpy(np.ascontiguousarray(x[s])).cuda() for x in (case.k, case.v))
-        want, tol = rows_and_bound(q, k, v, torch.from_numpy(case.mask[s]).cuda(), case.heads // case.kv_heads)
+        want, tol = bound(q, k, v, torch.from_numpy(case.mask[s]).cuda(), case.heads // case.kv_heads)
         off = (got[r, :width].reshape(n, case.heads, case.d) - want).abs()
         assert (off <= tol).all(), (s, off.max().item(), (off - tol).max().item())  # NaN is not below its bound
     assert int(case.dev.keep["status"].item()) == 0

@@ -283,7 +283,8 @@ struct TreeMeta {  // at kOffMeta
         long long warp_sum[16];  // while the run is cut out
     };
     alignas(16) unsigned valid[kMetaRing][4];   // columns of a tile that hold a row
-    alignas(16) float vmax[kMetaRing][4];       // largest V scale per load warp
+    alignas(16) unsigned vspan[kMetaRing][4];   // per load warp: the largest V scale (upper half of its bits, rounded
+                                                // up) and the smallest one that is not zero (rounded down)
     union {
         unsigned vbad[kMetaRing][4];  // nodes whose V (kept out of the products: 0 * inf) is not finite
         struct {                      // while the run is cut out
@@ -864,7 +865,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                 }
             }
             float m = -INFINITY, l = 0.f;
-            float vref = 8.0779357e-28f;  // 2^-90: the weights' unit must not overflow
+            float m_v = 0.f;  // O and l are in units of 2^(m + m_v): of the scores, and of the V scales
 #pragma unroll
             for (int i = 0; i < DP; ++i) o[i] = 0.f;
             const int tiles = q.t1 - q.t0;
@@ -929,39 +930,65 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                                 if (seen[k] & M.vbad[ring][k]) l = NAN;  // the row's result is not finite
                         }
                     }
-                    const float mn = fmaxf(m, top * c);
-                    float off = mn == -INFINITY ? 11.f : 11.f - mn, v_unit = 0.f;
-                    keep = mn == -INFINITY ? 1.f : ex2(m - mn);
-                    m = mn;
-                    if constexpr (KV != 1) {
-                        // weights are kept in units of the largest V scale so far,
-                        // in O and l alike: times a V scale they stay below 2^11
-                        const float4 big4 = *reinterpret_cast<const float4*>(M.vmax[ring]);
-                        const float big = fmaxf(fmaxf(vref, fmaxf(big4.x, big4.y)), fmaxf(big4.z, big4.w));
-                        keep *= vref / big;
-                        vref = big;
-                        v_unit = __log2f(vref);
-                        off -= v_unit;
-                        tm_wait_st();
-                    }
+                    // The reference of the weights.  F16: the largest score so far.
+                    // With V scales it has a second part, so that weight times
+                    // scale stays below 2^11 and a row keeps the digits of what
+                    // it sees, whatever the V of others are: the largest score -
+                    // m + log2(V scale).  Where a tile's scales lie within 2^6 of
+                    // one another (zeros apart) its largest score and its largest
+                    // scale together stand for that; elsewhere (a masked node's
+                    // or a single position's V far above the rest) every column
+                    // is looked at.  The weights themselves, which l sums, stay
+                    // below 2^101.  Both parts are whole, so that a change of
+                    // reference costs O and l no digit.
+                    const float score = top * c;
+                    const float mn = fmaxf(m, KV == 1 ? score : ceilf(score));
+                    const bool none = mn == -INFINITY;
                     // Beyond 2^22 the reference is so coarse that the exact product
                     // less it could reach past F16's range: scores rounded to F32,
                     // less their maximum, go back into S.
-                    if (__any_sync(0xffffffffu, fabsf(mn) >= 4194304.f && mn != -INFINITY)) {
-                        const bool far = fabsf(mn) >= 4194304.f && mn != -INFINITY;
-                        if (far) off = 11.f - v_unit;
+                    const bool far = fabsf(mn) >= 4194304.f && !none;
+                    bool look = far;
+                    float mv = -90.f, big = 0.f;
+                    if constexpr (KV != 1) {
+                        const uint4 span = *reinterpret_cast<const uint4*>(M.vspan[ring]);
+                        big = __uint_as_float(max(max(span.x, span.y), max(span.z, span.w)) & 0xffff0000u);
+                        const float low = __uint_as_float(
+                            min(min(span.x & 0xffffu, span.y & 0xffffu), min(span.z & 0xffffu, span.w & 0xffffu)) << 16);
+                        look |= big > 64.f * low;
+                        mv = fmaxf(mv, __log2f(big));
+                        tm_wait_st();
+                    }
+                    if (__any_sync(0xffffffffu, look)) {
                         const float back = 1.f / c;
+                        mv = -90.f;
+                        float most = -INFINITY;
 #pragma unroll 1
                         for (int k = 0; k < F::kBn / 16; ++k) {
                             unsigned x[16];
                             tm_ld16(s_at + 16 * k, x);
 #pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                if (far) x[i] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(x[i]), c), mn) * back);
+                            for (int i = 0; i < 16; ++i) {
+                                const float y = __fsub_rn(__fmul_rn(__uint_as_float(x[i]), c), mn);
+                                if constexpr (KV != 1) most = fmaxf(most, y + __log2f(fabsf(v_scale[16 * k + i])));
+                                if (far) x[i] = __float_as_uint(y * back);
+                            }
                             tm_st16(s_at + 16 * k, x);
                         }
+                        mv = fmaxf(mv, most - (score - mn));
                         tm_wait_st();
                     }
+                    float off = none ? 11.f : far ? 11.f : 11.f - mn;
+                    keep = none ? 1.f : ex2(m - mn);
+                    if constexpr (KV != 1) {
+                        if (!none) {
+                            mv = fmaxf(m_v + (m - mn), ceilf(mv + (score - mn)));
+                            off -= mv;
+                            keep = ex2((m - mn) + (m_v - mv));
+                            m_v = mv;
+                        }
+                    }
+                    m = mn;
                     l *= keep;
                     // P over S, sixteen positions (one K step of the MMA) at a
                     // time: hi in their first eight columns, lo in the others.
@@ -1026,7 +1053,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                 }
             }
             if (!go) break;
-            if constexpr (KV != 1) m += __log2f(vref);  // the unit of O and l joins their reference
+            if constexpr (KV != 1) m += m_v;
             // The part of an item that other CTAs continue: (O, m, l) of each
             // stream into the workspace, one thread a row, rows side by side.
             // The CTA's slot 1 holds an item that begins here, slot 0 one that
@@ -1321,7 +1348,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                     unsigned char* out = tree_smem + slot_at(slot);
                     unsigned char* src = tree_smem + F::kOffRaw + raw * F::kRaw + row * F::kRawPitch;
                     const int swizzle = F::kRawPitch == 128 ? row & 7 : row >> 1 & 3;
-                    float big = 0.f;
+                    float big = 0.f, low = INFINITY;
                     unsigned bad_rows = 0;
                     unsigned char* dst = out + row * 128;
                     if constexpr (KV == 2) {
@@ -1331,6 +1358,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                             if (bad) scale_col[row] = sc = 0.f;
                             bad_rows = __ballot_sync(0xffffffffu, bad);
                             big = fabsf(sc);
+                            if (big > 0.f) low = big;
                         }
                         uint4 row_codes[DP / 16];  // all read before any is written: no load waits behind a store
 #pragma unroll
@@ -1394,6 +1422,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                             const float f = two_to(up), back = top > 0.f ? two_to(-up) : 0.f;
                             if (lane < kRound) scale_col[row + round] = is_v ? back : back * two_to(-14);
                             big = fmaxf(big, back);
+                            if (back > 0.f) low = fminf(low, back);
                             const f32x2 f2 = pair_of(f, f);
 #pragma unroll
                             for (int i = 0; i < 8; i += 2) {
@@ -1417,8 +1446,12 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                                 reinterpret_cast<unsigned short*>(M.vbad[meta])[lw] = (unsigned short)bad_rows;
                         }
 #pragma unroll
-                        for (int d = 16; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
-                        if (lane == 0) M.vmax[meta][lw] = big;
+                        for (int d = 16; d; d >>= 1) {
+                            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
+                            low = fminf(low, __shfl_xor_sync(0xffffffffu, low, d));
+                        }
+                        if (lane == 0)
+                            M.vspan[meta][lw] = ((__float_as_uint(big) + 0xffffu) & 0xffff0000u) | __float_as_uint(low) >> 16;
                     }
                     proxy_fence();
                     __syncwarp();
