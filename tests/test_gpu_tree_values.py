@@ -151,3 +151,23 @@ def test_scores_of_any_size(capi, kv, q_scale, k_scale, d):
                     # hi + lo parts: 2^-21 of the element (V and weight), 2^-23 of the row's largest
                     assert (np.abs(row - want) <= 2.0 ** -20 * np.abs(want) + 2.0 ** -23 * np.abs(want).max()).all()
     assert clear > 300
+
+
+@pytest.mark.parametrize("times", [300, 3000])
+@pytest.mark.parametrize("side", ["k", "v", "both"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_f32_outlier_channel(capi, times, side, d):
+    """One channel far above the others, as keys of trained models have: the
+    other channels keep the digits of their own size."""
+    rng = np.random.default_rng(55)
+    lengths, nodes = [0, 2, 40, 300], [1, 1, 20, 30]
+    c = T.AttentionCase(rng, "f32", lengths, nodes, 8, 2, d, q_scale=0.01 if side == "v" else 1.5)
+    c.q.reshape(-1, 8, d)[:, :, 5] /= times  # scores stay ordinary
+    for kind, name, to in ((0, "k", c.k), (1, "v", c.v)):
+        if side in (name, "both"):
+            c.pool[:, :, kind, ..., 5] *= np.float32(times)
+            for s, length in enumerate(lengths):
+                p = np.arange(length)
+                slot = np.concatenate([c.tables[s][p // c.bt].astype(np.int64) * c.bt + p % c.bt, c.slots[c.cu[s]:c.cu[s + 1]]])
+                to[s] = np.moveaxis(c.pool[slot // c.bt, 1, kind, :, slot % c.bt].astype(np.float64), 1, 0)
+    tree_bounds.check_case(c.upload().run(capi), tree_bounds.rows_and_bound_by_element)

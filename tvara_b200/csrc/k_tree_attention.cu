@@ -484,8 +484,11 @@ __device__ __forceinline__ void mul2_in(unsigned& x, unsigned& y, f32x2 f) {
     y = __float_as_uint(v);
 }
 // A pair of values below 2^16 as hi + lo, F16 each: hi is the value rounded to
-// 11 bits and lo what is left, so hi + lo carries 2^-22 of each value (not of
-// the largest: small softmax weights keep their digits), down to 2^-25 absolute.
+// 11 bits and lo what is left, so hi + lo carries 2^-23 of each value (not of
+// the largest: small softmax weights, and the other channels of a K or V row
+// with a large one, keep their digits), down to 2^-25 absolute.  (A split in
+// packed additions alone, lo in steps of the row's largest, is no faster: F32
+// heads of 64 89.8 and 89.6 us, of 128 140.8 and 142.3.)
 __device__ __forceinline__ void split_pair(float x, float y, unsigned& hi, unsigned& lo) {
     const __half2 h = __floats2half2_rn(x, y);
     const float2 f = __half22float2(h);
@@ -493,21 +496,7 @@ __device__ __forceinline__ void split_pair(float x, float y, unsigned& hi, unsig
     hi = *reinterpret_cast<const unsigned*>(&h);
     lo = *reinterpret_cast<const unsigned*>(&l);
 }
-// A pair below 2^15 as hi (a multiple of 16) + lo (|lo| <= 8): 2^-9 absolute,
-// in three packed additions.  Enough for K and V of F32 rows, whose largest
-// value lies in [2^14, 2^15); the products of their lo with that of Q or P,
-// which are left out, are 2^-23 of the value.
-__device__ __forceinline__ void split_fixed(f32x2 x, unsigned& hi, unsigned& lo) {
-    const f32x2 up = pair_of(201326592.f, 201326592.f), down = pair_of(-201326592.f, -201326592.f);  // 1.5 * 2^27
-    const f32x2 h = add2(add2(x, up), down), r = fma2(h, pair_of(-1.f, -1.f), x);
-    float a, b, c, d;
-    halves_of(h, a, b);
-    halves_of(r, c, d);
-    const __half2 hh = __floats2half2_rn(a, b), ll = __floats2half2_rn(c, d);
-    hi = *reinterpret_cast<const unsigned*>(&hh);
-    lo = *reinterpret_cast<const unsigned*>(&ll);
-}
-__device__ __forceinline__ void split_weight(f32x2 p, unsigned& hi, unsigned& lo) {
+__device__ __forceinline__ void split_packed(f32x2 p, unsigned& hi, unsigned& lo) {
     float x, y;
     halves_of(p, x, y);
     split_pair(x, y, hi, lo);
@@ -1021,8 +1010,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                                     p = mul2(p, f.x);
                                     r2 = mul2(r2, f.y);
                                 }
-                                split_weight(p, y[i], y[8 + i]);
-                                split_weight(r2, y[i + 1], y[9 + i]);
+                                split_packed(p, y[i], y[8 + i]);
+                                split_packed(r2, y[i + 1], y[9 + i]);
                             }
                             tm_st16(s_at + 32 * k + 16 * g, y);
                         }
@@ -1427,10 +1416,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
 #pragma unroll
                             for (int i = 0; i < 8; i += 2) {
                                 uint4 hi, lo;
-                                split_fixed(mul2(pair_of(__uint_as_float(quads[i].x), __uint_as_float(quads[i].y)), f2), hi.x, lo.x);
-                                split_fixed(mul2(pair_of(__uint_as_float(quads[i].z), __uint_as_float(quads[i].w)), f2), hi.y, lo.y);
-                                split_fixed(mul2(pair_of(__uint_as_float(quads[i + 1].x), __uint_as_float(quads[i + 1].y)), f2), hi.z, lo.z);
-                                split_fixed(mul2(pair_of(__uint_as_float(quads[i + 1].z), __uint_as_float(quads[i + 1].w)), f2), hi.w, lo.w);
+                                split_packed(mul2(pair_of(__uint_as_float(quads[i].x), __uint_as_float(quads[i].y)), f2), hi.x, lo.x);
+                                split_packed(mul2(pair_of(__uint_as_float(quads[i].z), __uint_as_float(quads[i].w)), f2), hi.y, lo.y);
+                                split_packed(mul2(pair_of(__uint_as_float(quads[i + 1].x), __uint_as_float(quads[i + 1].y)), f2), hi.z, lo.z);
+                                split_packed(mul2(pair_of(__uint_as_float(quads[i + 1].z), __uint_as_float(quads[i + 1].w)), f2), hi.w, lo.w);
                                 const int hc = part * 4 + i / 2;  // 16-byte chunk of the F16 row
                                 unsigned char* at = dst + round * 128 + (hc >> 3) * (F::kBn * 128) + (((hc & 7) ^ f16_swizzle) << 4);
                                 *reinterpret_cast<uint4*>(at) = hi;
