@@ -168,11 +168,11 @@ TVARA_API int tvara_paged_attention_noalloc(const tvara_attention_args* args, vo
 enum {
     TVARA_TREE_BAD_BLOCK = 1,   /* a block id or slot outside the pool; its row is not read or written (in the
                                    attention it counts as masked) */
-    TVARA_TREE_BAD_LENGTHS = 2, /* negative or decreasing cu_nodes, more rows than capacity, more nodes than
-                                   max_nodes, a negative length, a sequence longer than its table row, a count of
-                                   free blocks outside [0, free_capacity], or held blocks that are fewer than the
-                                   cached positions need: the plan writes nothing, the other calls skip the
-                                   sequence */
+    TVARA_TREE_BAD_LENGTHS = 2, /* cu_nodes that are negative, decrease or do not begin with 0, more rows than
+                                   capacity, more nodes than max_nodes, a negative length, a sequence longer than
+                                   its table row (with or without rows of its own), a count of free blocks outside
+                                   [0, free_capacity], or held blocks that are fewer than the cached positions need:
+                                   the plan writes nothing, the other calls skip the sequence */
     TVARA_TREE_NO_BLOCKS = 4,   /* the plan needs more blocks than are free: it writes nothing */
     TVARA_TREE_BAD_PARENT = 8,  /* a parent that is not an earlier node: the plan treats the node as a root, the
                                    commit never accepts it */

@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(TreeCommit 
     // (lengths_out may be lengths: other slices see either value, and only ask whether it is negative)
     const int c0 = a.cu[s], c1 = a.cu[s + 1], len = a.lengths[s];
     const long long n64 = (long long)c1 - c0;
-    if (c0 < 0 || n64 < 0 || n64 > a.max_nodes || c1 > a.capacity || len < 0) {
+    if (c0 < 0 || n64 < 0 || n64 > a.max_nodes || c1 > a.capacity || c1 > a.cu[a.n_seq] || len < 0) {
         if (blockIdx.y == 0 && tid == 0) atomicOr(a.status, kTreeBadLengths);
         return;
     }
@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(TreeCommit 
     const int parent0 = tid < n ? a.parents[c0 + tid] : 0;
     const unsigned token0 = tid < n ? a.tokens[c0 + tid] : 0;
     __syncthreads();
-    int flags = 0;
+    int flags = s == 0 && c0 != 0 ? kTreeBadLengths : 0;
     for (int i = tid; i < n; i += kCommitThreads) {
         const int p = i == tid ? parent0 : a.parents[c0 + i];
         if (p < -1 || p >= i) {

@@ -15,16 +15,21 @@
 namespace tvara {
 namespace {
 
-// The sequence of row t: the last one whose rows begin at or before it.
-// False when the row belongs to none or its sequence's sizes are invalid.
+// Rows, node count and length of sequence s; false when they are invalid.
 __device__ __forceinline__ bool tree_sequence_ok(const TreeAttn& a, int s, int& c0, int& n, int& len) {
     c0 = a.cu[s];
-    const int c1 = a.cu[s + 1];
+    const int c1 = a.cu[s + 1], end = a.cu[a.n_seq];  // rows from `end` on are no sequence's
     len = a.lengths[s];
     const long long rows = (long long)c1 - c0;
     n = int(rows);
-    return c0 >= 0 && rows >= 0 && rows <= a.max_nodes && c1 <= a.capacity && len >= 0 &&
+    return c0 >= 0 && rows >= 0 && rows <= a.max_nodes && c1 <= a.capacity && c1 <= end && len >= 0 &&
            len <= (long long)a.stride * a.bt && len <= 0x7fffffff - 2 * kTreeMaxNodes;
+}
+
+// What every form reports about sequence s, rows or not.
+__device__ __forceinline__ bool tree_reported(const TreeAttn& a, int s) {
+    int c0, n, len;
+    return !tree_sequence_ok(a, s, c0, n, len) || (s == 0 && c0 != 0);
 }
 
 // x / bt for x < 2^44 by the reciprocal 2^64 / bt rounded up (0 stands for
@@ -74,6 +79,11 @@ __global__ void __launch_bounds__(kAnyWarps * 32) tree_any_kernel(TreeAttn a) {
     __shared__ float sm_m[kAnyWarps], sm_l[kAnyWarps];
     __shared__ float sm_acc[kAnyWarps][E * 32];
     const int t = blockIdx.x, h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (t == 0 && h == 0) {  // sizes are reported by sequence: an empty one has no row here
+        bool bad = false;
+        for (int s = threadIdx.x; s < a.n_seq; s += kAnyWarps * 32) bad |= tree_reported(a, s);
+        if (__syncthreads_or(bad) && threadIdx.x == 0) atomicOr(a.status, kTreeBadLengths);
+    }
     if (t >= a.cu[a.n_seq]) return;
     int lo = 0, hi = a.n_seq;
     while (hi - lo > 1) {
@@ -84,10 +94,21 @@ __global__ void __launch_bounds__(kAnyWarps * 32) tree_any_kernel(TreeAttn a) {
             hi = mid;
     }
     int c0, n, len, flags = 0;
-    const bool ok = tree_sequence_ok(a, lo, c0, n, len);
-    if (!ok || t < c0 || t - c0 >= n) {
-        if (threadIdx.x == 0 && h == 0) atomicOr(a.status, kTreeBadLengths);
-        return;
+    const auto holds = [&](int s) { return tree_sequence_ok(a, s, c0, n, len) && t >= c0 && t - c0 < n; };
+    if (!holds(lo)) {
+        // a row of no sequence, or one that the search missed among sizes that
+        // do not ascend: of the valid sequences that hold it, the last
+        __shared__ int holder;
+        if (threadIdx.x == 0) holder = -1;
+        __syncthreads();
+        int mine = -1;
+        for (int s = threadIdx.x; s < a.n_seq; s += kAnyWarps * 32)
+            if (holds(s)) mine = s;
+        if (mine >= 0) atomicMax(&holder, mine);
+        __syncthreads();
+        lo = holder;
+        if (lo < 0) return;
+        holds(lo);
     }
     const int node = t - c0, g = h / a.group;
     const unsigned long long* mask = a.ancestors ? a.ancestors + (long long)t * a.words : nullptr;
@@ -518,9 +539,10 @@ struct TreeSeq {
 template <class F>
 __device__ __forceinline__ bool tree_seq(const TreeAttn& a, int s, TreeSeq& q) {
     q.s = s;
-    if (!tree_sequence_ok(a, s, q.c0, q.n, q.len) || q.n == 0) {
+    const bool ok = tree_sequence_ok(a, s, q.c0, q.n, q.len);
+    if (!ok || q.n == 0) {
         q.total = 0;
-        return q.n == 0;
+        return ok && !(s == 0 && q.c0 != 0);
     }
     const int vectors = q.n * a.group;
     const int most = F::kPairs ? 256 : 128;
@@ -529,7 +551,7 @@ __device__ __forceinline__ bool tree_seq(const TreeAttn& a, int s, TreeSeq& q) {
     q.weight = q.pair ? 2 : 1;
     q.tiles = (unsigned(q.len) + unsigned(q.n) + F::kBn - 1) / F::kBn;
     q.total = q.tiles * q.groups * a.hkv;
-    return true;
+    return !(s == 0 && q.c0 != 0);
 }
 
 // Bits [j0, j0 + 32) of the mask row of node `node` (negative j0: cached
