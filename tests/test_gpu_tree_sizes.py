@@ -6,6 +6,7 @@ import pytest
 
 from tests import tree_cases as T
 from tests.test_gpu_tree import commit_case
+from tvara_b200 import _bindings as B
 
 pytestmark = pytest.mark.gpu
 
@@ -96,3 +97,32 @@ def test_commit_skips_and_reports_the_same(capi, edit, skipped):
         elif edit != (0, 1):
             assert np.array_equal(dev.get("path")[r], path[r])
             assert all(dev.get(name)[s] == answers[name][s] for name in answers)
+
+
+@pytest.mark.parametrize("bt", [1 << 20, 1])
+def test_plan_of_nearly_two_to_the_31_rows(capi, bt):
+    """Row (and, with blocks of one position, block) counts at the end of 32 bits."""
+    import torch
+    rows = 0x7fffffff
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB of device memory")
+    blocks = -(-rows // bt)
+    free = torch.arange(blocks - 1, -1, -1, dtype=torch.int32, device="cuda")  # so that block j of the sequence is j
+    d = T.Dev(B.TreePlanArgs, block_tokens=bt, n_seq=2, capacity=rows, max_nodes=1, max_blocks=blocks, table_stride=blocks,
+              free_capacity=blocks)
+    d.set(lengths=np.zeros(2, np.int32), held=np.zeros(2, np.int32), cu_nodes=np.array([0, rows, rows], np.int32),
+          free_blocks=free, free_count=np.array([blocks], np.int32), held_out=np.zeros(2, np.int32),
+          free_left=np.zeros(1, np.int32), status=np.zeros(1, np.int32),
+          tables=torch.full((2 * blocks,), -1, dtype=torch.int32, device="cuda"),
+          slots=torch.full((rows,), -1, dtype=torch.int64, device="cuda"),
+          positions=torch.full((rows,), -1, dtype=torch.int32, device="cuda"))
+    assert capi.tvara_tree_plan(d.by, None) == 0, capi.tvara_last_error()
+    assert d.get("status")[0] == 0 and d.get("held_out").tolist() == [blocks, 0] and d.get("free_left")[0] == 0
+    assert torch.equal(d.keep["tables"][:blocks], torch.arange(blocks, dtype=torch.int32, device="cuda"))
+    assert (d.keep["tables"][blocks:] == -1).all()
+    for at in range(0, rows, 1 << 27):
+        want = torch.arange(at, min(at + (1 << 27), rows), device="cuda")
+        assert torch.equal(d.keep["slots"][at:at + (1 << 27)], want)
+        assert torch.equal(d.keep["positions"][at:at + (1 << 27)], want.int())
+    d.keep.clear()
+    torch.cuda.empty_cache()

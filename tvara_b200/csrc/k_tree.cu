@@ -107,7 +107,8 @@ __global__ void __launch_bounds__(kPlanThreads) tree_plan_kernel(TreePlan a, int
     }
     if (!(mode & kPlanRows)) return;
     int flags = 0;
-    for (int j = at; j < fresh; j += step) {
+    for (long long at_new = at; at_new < fresh; at_new += step) {  // (fresh may be near 2^31, as total below)
+        const int j = int(at_new);
         // first_s repeats over sequences that need nothing: the last of equal
         // entries is the one that takes block j
         const int s = last_at_most(first_s, a.n_seq, j);
@@ -126,9 +127,10 @@ __global__ void __launch_bounds__(kPlanThreads) tree_plan_kernel(TreePlan a, int
         return p;
     };
     if (!a.parents) {
-        for (int t0 = at * kPlanRun; t0 < total; t0 += step * kPlanRun) {
-            int s = last_at_most(cu_s, a.n_seq, t0), len = a.lengths[s], held = a.held[s];
-            for (int t = t0; t < min(t0 + kPlanRun, total); ++t) {
+        for (long long t0 = at * kPlanRun; t0 < total; t0 += step * kPlanRun) {
+            int s = last_at_most(cu_s, a.n_seq, int(t0)), len = a.lengths[s], held = a.held[s];
+            const int behind = int(min(t0 + kPlanRun, (long long)total));
+            for (int t = int(t0); t < behind; ++t) {
                 while (t >= cu_s[s + 1]) {
                     ++s;
                     len = a.lengths[s];
@@ -337,7 +339,7 @@ void launch_tree_plan(const TreePlan& a, cudaStream_t s) {
     const std::size_t smem = std::size_t(a.n_seq + 1) * 8 + (a.parents ? (kPlanThreads + kTreeMaxNodes) * 4 : 0);
     if (smem > 48 * 1024)
         TVARA_CUDA(cudaFuncSetAttribute(tree_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
-    const long long most = std::max<long long>(a.parents ? a.capacity : (a.capacity + kPlanRun - 1) / kPlanRun, a.n_seq);
+    const long long most = std::max<long long>(a.parents ? a.capacity : (a.capacity + kPlanRun - 1ll) / kPlanRun, a.n_seq);
     const int grid = int(std::clamp<long long>((most + kPlanThreads - 1) / kPlanThreads, 1, 296));
     // counts written over their own inputs wait until no CTA reads these
     const bool in_place = a.held_out == a.held || a.free_left == a.free_count;
