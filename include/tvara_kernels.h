@@ -188,8 +188,9 @@ enum {
  * row; row i gets the slot of position lengths[s] + i.  positions[i] is
  * lengths[s] + depth of node i (roots have depth 0) and bit j of row i of
  * ancestors says that node j is node i or one of its ancestors.  held_out and
- * free_left may be held and free_count themselves; the free list is only
- * read, its first *free_left entries stay free. */
+ * free_left may be held and free_count themselves (a second small launch then
+ * writes them); no output may overlap another array otherwise.  The free list
+ * is only read, its first *free_left entries stay free. */
 typedef struct tvara_tree_plan_args {
     uint32_t struct_size;         /* sizeof(tvara_tree_plan_args) */
     uint32_t block_tokens;
@@ -219,8 +220,9 @@ TVARA_API int tvara_tree_plan(const tvara_tree_plan_args* args, void* stream);
  * h / (heads / kv_heads), arithmetic and outputs are F32 to within rounding
  * for every pool type (as tvara_paged_attention).  A row that attends to
  * nothing is zero; masked K and V may hold anything, NaN included.  Rows of
- * out may not meet rows of q (column slices of one buffer are fine).  One
- * workspace serves one call at a time. */
+ * out may not meet rows of q (column slices of one buffer are fine), and out,
+ * workspace and status no other array.  One workspace serves one call at a
+ * time. */
 typedef struct tvara_tree_attention_args {
     uint32_t struct_size;         /* sizeof(tvara_tree_attention_args) */
     uint32_t kv_dtype;            /* TVARA_KV_F32, TVARA_KV_F16 or TVARA_KV_I8 (needs kv_scales) */
@@ -255,7 +257,9 @@ TVARA_API int tvara_tree_attention(const tvara_tree_attention_args* args, void* 
  * k-th accepted node, -1 behind the last; accepted[s] counts them; next[s] is
  * the choice the walk ended with (0xFFFFFFFF when there is none), and may be
  * first itself; lengths_out[s] = lengths[s] + accepted[s], and may be lengths
- * itself.  No other output may overlap an input.
+ * itself (with next over first and a pool, a second small launch writes the
+ * answers).  No output, the pool among them, may overlap another array
+ * otherwise.
  * With a pool, the K and V rows of the k-th accepted node (every layer and KV
  * head, int8 scales too) are copied from its slot to dest[cu_nodes[s] + k];
  * dest NULL means slots: the drafts were written behind the cached positions,

@@ -353,9 +353,33 @@ void check_tree_sizes(std::size_t n_seq, std::size_t capacity, std::size_t max_n
         throw std::invalid_argument("invalid KV pool size");
 }
 
-bool overlap(const void* a, std::size_t na, const void* b, std::size_t nb) {
-    const auto x = reinterpret_cast<std::uintptr_t>(a), y = reinterpret_cast<std::uintptr_t>(b);
-    return x < y + nb && y < x + na;
+using wide = unsigned __int128;
+
+// An array of a call, [from, to): `as`, where given, is the output that may be
+// this very array.  One that would reach past the end of memory ends there.
+struct Span {
+    std::uintptr_t from, to, as;
+    Span(const void* at, wide bytes, const void* as_output = nullptr)
+        : from(bytes ? reinterpret_cast<std::uintptr_t>(at) : 0), to(from), as(reinterpret_cast<std::uintptr_t>(as_output)) {
+        if (from) to = bytes > ~from ? ~std::uintptr_t(0) : from + std::uintptr_t(bytes);
+    }
+};
+
+// What a call writes may be neither what it reads nor what else it writes: its
+// CTAs read and write in any order.
+void check_apart(std::initializer_list<Span> outs, std::initializer_list<Span> ins, const char* text) {
+    bool met = false;
+    for (const Span* o = outs.begin(); o != outs.end(); ++o) {
+        for (const Span* other = o + 1; other != outs.end(); ++other) met |= o->from < other->to && other->from < o->to;
+        for (const Span& in : ins)
+            met |= o->from < in.to && in.from < o->to && !(in.as && o->from == in.as && in.from == in.as);
+    }
+    if (met) throw std::invalid_argument(text);
+}
+
+// Rows of `width` elements, `stride` apart.
+wide rows_span(std::size_t rows, std::size_t stride, std::size_t width, std::size_t elem) {
+    return rows ? ((wide(rows) - 1) * stride + width) * elem : 0;
 }
 
 // Arrays are read by their own types; an address off by half of one would fault on the device.
@@ -368,7 +392,6 @@ void check_aligned(std::size_t bytes, std::initializer_list<const void*> arrays)
 // of one may meet a row of the other; column slices of one buffer are apart.
 bool rows_overlap(const float* q, std::size_t q_stride, const float* out, std::size_t out_stride, std::size_t rows,
                   std::size_t width) {
-    using wide = unsigned __int128;
     const wide x = reinterpret_cast<std::uintptr_t>(q), y = reinterpret_cast<std::uintptr_t>(out);
     const wide nx = ((wide(rows) - 1) * q_stride + width) * 4, ny = ((wide(rows) - 1) * out_stride + width) * 4;
     if (x >= y + ny || y >= x + nx) return false;
@@ -439,13 +462,21 @@ int tvara_tree_plan(const tvara_tree_plan_args* a, void* stream) {
             throw std::invalid_argument("parents and ancestor masks go together");
         if (!a->table_stride || a->table_stride > 0x7fffffff || a->free_capacity > 0x7fffffff)
             throw std::invalid_argument("invalid block table width or free list");
-        const std::size_t counts = a->n_seq * 4;
-        if ((a->held_out != a->held && overlap(a->held_out, counts, a->held, counts)) ||
-            overlap(a->held_out, counts, a->lengths, counts) || overlap(a->free_left, 4, a->held, counts) ||
-            overlap(a->held_out, counts, a->free_count, 4) || overlap(a->held_out, counts, a->cu_nodes, counts + 4) ||
-            overlap(a->free_left, 4, a->lengths, counts) || overlap(a->free_left, 4, a->cu_nodes, counts + 4) ||
-            (a->free_left != a->free_count && overlap(a->free_left, 4, a->free_count, 4)))
-            throw std::invalid_argument("plan outputs overlap its inputs");
+        const wide counts = wide(a->n_seq) * 4, rows = a->capacity;
+        check_apart({{a->tables, wide(a->n_seq) * a->table_stride * 4},
+                     {a->slots, rows * 8},
+                     {a->positions, rows * 4},
+                     {a->ancestors, rows * ((max_nodes + 63) / 64) * 8},
+                     {a->held_out, counts},
+                     {a->free_left, 4},
+                     {a->status, 4}},
+                    {{a->lengths, counts},
+                     {a->held, counts, a->held_out},
+                     {a->cu_nodes, counts + 4},
+                     {a->parents, rows * 4},
+                     {a->free_blocks, wide(a->free_capacity) * 4},
+                     {a->free_count, 4, a->free_left}},
+                    "plan outputs overlap its inputs or one another");
         check_aligned(4, {a->lengths, a->held, a->cu_nodes, a->parents, a->free_blocks, a->free_count, a->tables,
                           a->positions, a->held_out, a->free_left, a->status});
         check_aligned(8, {a->slots, a->ancestors});
@@ -499,6 +530,19 @@ int tvara_tree_attention(const tvara_tree_attention_args* a, void* workspace, si
             throw std::invalid_argument("attention workspace too small");
         if (reinterpret_cast<std::uintptr_t>(workspace) % 16) throw std::invalid_argument("attention workspace is not 16-byte aligned");
         if (!a->capacity) return;
+        const std::size_t elem = j.kv_kind == 0 ? 4 : j.kv_kind == 1 ? 2 : 1, width = std::size_t(a->heads) * a->head_dim;
+        const wide pool_rows = wide(j.max_blocks) * j.block_rows;
+        const Span q{a->q, rows_span(a->capacity, a->q_stride, width, 4)}, out{a->out, rows_span(a->capacity, a->out_stride, width, 4)},
+            work{workspace, tvara::tree_attention_workspace(j)};
+        const std::initializer_list<Span> ins{{a->pool, pool_rows * a->head_dim * elem},
+                                              {j.scales, pool_rows * 4},
+                                              {a->tables, wide(a->n_seq) * a->table_stride * 4},
+                                              {a->lengths, wide(a->n_seq) * 4},
+                                              {a->cu_nodes, wide(a->n_seq) * 4 + 4},
+                                              {a->slots, wide(a->capacity) * 8},
+                                              {a->ancestors, wide(a->capacity) * j.words * 8}};
+        check_apart({out, work, {a->status, 4}}, ins, "attention outputs or workspace overlap its inputs or one another");
+        check_apart({work, {a->status, 4}}, {q}, "attention workspace or status overlap the query rows");
         tvara::launch_tree_attention(j, workspace, static_cast<cudaStream_t>(stream));
     });
 }
@@ -511,20 +555,23 @@ int tvara_tree_commit(const tvara_tree_commit_args* a, void* stream) {
         if (!a->lengths || !a->cu_nodes || !a->accepted || !a->next || !a->lengths_out || !a->status ||
             (a->capacity && (!a->parents || !a->tokens || !a->choices || !a->path)))
             throw std::invalid_argument("invalid tree commit arguments");
-        const std::size_t per_seq = a->n_seq * 4;
-        const void* outs[] = {a->accepted, a->next, a->lengths_out};
-        for (const void* out : outs) {
-            // next may be first, lengths_out may be lengths; anything else would change what the walk reads
-            const bool over = overlap(out, per_seq, a->cu_nodes, per_seq + 4) ||
-                              (a->first && out != (out == a->next ? a->first : nullptr) && overlap(out, per_seq, a->first, per_seq)) ||
-                              (out != (out == a->lengths_out ? a->lengths : nullptr) && overlap(out, per_seq, a->lengths, per_seq));
-            if (over) throw std::invalid_argument("commit outputs overlap its inputs");
-        }
-        const std::size_t per_row = a->capacity * 4;
-        for (const void* in : std::initializer_list<const void*>{a->parents, a->tokens, a->choices})
-            if (a->capacity && (overlap(a->path, per_row, in, per_row) || overlap(a->accepted, per_seq, in, per_row) ||
-                                overlap(a->next, per_seq, in, per_row) || overlap(a->lengths_out, per_seq, in, per_row)))
-                throw std::invalid_argument("commit outputs overlap its inputs");
+        const wide per_seq = wide(a->n_seq) * 4, rows = a->capacity;
+        // next may be first, lengths_out may be lengths; anything else would
+        // change what the walk or the move, repeated by every slice, reads
+        check_apart({{a->path, rows * 4},
+                     {a->accepted, per_seq},
+                     {a->next, per_seq},
+                     {a->lengths_out, per_seq},
+                     {a->status, 4}},
+                    {{a->lengths, per_seq, a->lengths_out},
+                     {a->cu_nodes, per_seq + 4},
+                     {a->parents, rows * 4},
+                     {a->tokens, rows * 4},
+                     {a->choices, rows * 4},
+                     {a->first, per_seq, a->next},
+                     {a->pool ? a->slots : nullptr, rows * 8},
+                     {a->pool ? a->dest : nullptr, rows * 8}},
+                    "commit outputs overlap its inputs or one another");
         check_aligned(4, {a->lengths, a->cu_nodes, a->parents, a->tokens, a->choices, a->first, a->path, a->accepted,
                           a->next, a->lengths_out, a->status});
         tvara::TreeCommit j;
@@ -548,6 +595,13 @@ int tvara_tree_commit(const tvara_tree_commit_args* a, void* stream) {
             j.slots = reinterpret_cast<const long long*>(a->slots);
             j.dest = reinterpret_cast<const long long*>(a->dest);
             check_aligned(4, {j.scales});
+            const wide pool_rows = wide(a->max_blocks) * a->block_tokens * a->layers * 2 * a->kv_heads;
+            check_apart({{a->pool, pool_rows * a->head_dim * j.elem}, {j.scales, pool_rows * 4}},
+                        {{a->lengths, per_seq}, {a->cu_nodes, per_seq + 4}, {a->parents, rows * 4}, {a->tokens, rows * 4},
+                         {a->choices, rows * 4}, {a->first, per_seq}, {a->slots, rows * 8}, {a->dest, rows * 8},
+                         {a->path, rows * 4}, {a->accepted, per_seq}, {a->next, per_seq}, {a->lengths_out, per_seq},
+                         {a->status, 4}},
+                        "the KV pool overlaps the commit's other arrays");
         }
         j.n_seq = int(a->n_seq);
         j.capacity = int(a->capacity);
