@@ -171,3 +171,29 @@ def test_f32_outlier_channel(capi, times, side, d):
                 slot = np.concatenate([c.tables[s][p // c.bt].astype(np.int64) * c.bt + p % c.bt, c.slots[c.cu[s]:c.cu[s + 1]]])
                 to[s] = np.moveaxis(c.pool[slot // c.bt, 1, kind, :, slot % c.bt].astype(np.float64), 1, 0)
     tree_bounds.check_case(c.upload().run(capi), tree_bounds.rows_and_bound_by_element)
+
+
+@pytest.mark.parametrize("kv,scale", [("f32", 0), ("i8", 0.0), ("i8", 1.0), ("i8", 1e6)])
+@pytest.mark.parametrize("v_size", [1, 1e-5])
+@pytest.mark.parametrize("strength", [1, 3, 8])
+def test_row_of_zeros_with_all_the_weight(capi, kv, scale, v_size, strength):
+    """A position whose V is zero (codes of zero with any scale) takes nearly all
+    of every row's weight; what is left keeps its digits."""
+    rng = np.random.default_rng(58)
+    c = T.AttentionCase(rng, kv, [90, 700, 3], [9, 30, 4], 8, 2, 64)
+    c.q = np.abs(c.q)
+    if kv == "i8":
+        c.scales[:, :, 1] *= np.float32(v_size)
+    else:
+        c.pool[:, :, 1] *= np.float32(v_size)
+    for s, length in enumerate(c.lengths):
+        p = np.arange(length)
+        slot = np.concatenate([c.tables[s][p // c.bt].astype(np.int64) * c.bt + p % c.bt, c.slots[c.cu[s]:c.cu[s + 1]]])
+        v = c.pool[slot // c.bt, 1, 1, :, slot % c.bt].astype(np.float64)
+        if kv == "i8":
+            v = v * c.scales[slot // c.bt, 1, 1, :, slot % c.bt].astype(np.float64)[..., None]
+        c.v[s] = np.moveaxis(v, 1, 0)
+    for s, index in ((0, 5), (1, 3), (1, 699), (2, 1)):
+        set_row(c, s, index, 0, 127 if kv == "i8" else strength, strength / 127)
+        set_row(c, s, index, 1, 0, scale)
+    tree_bounds.check_case(c.upload().run(capi), tree_bounds.rows_and_bound_by_element)

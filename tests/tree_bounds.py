@@ -42,7 +42,10 @@ def rows_and_bound_by_element(q, k, v, mask, group):
     least 2^3 (a tile's scales within 2^6 of one another, two references rounded
     up), where F16 leaves out 2^-25: 2^-28 of the largest weight times row
     maximum (its power of two at most twice it: 2^-27), of either sign, six
-    deviations of sqrt(m) of them."""
+    deviations of sqrt(m) of them.  That largest is taken as no less than 2^-90
+    of the largest weight (the unscaled weights, which are summed, must not
+    overflow): F16's 2^-25 is then 2^-25 2^-11 2^-90, times elements below 2^15:
+    2^-111, of either sign, again six deviations."""
     import torch
     n, heads, d = q.shape
     out, tol = torch.zeros_like(q), torch.zeros_like(q)
@@ -59,7 +62,7 @@ def rows_and_bound_by_element(q, k, v, mask, group):
         row = v_seen.abs().amax(1)
         bound = (w @ v_seen.abs()) * (2 * e + 2.0 ** -22 + 24 * 2.0 ** -23 + 2.0 ** -21) \
             + 2.0 ** -39 * (w @ row)[:, None] \
-            + 6 * seen.sum(1, keepdim=True).sqrt() * 2.0 ** -27 * (w * row).amax(1, keepdim=True) + 1e-37
+            + 6 * seen.sum(1, keepdim=True).sqrt() * (2.0 ** -27 * (w * row).amax(1, keepdim=True) + 2.0 ** -111)
         out[:, g * group:(g + 1) * group] = (w @ v_seen).reshape(n, group, d)
         tol[:, g * group:(g + 1) * group] = bound.masked_fill(~some[:, None], 0.0).reshape(n, group, d)
     return out, tol

@@ -305,7 +305,7 @@ struct TreeMeta {  // at kOffMeta
     };
     alignas(16) unsigned valid[kMetaRing][4];   // columns of a tile that hold a row
     alignas(16) unsigned vspan[kMetaRing][4];   // per load warp: the largest V scale (upper half of its bits, rounded
-                                                // up) and the smallest one that is not zero (rounded down)
+                                                // up) and the smallest one (rounded down; rows that do not exist apart)
     union {
         unsigned vbad[kMetaRing][4];  // nodes whose V (kept out of the products: 0 * inf) is not finite
         struct {                      // while the run is cut out
@@ -946,10 +946,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                     // scale stays below 2^11 and a row keeps the digits of what
                     // it sees, whatever the V of others are: the largest score -
                     // m + log2(V scale).  Where a tile's scales lie within 2^6 of
-                    // one another (zeros apart) its largest score and its largest
-                    // scale together stand for that; elsewhere (a masked node's
-                    // or a single position's V far above the rest) every column
-                    // is looked at.  The weights themselves, which l sums, stay
+                    // one another its largest score and its largest scale together
+                    // stand for that; elsewhere (a masked node's or a single
+                    // position's V far above the rest, a row of zeros with all the
+                    // weight) every column is looked at.  The weights themselves, which l sums, stay
                     // below 2^101.  Both parts are whole, so that a change of
                     // reference costs O and l no digit.
                     const float score = top * c;
@@ -1363,18 +1363,23 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                     unsigned bad_rows = 0;
                     unsigned char* dst = out + row * 128;
                     if constexpr (KV == 2) {
-                        if (is_v) {
-                            float sc = scale_col[row];
-                            const bool bad = node_values && p0 + row >= len && !isfinite(sc);
-                            if (bad) scale_col[row] = sc = 0.f;
-                            bad_rows = __ballot_sync(0xffffffffu, bad);
-                            big = fabsf(sc);
-                            if (big > 0.f) low = big;
-                        }
                         uint4 row_codes[DP / 16];  // all read before any is written: no load waits behind a store
 #pragma unroll
                         for (int i = 0; i < DP / 16; ++i)
                             row_codes[i] = i < chunks ? *reinterpret_cast<const uint4*>(src + ((i ^ swizzle) << 4)) : make_uint4(0, 0, 0, 0);
+                        if (is_v) {
+                            float sc = scale_col[row];
+                            const bool bad = node_values && p0 + row >= len && !isfinite(sc);
+                            bad_rows = __ballot_sync(0xffffffffu, bad);
+                            unsigned any = 0;
+#pragma unroll
+                            for (int i = 0; i < DP / 16; ++i) any |= row_codes[i].x | row_codes[i].y | row_codes[i].z | row_codes[i].w;
+                            // a row of zeros may have any scale (the encoder gives 1): it adds nothing, and is not to be
+                            // what the others' digits are measured by
+                            if (bad || (!any && isfinite(sc))) scale_col[row] = sc = 0.f;
+                            big = fabsf(sc);
+                            if (M.valid[meta][lw] >> lane & 1) low = big;
+                        }
 #pragma unroll
                         for (int i = 0; i < DP / 16; ++i) {
                             const unsigned w[4] = {row_codes[i].x, row_codes[i].y, row_codes[i].z, row_codes[i].w};
@@ -1433,7 +1438,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                             const float f = two_to(up), back = top > 0.f ? two_to(-up) : 0.f;
                             if (lane < kRound) scale_col[row + round] = is_v ? back : back * two_to(-14);
                             big = fmaxf(big, back);
-                            if (back > 0.f) low = fminf(low, back);
+                            if (is_v && (M.valid[meta][(row + round) >> 5] >> ((row + round) & 31) & 1)) low = fminf(low, back);
                             const f32x2 f2 = pair_of(f, f);
 #pragma unroll
                             for (int i = 0; i < 8; i += 2) {
