@@ -197,3 +197,35 @@ def test_row_of_zeros_with_all_the_weight(capi, kv, scale, v_size, strength):
         set_row(c, s, index, 0, 127 if kv == "i8" else strength, strength / 127)
         set_row(c, s, index, 1, 0, scale)
     tree_bounds.check_case(c.upload().run(capi), tree_bounds.rows_and_bound_by_element)
+
+
+@pytest.mark.parametrize("kv", ["f32", "i8"])
+@pytest.mark.parametrize("large", [1e11, 1e18, 1e30])
+@pytest.mark.parametrize("lengths", [[100], [40, 2000], [130, 30], [20000]])
+def test_weight_on_zeros_beside_large_values(capi, kv, large, lengths):
+    """Nodes share the weight but have V zero, and the tiles before hold V of up
+    to 1e30: sums of weights and of products are in units far apart, within a
+    stream, between streams and between the parts of a cut item."""
+    rng = np.random.default_rng(59)
+    c = T.AttentionCase(rng, kv, lengths, [128] * len(lengths), 4, 2, 64, masks="any", q_scale=0.3)
+    for s, length in enumerate(lengths):
+        row = rng.integers(-127, 128, c.d) if kv == "i8" else rng.standard_normal(c.d) * large
+        for index in range(min(length, 300)):
+            set_row(c, s, index, 1, row, large / 100)
+        for node in range(128):
+            set_row(c, s, length + node, 1, 0, 1.0)
+    tree_bounds.check_case(c.upload().run(capi), tree_bounds.rows_and_bound_by_element)
+
+
+@pytest.mark.parametrize("kv", ["f32", "i8"])
+@pytest.mark.parametrize("lengths", [[100], [40, 2000], [20000]])
+def test_values_of_all_sizes(capi, kv, lengths):
+    """V from 1e-18 to 1e18 among positions of like weight."""
+    rng = np.random.default_rng(64)
+    c = T.AttentionCase(rng, kv, lengths, [33] * len(lengths), 4, 2, 64, masks="any", q_scale=0.3)
+    for s, length in enumerate(lengths):
+        for index in range(min(length, 500)):
+            size = 10.0 ** rng.uniform(-18, 18)
+            row = rng.integers(-127, 128, c.d) if kv == "i8" else rng.standard_normal(c.d) * size
+            set_row(c, s, index, 1, row, size / 100)
+    tree_bounds.check_case(c.upload().run(capi), tree_bounds.rows_and_bound_by_element)

@@ -43,9 +43,9 @@ def rows_and_bound_by_element(q, k, v, mask, group):
     up), where F16 leaves out 2^-25: 2^-28 of the largest weight times row
     maximum (its power of two at most twice it: 2^-27), of either sign, six
     deviations of sqrt(m) of them.  That largest is taken as no less than 2^-90
-    of the largest weight (the unscaled weights, which are summed, must not
-    overflow): F16's 2^-25 is then 2^-25 2^-11 2^-90, times elements below 2^15:
-    2^-111, of either sign, again six deviations."""
+    of the largest weight (a little less in fact, so that the sum of unscaled
+    weights does not overflow): F16's 2^-25 is then 2^-25 2^-11 2^-90, times
+    elements below 2^15: 2^-111, of either sign, again six deviations."""
     import torch
     n, heads, d = q.shape
     out, tol = torch.zeros_like(q), torch.zeros_like(q)

@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(kAnyWarps * 32) tree_any_kernel(TreeAttn a) {
 // Work is dealt to one CTA per SM in equal runs of tiles over all items
 // (each CTA scans the lengths and cuts out its run), so ragged batches and a
 // single long sequence fill the device alike; an item cut by a run boundary
-// leaves partial (O, m, l) in the workspace for tree_combine_kernel.
+// leaves partial (O, m, l, m_v) in the workspace for tree_combine_kernel.
 //
 // What bounds it.  A tile of 128 positions costs a stream 32 MMAs of 64
 // cycles (hi and lo of Q, and of P), of which the Q K^T half reads shared
@@ -228,6 +228,7 @@ constexpr int kTreeLoadWarp = 8;
 constexpr unsigned kTreeNap = 2000;                       // ns a wait may sleep at a time
 constexpr unsigned long long kTreeLimit = 4000000000ull;  // ns after which a wait gives up
 constexpr int kTreeRows = 256;      // query vectors of a partial slot
+constexpr int kTreeState = 3;       // and values beside O: m, l, m_v
 constexpr int kPieceRing = 4;
 constexpr int kMetaRing = 8;        // tiles of column masks and int8 scales kept
 
@@ -876,7 +877,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                 }
             }
             float m = -INFINITY, l = 0.f;
-            float m_v = 0.f;  // O and l are in units of 2^(m + m_v): of the scores, and of the V scales
+            float m_v = 0.f;  // l is in units of 2^m, O of 2^(m + m_v)
 #pragma unroll
             for (int i = 0; i < DP; ++i) o[i] = 0.f;
             const int tiles = q.t1 - q.t0;
@@ -949,9 +950,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                     // one another its largest score and its largest scale together
                     // stand for that; elsewhere (a masked node's or a single
                     // position's V far above the rest, a row of zeros with all the
-                    // weight) every column is looked at.  The weights themselves, which l sums, stay
-                    // below 2^101.  Both parts are whole, so that a change of
-                    // reference costs O and l no digit.
+                    // weight) every column is looked at.  The weights themselves stay below 2^119,
+                    // so that a tile's sum does not overflow; l has the first
+                    // part alone as its reference.  Both are whole, so that a
+                    // change of reference costs no digit.
                     const float score = top * c;
                     const float mn = fmaxf(m, KV == 1 ? score : ceilf(score));
                     const bool none = mn == -INFINITY;
@@ -960,7 +962,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                     // less their maximum, go back into S.
                     const bool far = fabsf(mn) >= 4194304.f && !none;
                     bool look = far;
-                    float mv = -90.f, big = 0.f;
+                    float mv = -108.f, big = 0.f;
                     if constexpr (KV != 1) {
                         const uint4 span = *reinterpret_cast<const uint4*>(M.vspan[ring]);
                         big = __uint_as_float(max(max(span.x, span.y), max(span.z, span.w)) & 0xffff0000u);
@@ -972,7 +974,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                     }
                     if (__any_sync(0xffffffffu, look)) {
                         const float back = 1.f / c;
-                        mv = -90.f;
+                        mv = -108.f;
                         float most = -INFINITY;
 #pragma unroll 1
                         for (int k = 0; k < F::kBn / 16; ++k) {
@@ -995,12 +997,14 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                         if (!none) {
                             mv = fmaxf(m_v + (m - mn), ceilf(mv + (score - mn)));
                             off -= mv;
+                            l *= keep;
                             keep = ex2((m - mn) + (m_v - mv));
                             m_v = mv;
                         }
+                    } else {
+                        l *= keep;
                     }
                     m = mn;
-                    l *= keep;
                     // P over S, sixteen positions (one K step of the MMA) at a
                     // time: hi in their first eight columns, lo in the others.
                     f32x2 sums[2] = {0, 0};
@@ -1040,7 +1044,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                     }
                     float sum0, sum1;
                     halves_of(add2(sums[0], sums[1]), sum0, sum1);
-                    l += sum0 + sum1;
+                    l += KV == 1 ? sum0 + sum1 : (sum0 + sum1) * ex2(m_v);
                     tm_wait_st();
                 }
                 tm_before();
@@ -1064,13 +1068,12 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                 }
             }
             if (!go) break;
-            if constexpr (KV != 1) m += m_v;
-            // The part of an item that other CTAs continue: (O, m, l) of each
+            // The part of an item that other CTAs continue: (O, m, l, m_v) of each
             // stream into the workspace, one thread a row, rows side by side.
             // The CTA's slot 1 holds an item that begins here, slot 0 one that
             // began earlier; stream 1 uses the upper half of a slot.
             if (!q.whole && live) {
-                float* slot = partial + (long long)(2 * cta + (q.t0 == 0)) * kTreeRows * (DP + 2);
+                float* slot = partial + (long long)(2 * cta + (q.t0 == 0)) * kTreeRows * (DP + kTreeState);
                 const int pr = stream * 128 + r;
 #pragma unroll
                 for (int i = 0; i < DP / 4; ++i)
@@ -1078,6 +1081,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                         make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                 slot[kTreeRows * DP + pr] = m;
                 slot[kTreeRows * DP + kTreeRows + pr] = l;
+                if constexpr (KV != 1) slot[kTreeRows * DP + 2 * kTreeRows + pr] = m_v;
             }
             if (!q.pair) {
                 // A whole item: the odd tiles' (O, m, l) through stream 1's tensor
@@ -1094,7 +1098,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                             for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(o[16 * k + i]);
                             tm_st16(b_o + 16 * k, x);
                         }
-                        unsigned x[16] = {__float_as_uint(m), __float_as_uint(l)};
+                        unsigned x[16] = {__float_as_uint(m), __float_as_uint(l), __float_as_uint(m_v)};
                         tm_st16(b_ml, x);
                         tm_wait_st();
                     }
@@ -1111,9 +1115,15 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                         tm_ld16(b_ml, ml);
                         const float m2 = __uint_as_float(ml[0]), l2 = __uint_as_float(ml[1]);
                         const float mn = fmaxf(m, m2);
-                        const float ka = mn == -INFINITY ? 0.f : ex2(m - mn), kb = mn == -INFINITY ? 0.f : ex2(m2 - mn);
-                        m = mn;
+                        float ka = mn == -INFINITY ? 0.f : ex2(m - mn), kb = mn == -INFINITY ? 0.f : ex2(m2 - mn);
                         l = l * ka + l2 * kb;
+                        if (KV != 1 && mn != -INFINITY) {
+                            const float va = (m - mn) + m_v, vb = (m2 - mn) + __uint_as_float(ml[2]);
+                            m_v = fmaxf(va, vb);
+                            ka = ex2(va - m_v);
+                            kb = ex2(vb - m_v);
+                        }
+                        m = mn;
                         const f32x2 ka2 = pair_of(ka, ka), kb2 = pair_of(kb, kb);
 #pragma unroll
                         for (int k = 0; k < DP / 32; ++k) {
@@ -1143,7 +1153,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                 const auto stage = [&](int row, int ch) {
                     return reinterpret_cast<float4*>(tile + (ch >> 3) * 16384 + row * 128 + (((ch & 7) ^ (row & 7)) << 4));
                 };
-                const float f = m == -INFINITY && l == 0.f ? 0.f : 1.f / l;
+                const float f = m == -INFINITY && l == 0.f ? 0.f : KV == 1 ? 1.f / l : ex2(m_v) / l;
 #pragma unroll
                 for (int i = 0; i < DP / 4; ++i)  // lane is the row
                     *stage(lane, i) = make_float4(o[4 * i] * f, o[4 * i + 1] * f, o[4 * i + 2] * f, o[4 * i + 3] * f);
@@ -1711,7 +1721,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
 // over the pieces in order (a fixed order, so results repeat bit for bit).
 // Block (b, y) takes rows 32 y .. 32 y + 31 of the item that starts in CTA b:
 // columns 32 z .. 32 z + 31: lanes are rows, warps groups of four columns.
-template <int DP>
+// With V scales (kScaled) O_i is in units of 2^(m_i + v_i), l_i of 2^m_i.
+template <int DP, bool kScaled>
 __global__ void __launch_bounds__(256) tree_combine_kernel(TreeAttn a, const float* partial, const TreeRec* recs) {
     __shared__ float4 stage[32][9];
     asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the tiles are still being worked on
@@ -1724,15 +1735,18 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(TreeAttn a, const flo
     const auto slot_of = [&](int i, int& at) {  // part i: its slot, and the row's place in it
         const int piece = rec.streams == 2 ? i >> 1 : i;
         at = rec.streams == 2 ? (i & 1) * 128 + pr : pr;
-        return partial + (2ll * (int(blockIdx.x) + piece) + (piece == 0)) * kTreeRows * (DP + 2);
+        return partial + (2ll * (int(blockIdx.x) + piece) + (piece == 0)) * kTreeRows * (DP + kTreeState);
     };
-    float top = -INFINITY;
+    float top = -INFINITY, top_v = -INFINITY;
 #pragma unroll 4
     for (int i = 0; i < parts; ++i) {
         int at;
         const float* slot = slot_of(i, at);
-        top = fmaxf(top, slot[kTreeRows * DP + at]);
+        const float m = slot[kTreeRows * DP + at];
+        top = fmaxf(top, m);
+        if constexpr (kScaled) top_v = fmaxf(top_v, m + slot[kTreeRows * DP + 2 * kTreeRows + at]);
     }
+    if (kScaled && top != -INFINITY) top_v -= top;  // O's reference beyond l's: any near the largest will do
     float l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
@@ -1740,15 +1754,18 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(TreeAttn a, const flo
         int at;
         const float* slot = slot_of(i, at);
         // nothing seen (or nothing but NaN scores): the sums decide
-        const float f = top == -INFINITY ? 1.f : ex2(slot[kTreeRows * DP + at] - top);
+        const float down = slot[kTreeRows * DP + at] - top;
+        float f = top == -INFINITY ? 1.f : ex2(down);
         const float4 x = *reinterpret_cast<const float4*>(slot + (group4 * kTreeRows + at) * 4);
         l += slot[kTreeRows * DP + kTreeRows + at] * f;
+        if (kScaled && top != -INFINITY) f = ex2(down + slot[kTreeRows * DP + 2 * kTreeRows + at] - top_v);
         o.x += x.x * f;
         o.y += x.y * f;
         o.z += x.z * f;
         o.w += x.w * f;
     }
-    const float f = l == 0.f && top == -INFINITY ? 0.f : 1.f / l;
+    float f = l == 0.f && top == -INFINITY ? 0.f : 1.f / l;
+    if (kScaled && top != -INFINITY) f = ex2(top_v) / l;
     stage[lane][warp] = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
     __syncthreads();
     // eight lanes write a row's 32 columns
@@ -1810,7 +1827,7 @@ void run_tree_mma(const TreeAttn& a, void* workspace, cudaStream_t s) {
     early.val.programmaticStreamSerializationAllowed = 1;
     config.attrs = &early;
     config.numAttrs = 1;
-    TVARA_CUDA(cudaLaunchKernelEx(&config, tree_combine_kernel<DP>, a, static_cast<const float*>(partial),
+    TVARA_CUDA(cudaLaunchKernelEx(&config, tree_combine_kernel<DP, KV != 1>, a, static_cast<const float*>(partial),
                                   static_cast<const TreeRec*>(recs)));
     TVARA_LAUNCHED();
 }
@@ -1828,7 +1845,7 @@ bool tree_mma_takes(const TreeAttn& a) {
 std::size_t tree_attention_workspace(const TreeAttn& a) {
     static_assert(sizeof(TreeRec) * kTreeMaxCtas <= kTreeRecBytes);
     const int dp = a.dim <= 64 ? 64 : 128;
-    return a.dim <= 128 ? kTreeRecBytes + std::size_t(2) * kTreeMaxCtas * kTreeRows * (dp + 2) * 4 : 256;
+    return a.dim <= 128 ? kTreeRecBytes + std::size_t(2) * kTreeMaxCtas * kTreeRows * (dp + kTreeState) * 4 : 256;
 }
 
 void launch_tree_attention(const TreeAttn& a, void* workspace, cudaStream_t s) {
