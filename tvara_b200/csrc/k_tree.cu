@@ -20,8 +20,10 @@ namespace {
 //
 // Bound by latency, not bytes: a launch, one read of the lengths, the scan, a
 // search and, for trees, the walk up in shared memory.  One tree of 26 nodes
-// 7.6 us a call, 500 trees of up to 63 nodes 8.0 us, 511 prompts of up to 2,047
-// rows (6.3 MB) 10.2 us.  (Summing all needs with one contended shared-memory
+// 7.5 us a call, 500 trees of up to 63 nodes 7.8 us, 511 prompts of up to 2,047
+// rows (6.3 MB) 10.2 us.  Counts in place (held_out = held or free_left =
+// free_count) take a second launch of one CTA, once no CTA reads them any more:
+// 10.4 and 11.7 us for the first two.  (Summing all needs with one contended shared-memory
 // atomic cost 12 us; a thread per prompt row instead of four, another 8 us.)
 constexpr int kPlanThreads = 512;
 constexpr int kPlanRun = 4;  // consecutive rows a thread takes when there are no trees
@@ -193,9 +195,10 @@ __global__ void __launch_bounds__(kPlanThreads) tree_plan_kernel(TreePlan a, int
 // or the rows coincide, and a batch is read before it is written, so
 // ascending batches never read a row that was overwritten.
 //
-// 48 sequences, 32 layers of 8 heads of 128 F16: 34 MB in 12.3 us (5.3 us at
-// the copy bandwidth); one sequence 6.6 us, a launch and four dependent
-// fetches.  Slices of one sequence beyond those that run at the same time only
+// 48 sequences, 32 layers of 8 heads of 128 F16: 34 MB in 14.3 us (5.3 us at
+// the copy bandwidth; in a loop over two inputs 12.2, and 10.3 in place); one
+// sequence 7.2 us, a launch and four dependent fetches.  next over first with several slices takes a second launch
+// for the answers: 2 to 3.5 us more.  Slices of one sequence beyond those that run at the same time only
 // repeat the walk (1,536 instead of 864 CTAs: 16.4 us).
 constexpr int kCommitThreads = 256;
 constexpr int kCommitRows = 8;

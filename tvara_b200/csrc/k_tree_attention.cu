@@ -64,8 +64,11 @@ __device__ __forceinline__ long long tree_row(const TreeAttn& a, int s, int c0, 
 // One CTA of four warps per (row, query head), positions dealt to the warps,
 // online softmax in F32, merged through shared memory.  Each position's K is
 // reduced across the warp, so this form is bound by those shuffles (a few
-// percent of memory bandwidth); it serves the shapes that the tensor-core
-// form does not take (launch_tree_attention).
+// percent of memory bandwidth), and every row and head reads K and V again; it
+// serves the shapes that the tensor-core form does not take
+// (launch_tree_attention).  26 nodes on 1,900 positions: 16/4 heads of 256 F16
+// 522 us, int8 823, F32 668 (16 such sequences 4.2, 6.1, 6.6 ms); 32/8 heads of
+// 128 F16 with query rows off 16 bytes 447 us, where aligned ones take 29.
 constexpr int kAnyWarps = 4;
 
 __device__ __forceinline__ float kv_value(const TreeAttn& a, long long at) {
@@ -189,9 +192,10 @@ __global__ void __launch_bounds__(kAnyWarps * 32) tree_any_kernel(TreeAttn a) {
 // tile (the small lo products first) and the long sum over tiles is rounded
 // to nearest in registers; that costs one fused multiply-add per element.
 // F32 results from F16 operands: Q, P (and K, V of F32 pools) enter as hi +
-// lo F16 pairs of 22 bits, int8 codes are exact in F16; the scales of int8
-// rows, and the powers of two that bring F32 rows below 2^15, are applied to
-// the columns of S and to P.
+// lo F16 pairs that carry 2^-23 of each value, int8 codes are exact in F16; the
+// scales of int8 rows, and the powers of two that bring F32 rows below 2^15,
+// are applied to the columns of S and to P.  With such scales O has a reference
+// of its own, 2^(m + m_v), m_v from the V scales that a row sees.
 //
 // Two softmax warpgroups ("streams") keep the tensor core busy: with one M
 // tile they take the even and the odd tiles of the same item, each with its
@@ -211,13 +215,13 @@ __global__ void __launch_bounds__(kAnyWarps * 32) tree_any_kernel(TreeAttn a) {
 // positions: 560 us sustained, tensor pipe 65% busy).  F16 with one M tile:
 // about 3,200 cycles a tile, 2,835 of HBM; a ragged batch adds some 17,000 to
 // 25,000 cycles an item for Q, the pipeline's ends and the output (64 trees
-// over 200-4,000 positions: 265 us, 35% of the copy bandwidth, tensor pipe
+// over 200-4,000 positions: 262 us, 36% of the copy bandwidth, tensor pipe
 // 49%).  int8 and F32 pools: the conversion warps, whose loads wait behind the
-// MMAs' reads of shared memory (24 sequences int8: 197 us, 206 sustained; 31
-// of the small heads F32: 89 us).  Small calls: instruction fetch; code executed once costs
-// about a nanosecond per three instructions, so loops here stay rolled unless
-// registers force them open (unrolling everything was 181 KB and 3 times
-// slower on the batch).  Register shares of 200/64/48 or 184/96/48 for softmax,
+// MMAs' reads of shared memory (24 sequences int8: 205 us; F32: 31 of the small
+// heads 91 us, 32 of 128 values 146 us).  Small calls: instruction fetch; code
+// executed once costs about a nanosecond per three instructions, so loops here
+// stay rolled unless registers force them open (unrolling everything was 181 KB
+// and 3 times slower on the batch).  Register shares of 200/64/48 or 184/96/48 for softmax,
 // loads and the rest were 2 to 10% slower than 192/72/56.
 constexpr int kTreeThreads = 512;   // WG0, WG1 softmax; WG2 loads; warp 12 issues the MMAs, warp 13 deals
                                     // the pieces, warp 14 fetches the rows that WG2 converts (F32, int8)
@@ -245,7 +249,8 @@ struct TreeForm {  // KV: 0 F32, 1 F16, 2 int8
     static constexpr int kSlotPart = kHalves * kBn * 128;
     static constexpr int kSlot = kParts * kSlotPart;     // one K or V tile
     // an item's own cost (Q, merge, output) in tiles, chosen on ragged batches
-    // of each type (64 trees F16 with 4, 6, 8, 11: 248, 244, 231, 233 us; F32
+    // of each type, before F32 and int8 weights had their present reference (2 to
+    // 3% slower at every choice) (64 trees F16 with 4, 6, 8, 11: 248, 244, 231, 233 us; F32
     // heads of 128 with 4, 7, 9: 32 sequences 152, 141, 139 us, 8 sequences 68,
     // 64, 75; F32 heads of 64 with 3, 4, 7: 31 sequences 88, 86, 93 us, 12
     // sequences 74, 77, 79; int8 with 5, 6, 7: 24 sequences 197, 195, 199 us,
@@ -1448,7 +1453,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                             const float f = two_to(up), back = top > 0.f ? two_to(-up) : 0.f;
                             if (lane < kRound) scale_col[row + round] = is_v ? back : back * two_to(-14);
                             big = fmaxf(big, back);
-                            if (is_v && (M.valid[meta][(row + round) >> 5] >> ((row + round) & 31) & 1)) low = fminf(low, back);
+                            low = fminf(low, back > 0.f || (M.valid[meta][(row + round) >> 5] >> ((row + round) & 31) & 1) ? back : INFINITY);
                             const f32x2 f2 = pair_of(f, f);
 #pragma unroll
                             for (int i = 0; i < 8; i += 2) {
