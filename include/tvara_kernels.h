@@ -218,7 +218,8 @@ TVARA_API int tvara_tree_plan(const tvara_tree_plan_args* args, void* stream);
  * mask; NULL: j <= i, a chain), their K and V at slots[cu_nodes[s] + j].
  * Scores are q.k / sqrt(head_dim), query head h reads KV head
  * h / (heads / kv_heads), arithmetic and outputs are F32 to within rounding
- * for every pool type (as tvara_paged_attention).  A row that attends to
+ * for every pool type (as tvara_paged_attention; F16 pools: weights down to
+ * 2^-36 of a row's largest).  A row that attends to
  * nothing is zero; masked K and V may hold anything, NaN included.  Rows of
  * out may not meet rows of q (column slices of one buffer are fine), and out,
  * workspace and status no other array.  One workspace serves one call at a
