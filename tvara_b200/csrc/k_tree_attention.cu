@@ -249,8 +249,8 @@ struct TreeForm {  // KV: 0 F32, 1 F16, 2 int8
     static constexpr int kSlotPart = kHalves * kBn * 128;
     static constexpr int kSlot = kParts * kSlotPart;     // one K or V tile
     // an item's own cost (Q, merge, output) in tiles, chosen on ragged batches
-    // of each type, before F32 and int8 weights had their present reference (2 to
-    // 3% slower at every choice) (64 trees F16 with 4, 6, 8, 11: 248, 244, 231, 233 us; F32
+    // of each type before F32 and int8 weights had their present reference, which
+    // cost 2 to 3% (64 trees F16 with 4, 6, 8, 11: 248, 244, 231, 233 us; F32
     // heads of 128 with 4, 7, 9: 32 sequences 152, 141, 139 us, 8 sequences 68,
     // 64, 75; F32 heads of 64 with 3, 4, 7: 31 sequences 88, 86, 93 us, 12
     // sequences 74, 77, 79; int8 with 5, 6, 7: 24 sequences 197, 195, 199 us,
@@ -955,10 +955,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_
                     // one another its largest score and its largest scale together
                     // stand for that; elsewhere (a masked node's or a single
                     // position's V far above the rest, a row of zeros with all the
-                    // weight) every column is looked at.  The weights themselves stay below 2^119,
-                    // so that a tile's sum does not overflow; l has the first
-                    // part alone as its reference.  Both are whole, so that a
-                    // change of reference costs no digit.
+                    // weight) every column is looked at.  The weights themselves
+                    // stay below 2^119, so that a tile's sum does not overflow; l
+                    // has the first part alone as its reference.  Both are whole,
+                    // so that a change of reference costs no digit.
                     const float score = top * c;
                     const float mn = fmaxf(m, KV == 1 ? score : ceilf(score));
                     const bool none = mn == -INFINITY;
